@@ -13,6 +13,8 @@ LIB_PATH = os.environ.get("BATCHFIRST_LIB") or os.path.join(_HERE, "libbatchfirs
 
 BF_OK, BF_E_ARG, BF_E_HIP, BF_E_FORMAT, BF_E_NOGPU = 0, -1, -2, -3, -4
 BF_PRECISION_F32, BF_PRECISION_BF16, BF_PRECISION_F32_SPLIT, BF_PRECISION_F32_SPLIT3 = 0, 1, 2, 3
+BF_TYPE_F32, BF_TYPE_BF16, BF_TYPE_F16 = 0, 1, 2
+BF_POLICY_VOCABULARY = 4672
 BF_NOALLOC_MAX_BOARDS = 262144
 BF_SPLIT_BOARDS_DEFAULT = 512
 PRECISIONS = {"f32": BF_PRECISION_F32, "fp32": BF_PRECISION_F32, "float32": BF_PRECISION_F32,
@@ -73,6 +75,15 @@ SIGNATURES = {
     "bf_policy_start_wire_host": (_int, [_vp, _vp, _sz, _vp, _sz]),
     "bf_policy_start_structs_host": (_int, [_vp, _vp, _sz, _vp, _sz]),
     "bf_policy_finish_host": (_int, [_vp, _vp, _vp, _vp, _sz, _sz, _vp]),
+    "bf_policy_loss": (_int, [_vp, _vp, _int, _sz, _vp, _vp, _vp, _vp]),
+    "bf_policy_loss_workspace": (_sz, [_sz]),
+    "bf_policy_loss_grad": (_int, [_vp, _vp, _int, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "bf_policy_move_loss_workspace": (_sz, [_sz]),
+    "bf_policy_move_loss": (_int, [_vp, _vp, _int, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _sz, _vp]),
+    "bf_policy_move_loss_grad": (_int, [_vp, _vp, _int, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "bf_grad_norm_workspace": (_sz, [_vp, _sz]),
+    "bf_global_norm": (_int, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp]),
+    "bf_clip_grad_norm": (_int, [_vp, _vp, _vp, _vp, _sz, _c.c_float, _vp, _vp, _sz, _vp]),
     "bf_packed_t16_bytes": (_sz, []),
     "bf_pack_weights_t16": (_int, [_vp, _sz, _vp, _sz]),
     # debugging aids, not part of the public header

@@ -8,6 +8,7 @@
 #include <cstring>
 #include <mutex>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "../../include/batchfirst.h"
@@ -17,6 +18,7 @@
 #include "bf_layout.h"
 #include "bf_layout_t16.h"
 #include "bf_split.h"
+#include "bf_train.h"
 
 #define BF_HIP(call)                                                                         \
     do {                                                                                     \
@@ -301,6 +303,7 @@ int read_err_flag(Lane* c, hipStream_t s) {
     if (flag) {
         BF_HIP(hipMemsetAsync(c->d_err, 0, sizeof(int), s));
         BF_HIP(hipStreamSynchronize(s));
+        if (flag & 8) return bf::fail(BF_E_FORMAT, "loss input: a target or the move lists are out of range");
         if (flag & 4) return bf::fail(BF_E_FORMAT, "move input: board index, from-square or move filter out of range");
         if (flag & 2) return bf::fail(BF_E_FORMAT, "wire input holds code 15, which is not a piece code");
         return bf::fail(BF_E_FORMAT, "wire input: piece_filters length does not match the popcounts of occupied_bbs");
@@ -950,6 +953,146 @@ extern "C" int bf_policy_check(bf_ctx* c, void* stream) {
     DeviceGuard guard(c->device);
     std::lock_guard<std::mutex> lock(c->policy.mu);
     return read_err_flag(&c->policy, (hipStream_t)stream);
+}
+
+// ---- losses of the move-scoring head, gradient clipping ------------------------------------------
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// What both losses check, with and without gradients; fills in the context's part of the arguments.
+int check_loss(bf_ctx* c, bf::PolicyLossArgs* a, bool grad, size_t workspace_bytes, const char* who) {
+    if (int r = check_common(c, a->n, who)) return r;
+    if (a->type != BF_TYPE_F32 && a->type != BF_TYPE_BF16 && a->type != BF_TYPE_F16)
+        return bf::fail(BF_E_ARG, "%s: unknown element type %d", who, a->type);
+    if (grad && !a->loss && !a->d_features && !a->d_kernel) return bf::fail(BF_E_ARG, "%s: no output asked for", who);
+    if (a->n && (!a->features || !a->kernel || !a->targets || (!grad && !a->loss) || (grad && !a->weights)))
+        return bf::fail(BF_E_ARG, "%s: null pointer", who);
+    if (a->n && grad && a->n_weights != 1 && a->n_weights != a->n)
+        return bf::fail(BF_E_ARG, "%s: %zu weights for %zu boards", who, a->n_weights, a->n);
+    if (!aligned16(a->features) || !aligned16(a->kernel) || !aligned16(a->d_features) || !aligned16(a->d_kernel) || !aligned16(a->workspace))
+        return bf::fail(BF_E_ARG, "%s: features, kernels, gradients and the workspace must be 16-byte aligned", who);
+    if (a->per_board || a->n_moves) {
+        if (a->n_moves > ((size_t)1 << 31)) return bf::fail(BF_E_ARG, "%s: %zu moves exceeds the limit of 2^31", who, a->n_moves);
+        if (a->n_moves && (!a->from || !a->filter)) return bf::fail(BF_E_ARG, "%s: null pointer", who);
+        if (a->n == 0 && a->n_moves) return bf::fail(BF_E_ARG, "%s: moves given without boards", who);
+    }
+    const size_t need = bf::policy_loss_workspace(a->n, a->per_board != nullptr, a->d_kernel != nullptr);
+    if (workspace_bytes < need || (need && !a->workspace))
+        return bf::fail(BF_E_ARG, "%s: the workspace has %zu bytes, %zu are needed", who, a->workspace ? workspace_bytes : 0, need);
+    a->err = c->policy.d_err;
+    return BF_OK;
+}
+
+int run_loss(bf_ctx* c, const bf::PolicyLossArgs& a, void* stream) {
+    if (a.n == 0 && !a.d_kernel) return BF_OK;
+    DeviceGuard guard(c->device);
+    BF_HIP(bf::launch_policy_loss(a, (hipStream_t)stream));
+    return BF_OK;
+}
+
+int check_norm(const bf_ctx* c, const void* const* ptrs, const size_t* counts, const int* types, size_t n, const float* d_norm,
+               const void* workspace, size_t workspace_bytes, const char* who) {
+    if (!c) return bf::fail(BF_E_ARG, "%s: null context", who);
+    if (!d_norm || !workspace || (n && (!ptrs || !counts || !types))) return bf::fail(BF_E_ARG, "%s: null pointer", who);
+    for (size_t i = 0; i < n; ++i) {
+        if (types[i] != BF_TYPE_F32 && types[i] != BF_TYPE_BF16 && types[i] != BF_TYPE_F16)
+            return bf::fail(BF_E_ARG, "%s: tensor %zu has unknown element type %d", who, i, types[i]);
+        if (!counts[i]) continue;
+        if (counts[i] > ((size_t)1 << 40)) return bf::fail(BF_E_ARG, "%s: tensor %zu has %zu elements, more than 2^40", who, i, counts[i]);
+        if (!ptrs[i]) return bf::fail(BF_E_ARG, "%s: tensor %zu is a null pointer", who, i);
+        if (reinterpret_cast<uintptr_t>(ptrs[i]) & (types[i] == BF_TYPE_F32 ? 3u : 1u))
+            return bf::fail(BF_E_ARG, "%s: tensor %zu is not aligned to its elements", who, i);
+    }
+    if (!aligned16(workspace)) return bf::fail(BF_E_ARG, "%s: the workspace must be 16-byte aligned", who);
+    const size_t need = bf::grad_norm_workspace(counts, n);
+    if (workspace_bytes < need) return bf::fail(BF_E_ARG, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, need);
+    return BF_OK;
+}
+
+}  // namespace
+
+extern "C" size_t bf_policy_loss_workspace(size_t n) { return bf::policy_loss_workspace(n, false, true); }
+extern "C" size_t bf_policy_move_loss_workspace(size_t n) { return bf::policy_loss_workspace(n, true, true); }
+
+extern "C" int bf_policy_loss(bf_ctx* c, const void* d_features, int type, size_t n, const void* d_kernel, const int64_t* d_targets,
+                              float* d_loss, void* stream) {
+    bf::PolicyLossArgs a{};
+    a.features = d_features, a.type = type, a.n = n, a.kernel = d_kernel, a.targets = d_targets, a.loss = d_loss;
+    if (int r = check_loss(c, &a, false, 0, "bf_policy_loss")) return r;
+    return run_loss(c, a, stream);
+}
+
+extern "C" int bf_policy_loss_grad(bf_ctx* c, const void* d_features, int type, size_t n, const void* d_kernel, const int64_t* d_targets,
+                                   const float* d_weights, size_t n_weights, float* d_loss, void* d_features_grad, void* d_kernel_grad,
+                                   void* d_workspace, size_t workspace_bytes, void* stream) {
+    bf::PolicyLossArgs a{};
+    a.features = d_features, a.type = type, a.n = n, a.kernel = d_kernel, a.targets = d_targets, a.loss = d_loss;
+    a.weights = d_weights, a.n_weights = n_weights, a.d_features = d_features_grad, a.d_kernel = d_kernel_grad, a.workspace = d_workspace;
+    if (int r = check_loss(c, &a, true, workspace_bytes, "bf_policy_loss_grad")) return r;
+    return run_loss(c, a, stream);
+}
+
+extern "C" int bf_policy_move_loss(bf_ctx* c, const void* d_features, int type, size_t n, const void* d_kernel, const uint8_t* d_from,
+                                   const uint8_t* d_filter, const uint8_t* d_per_board, size_t n_moves, const int64_t* d_targets,
+                                   float* d_loss, void* d_workspace, size_t workspace_bytes, void* stream) {
+    bf::PolicyLossArgs a{};
+    a.features = d_features, a.type = type, a.n = n, a.kernel = d_kernel, a.targets = d_targets, a.loss = d_loss;
+    a.from = d_from, a.filter = d_filter, a.per_board = d_per_board, a.n_moves = n_moves, a.workspace = d_workspace;
+    if (n && !d_per_board) return bf::fail(BF_E_ARG, "bf_policy_move_loss: null pointer");
+    if (int r = check_loss(c, &a, false, workspace_bytes, "bf_policy_move_loss")) return r;
+    return run_loss(c, a, stream);
+}
+
+extern "C" int bf_policy_move_loss_grad(bf_ctx* c, const void* d_features, int type, size_t n, const void* d_kernel, const uint8_t* d_from,
+                                        const uint8_t* d_filter, const uint8_t* d_per_board, size_t n_moves, const int64_t* d_targets,
+                                        const float* d_weights, size_t n_weights, float* d_loss, void* d_features_grad,
+                                        void* d_kernel_grad, void* d_workspace, size_t workspace_bytes, void* stream) {
+    bf::PolicyLossArgs a{};
+    a.features = d_features, a.type = type, a.n = n, a.kernel = d_kernel, a.targets = d_targets, a.loss = d_loss;
+    a.from = d_from, a.filter = d_filter, a.per_board = d_per_board, a.n_moves = n_moves, a.workspace = d_workspace;
+    a.weights = d_weights, a.n_weights = n_weights, a.d_features = d_features_grad, a.d_kernel = d_kernel_grad;
+    if (n && !d_per_board) return bf::fail(BF_E_ARG, "bf_policy_move_loss_grad: null pointer");
+    if (int r = check_loss(c, &a, true, workspace_bytes, "bf_policy_move_loss_grad")) return r;
+    return run_loss(c, a, stream);
+}
+
+extern "C" size_t bf_grad_norm_workspace(const size_t* h_counts, size_t n_tensors) {
+    return bf::grad_norm_workspace(h_counts, h_counts ? n_tensors : 0);
+}
+
+extern "C" int bf_global_norm(bf_ctx* c, const void* const* h_tensors, const size_t* h_counts, const int* h_types, size_t n_tensors,
+                              float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int r = check_norm(c, h_tensors, h_counts, h_types, n_tensors, d_norm, d_workspace, workspace_bytes, "bf_global_norm")) return r;
+    DeviceGuard guard(c->device);
+    BF_HIP(bf::launch_grad_norm(const_cast<void* const*>(h_tensors), h_counts, h_types, n_tensors, false, 0.0f, d_norm, d_workspace,
+                                (hipStream_t)stream));
+    return BF_OK;
+}
+
+extern "C" int bf_clip_grad_norm(bf_ctx* c, void* const* h_tensors, const size_t* h_counts, const int* h_types, size_t n_tensors,
+                                 float max_norm, float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int r = check_norm(c, h_tensors, h_counts, h_types, n_tensors, d_norm, d_workspace, workspace_bytes, "bf_clip_grad_norm")) return r;
+    if (!(max_norm >= 0.0f)) return bf::fail(BF_E_ARG, "bf_clip_grad_norm: max_norm must be a number >= 0");
+    try {
+        std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+        spans.reserve(n_tensors);
+        for (size_t i = 0; i < n_tensors; ++i)
+            if (h_counts[i]) {
+                const uintptr_t at = reinterpret_cast<uintptr_t>(h_tensors[i]);
+                spans.emplace_back(at, at + h_counts[i] * (h_types[i] == BF_TYPE_F32 ? 4u : 2u));
+            }
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i].first < spans[i - 1].second)
+                return bf::fail(BF_E_ARG, "bf_clip_grad_norm: two of the tensors overlap");
+    } catch (const std::bad_alloc&) {
+        return bf::fail(BF_E_ARG, "bf_clip_grad_norm: out of host memory for %zu tensors", n_tensors);
+    }
+    DeviceGuard guard(c->device);
+    BF_HIP(bf::launch_grad_norm(h_tensors, h_counts, h_types, n_tensors, true, max_norm, d_norm, d_workspace, (hipStream_t)stream));
+    return BF_OK;
 }
 
 namespace {

@@ -287,6 +287,66 @@ int bf_multi_policy_start_structs_host(bf_multi* m, const void* h_structs, size_
 int bf_multi_policy_finish_host(bf_multi* m, const uint8_t* h_from_square, const uint8_t* h_move_filter,
                                 const uint8_t* h_moves_per_board, size_t n_boards, size_t n_moves, float* h_scores);
 
+/* ---- losses of the move-scoring head, their gradients, and gradient clipping --------------------
+ *
+ * What training or checking the head needs beside its scores.  The reference trains with TensorFlow's losses and
+ * optimisers, outside the inference graph: no counterpart on its evaluation path.
+ *
+ * Features are [n][32][64] as the bf_policy_features_* calls leave them, the logit kernel [32][73] as in the weight blob,
+ * both of one type (BF_TYPE_*).  The logits of a board's move vocabulary (index = move_filter * 64 + from_square) are
+ * l[filter][square] = sum over channels of kernel[channel][filter] * features[channel][square]; they are never written
+ * out.  Logits, softmax sums and the sums of the gradients are float32 or wider; a gradient has its input's type.
+ * All pointers but bf_global_norm's and bf_clip_grad_norm's tables are device pointers on the context's GPU.  Tensors
+ * and workspaces need 16-byte alignment.  The calls allocate nothing, read nothing back, enqueue kernels only (so they
+ * can be captured into a graph) and give the same bits for the same inputs.  A workspace belongs to one call at a time:
+ * calls that may overlap, or graphs whose replays may, need one each. */
+enum { BF_TYPE_F32 = 0, BF_TYPE_BF16 = 1, BF_TYPE_F16 = 2 };
+#define BF_POLICY_VOCABULARY 4672u /* 73 filters x 64 squares */
+
+/* Softmax cross entropy of one target a board over the whole vocabulary: d_loss[b] = log sum exp l - l[target].
+ * target -1: the board has none; its loss is 0.  A target outside [-1, 4671] counts as -1 and is reported by
+ * bf_policy_check(). */
+int bf_policy_loss(bf_ctx* ctx, const void* d_features, int type, size_t n, const void* d_logit_kernel,
+                   const int64_t* d_targets, float* d_loss, void* stream);
+
+/* The same with the gradients of sum_b weights[b] * loss[b], in one pass over the features.  d_weights holds n_weights
+ * floats: n, or one for all boards.  d_loss, d_features_grad and d_kernel_grad may be NULL (not wanted), not all three.
+ * A board without a target leaves zeros in its rows of d_features_grad, whatever its features hold.
+ * d_workspace: bf_policy_loss_workspace(n) bytes. */
+size_t bf_policy_loss_workspace(size_t n);
+int bf_policy_loss_grad(bf_ctx* ctx, const void* d_features, int type, size_t n, const void* d_logit_kernel,
+                        const int64_t* d_targets, const float* d_weights, size_t n_weights, float* d_loss,
+                        void* d_features_grad, void* d_kernel_grad, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* The two calls with the softmax over each board's own list of moves, as bf_policy_finish_host takes them:
+ * d_from_square and d_move_filter uint8 [n_moves], boards back to back, d_moves_per_board uint8 [n].  A target is a place
+ * in the board's own list, or -1; a board with no moves has none.  A move listed twice counts twice.  Out-of-range
+ * squares and filters are clamped, targets beyond the list count as -1, moves beyond n_moves are absent; each of these,
+ * and a sum of d_moves_per_board other than n_moves, is reported by bf_policy_check().
+ * d_workspace: bf_policy_move_loss_workspace(n) bytes, for both. */
+size_t bf_policy_move_loss_workspace(size_t n);
+int bf_policy_move_loss(bf_ctx* ctx, const void* d_features, int type, size_t n, const void* d_logit_kernel,
+                        const uint8_t* d_from_square, const uint8_t* d_move_filter, const uint8_t* d_moves_per_board,
+                        size_t n_moves, const int64_t* d_targets, float* d_loss, void* d_workspace, size_t workspace_bytes,
+                        void* stream);
+int bf_policy_move_loss_grad(bf_ctx* ctx, const void* d_features, int type, size_t n, const void* d_logit_kernel,
+                             const uint8_t* d_from_square, const uint8_t* d_move_filter, const uint8_t* d_moves_per_board,
+                             size_t n_moves, const int64_t* d_targets, const float* d_weights, size_t n_weights, float* d_loss,
+                             void* d_features_grad, void* d_kernel_grad, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* *d_norm = sqrt of the sum of squares over n_tensors tensors: h_tensors holds their device pointers, h_counts their
+ * element counts (0 is allowed, its pointer is then not read), h_types their BF_TYPE_*; host arrays, read before the
+ * call returns.  Each tensor is one contiguous range, aligned to its element.  Squares are summed in float64.
+ * d_workspace: bf_grad_norm_workspace(h_counts, n_tensors) bytes. */
+size_t bf_grad_norm_workspace(const size_t* h_counts, size_t n_tensors);
+int bf_global_norm(bf_ctx* ctx, const void* const* h_tensors, const size_t* h_counts, const int* h_types, size_t n_tensors,
+                   float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* The same, and then every element times min(1, max_norm / (norm + 1e-6)), in place: a norm of infinity makes the factor
+ * 0, one of NaN makes it NaN.  Tensors that overlap are refused (an element would be scaled twice). */
+int bf_clip_grad_norm(bf_ctx* ctx, void* const* h_tensors, const size_t* h_counts, const int* h_types, size_t n_tensors,
+                      float max_norm, float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* ---- host-only helpers (no GPU needed) ----------------------------------------------- */
 
 /* The host encoder itself, for callers that still want the wire format:

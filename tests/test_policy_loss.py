@@ -1,0 +1,515 @@
+"""Softmax cross entropy of the move-scoring head and its gradients (ops.policy_loss, ops.policy_move_loss) against the
+definitions in float64 (oracle/losses.py).
+
+Tolerances, with u = 2^-24 (half a step of float32), eps(t) / 2 half a step of the output's type t:
+  a logit adds 32 products in float32:  dl = 40 u logit_size  (32 sums, the products, what splitting into bf16 terms drops)
+  a loss is log(z) + top - l[target]:   2 dl + 16 u (1 + loss + top)
+  a probability exp(l - top) / z:       relative 2 dl + u (2 spread + 100)     (exp's argument, z's sum in at most 90 steps)
+  a gradient adds 73 (features) or 64 a board (kernel, at most 8 boards a partial sum) products of these, and is rounded
+  once:                                 (2 dl + u (2 spread + 100) + u k + split) size + eps(t) / 2 |value|,  k = 80 / 600,
+                                        split = 2^-17 where the probabilities travel as two bf16 terms (16-bit types)
+  A probability below float32's smallest normal number 2^-126, or a bf16 term of one, may be flushed to zero: up to three
+  flushes a product, 3 * 2^-126 * weight * |factor|, summed over the 73 filters / the boards' 64 squares.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from batch_first_amd import _lib
+from oracle import losses
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+ids = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}.get
+gpu = pytest.mark.gpu
+
+
+def moves_for(n, rng, longest=60, empty=0.1):
+    per = rng.integers(1, longest + 1, n)
+    per[rng.random(n) < empty] = 0
+    m = int(per.sum())
+    return (rng.integers(0, 64, m).astype(np.uint8), rng.integers(0, 73, m).astype(np.uint8), per.astype(np.uint8))
+
+
+def make(n, dtype, seed=0, moves=False, longest=60, scale=1.0):
+    """Host inputs as a dict: features and kernel in `dtype`."""
+    rng = np.random.default_rng(seed)
+    x = torch.from_numpy(np.maximum(rng.standard_normal((n, 32, 8, 8)), 0).astype(np.float32) * np.float32(scale)).to(dtype)
+    k = torch.from_numpy((rng.standard_normal((32, 73)) * 0.28).astype(np.float32)).to(dtype)
+    case = {"x": x, "k": k, "w": torch.from_numpy(rng.uniform(0.1, 1.0, n).astype(np.float32)), "moves": None}
+    if moves:
+        case["moves"] = moves_for(n, rng, longest)
+        per = case["moves"][2].astype(np.int64)
+        t = np.where(per > 0, (rng.random(n) * per).astype(np.int64), -1)
+    else:
+        t = rng.integers(0, 4672, n)
+    t[rng.random(n) < 0.1] = -1
+    case["t"] = torch.from_numpy(t)
+    return case
+
+
+def reference(case, weights=None):
+    w = case["w"] if weights is None else weights
+    return losses.policy_loss(case["x"].double().numpy(), case["k"].double().numpy(), case["t"].numpy(),
+                              np.broadcast_to(w.double().numpy(), len(case["t"])), case["moves"])
+
+
+def limits(ref, case):
+    """(loss, d_features, d_kernel) tolerances."""
+    dtype = case["x"].dtype
+    flush = 3 * 2.0 ** -126 * float(case["w"].max())
+    dl = 40 * U * ref["logit_size"]
+    p = 2 * dl + U * (2 * ref["spread"] + 100)
+    split = 0.0 if dtype == torch.float32 else 2.0 ** -17
+    half, least = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    return (2 * dl + 16 * U * (1 + np.abs(ref["loss"]) + ref["top"]),
+            (p[:, None, None] + U * 80 + split) * ref["d_features_size"] + half * np.abs(ref["d_features"]) + least
+            + flush * 73 * float(case["k"].abs().max()),
+            (p.max(initial=0.0) + U * 600 + split) * ref["d_kernel_size"] + half * np.abs(ref["d_kernel"]) + least
+            + flush * 64 * len(case["t"]) * float(case["x"].nan_to_num().abs().max()))
+
+
+def close(got, want, tol, what):
+    got = got.double().cpu().numpy().reshape(want.shape)
+    off = np.abs(got - want) - tol
+    assert np.all(off <= 0), "%s: off by %g over the tolerance at %s" % (what, off.max(), np.unravel_index(off.argmax(), off.shape))
+
+
+# ---- without a GPU ---------------------------------------------------------------------------------------------------
+
+def test_oracle_gradients_are_the_differences_of_its_losses():
+    rng = np.random.default_rng(3)
+    for moves in (False, True):
+        case = make(4, torch.float32, 5, moves=moves)
+        ref = reference(case)
+
+        def total(x, k):
+            r = losses.policy_loss(x, k, case["t"].numpy(), case["w"].numpy(), case["moves"])
+            return float((r["loss"] * case["w"].double().numpy()).sum())
+
+        x, k = case["x"].double().numpy().reshape(4, 32, 64), case["k"].double().numpy()
+        dx, dk = rng.standard_normal(x.shape), rng.standard_normal(k.shape)
+        h = 1e-5
+        diff = (total(x + h * dx, k + h * dk) - total(x - h * dx, k - h * dk)) / (2 * h)
+        # the third difference is below 100 here and the loss is known to 1e-14: h^2 * 100 / 6 + 1e-14 / h
+        assert abs(diff - (ref["d_features"] * dx).sum() - (ref["d_kernel"] * dk).sum()) < 1e-8
+
+
+def _fake_context():
+    """Memory that stands for a context: the checks look at nothing in it, and every call here is refused by them."""
+    return ctypes.cast(ctypes.create_string_buffer(1 << 16), ctypes.c_void_p)
+
+
+def test_refusals_of_the_c_entry_points():
+    lib, ctx = _lib.load(), _fake_context()
+    buf = ctypes.create_string_buffer(1 << 16)
+    p = (ctypes.addressof(buf) + 255) & ~255
+    big = lib.bf_policy_move_loss_workspace(2)
+
+    def refused(rc, text):
+        assert rc == _lib.BF_E_ARG and text in lib.bf_last_error().decode(), lib.bf_last_error()
+
+    def loss(ctx=ctx, x=p, type_=0, n=2, k=p, t=p, out=p):
+        return lib.bf_policy_loss(ctx, x, type_, n, k, t, out, None)
+
+    refused(loss(ctx=None), "null context")
+    refused(loss(type_=3), "element type 3")
+    refused(loss(n=(1 << 26) + 1), "exceeds the limit")
+    for name in ("x", "k", "t", "out"):
+        refused(loss(**{name: None}), "null pointer")
+    refused(loss(x=p + 4), "aligned")
+    refused(loss(k=p + 8), "aligned")
+    assert loss(n=0, x=None, k=None, t=None, out=p) == 0
+
+    def grad(n=2, w=p, nw=2, out=p, dx=p, dk=p, ws=p, size=big):
+        return lib.bf_policy_loss_grad(ctx, p, 0, n, p, p, w, nw, out, dx, dk, ws, size, None)
+
+    refused(grad(w=None), "null pointer")
+    refused(grad(nw=3), "3 weights for 2 boards")
+    refused(grad(nw=0), "0 weights")
+    refused(grad(out=None, dx=None, dk=None), "no output")
+    refused(grad(dx=p + 2), "aligned")
+    refused(grad(ws=p + 8), "aligned")
+    refused(grad(size=lib.bf_policy_loss_workspace(2) - 1), "workspace")
+    refused(grad(ws=None), "workspace")
+
+    def moves(n=2, frm=p, flt=p, per=p, m=4, ws=p, size=big):
+        return lib.bf_policy_move_loss(ctx, p, 0, n, p, frm, flt, per, m, p, p, ws, size, None)
+
+    refused(moves(frm=None), "null pointer")
+    refused(moves(flt=None), "null pointer")
+    refused(moves(per=None), "null pointer")
+    refused(moves(m=(1 << 31) + 1), "2^31")
+    refused(moves(n=0, per=None), "moves given without boards")
+    refused(moves(size=0), "workspace")
+    refused(lib.bf_policy_move_loss_grad(ctx, p, 0, 2, p, p, p, p, 4, p, p, 2, p, p, p, p, lib.bf_policy_move_loss_workspace(2) - 1, None),
+            "workspace")
+
+
+def test_ops_refuse_host_tensors_and_unknown_contexts():
+    from batch_first_amd import ops
+    x, k, t = torch.zeros(2, 32, 8, 8), torch.zeros(32, 73), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="unknown batchfirst context"):
+        torch.ops.batchfirst.policy_loss(1, x, k, t)
+    with pytest.raises(ValueError, match="device tensor"):
+        ops._head(None, x, k, t)
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        ops._head(None, x.double(), k, t)
+
+
+# ---- on the GPU ------------------------------------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def ctx():
+    from batch_first_amd import ops, weights
+    c = ops.DeviceContext(weights.make_weights(seed=7))
+    yield c
+    c.close()
+
+
+def on_gpu(case):
+    out = {k: v.cuda() for k, v in case.items() if torch.is_tensor(v)}
+    out["lists"] = () if case["moves"] is None else tuple(torch.from_numpy(a).cuda() for a in case["moves"])
+    return out
+
+
+def call(ctx, d, **kw):
+    """(loss, d_features, d_kernel) of the one-pass form."""
+    o = torch.ops.batchfirst
+    op = o.policy_move_loss_grad if d["lists"] else o.policy_loss_grad
+    return op(ctx.handle, d["x"], d["k"], *d["lists"], d["t"], d["w"], **kw)
+
+
+def forward(ctx, d):
+    o = torch.ops.batchfirst
+    op = o.policy_move_loss if d["lists"] else o.policy_loss
+    return op(ctx.handle, d["x"], d["k"], *d["lists"], d["t"])
+
+
+def check_all(ctx, case):
+    ref = reference(case)
+    tol = limits(ref, case)
+    d = on_gpu(case)
+    loss = forward(ctx, d)
+    close(loss, ref["loss"], tol[0], "loss")
+    got = call(ctx, d)
+    assert torch.equal(got[0], loss)
+    for g, name, t in zip(got[1:], ("d_features", "d_kernel"), tol[1:]):
+        assert g.dtype == case["x"].dtype
+        close(g, ref[name], t, name)
+    again = call(ctx, d)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    ctx.check_policy()
+    return got
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("n", [1, 2, 3, 7, 64, 301])
+def test_losses_and_gradients(ctx, n, dtype, moves):
+    check_all(ctx, make(n, dtype, seed=n, moves=moves))
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_boards_beyond_one_round_of_workgroups(ctx, dtype, moves):
+    check_all(ctx, make(2049, dtype, seed=9, moves=moves, longest=20))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_steep_logits(ctx, dtype, moves):
+    """Logits of a hundred and more: exp of them overflows, of their differences from the largest it does not."""
+    case = make(9, dtype, seed=4, moves=moves, scale=60.0)
+    ref = reference(case)
+    assert ref["top"].max() > 89      # where exp passes the largest float32
+    d = on_gpu(case)
+    close(forward(ctx, d), ref["loss"], limits(ref, case)[0], "loss")
+    got = call(ctx, d)
+    for g, name, t in zip(got[1:], ("d_features", "d_kernel"), limits(ref, case)[1:]):
+        close(g, ref[name], t, name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_lists_of_every_length(ctx, dtype):
+    """0 to 255 moves a board, the same move several times over, targets at both ends."""
+    rng = np.random.default_rng(2)
+    case = make(256, dtype, seed=2, moves=True)
+    per = rng.permutation(256).astype(np.uint8)
+    m = int(per.sum())
+    sq, fl = rng.integers(0, 64, m).astype(np.uint8), rng.integers(0, 73, m).astype(np.uint8)
+    sq[::3], fl[::3] = 63, 72
+    case["moves"] = sq, fl, per
+    case["t"] = torch.from_numpy(np.where(rng.random(256) < 0.5, 0, per.astype(np.int64) - 1))
+    case["t"][torch.from_numpy(per == 0)] = -1
+    check_all(ctx, case)
+
+
+@gpu
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 4095, 4096, 4097, 9000])
+def test_list_starts(ctx, n):
+    """Boards at the borders of whatever the prefix sum of the list lengths is cut into."""
+    check_all(ctx, make(n, torch.float32, seed=n, moves=True, longest=3))
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_boards_without_a_target(ctx, moves):
+    """They take no part whatever they hold; a NaN in a board that has a target stays in that board and the kernel."""
+    case = make(5, torch.float32, seed=1, moves=moves)
+    case["t"] = torch.tensor([3 if not moves else 0, -1, -1, 5 if not moves else 0, -1])
+    if moves:
+        case["moves"] = (case["moves"][0][:6].repeat(4), case["moves"][1][:6].repeat(4), np.array([6, 6, 0, 6, 6], np.uint8))
+    clean = check_all(ctx, case)
+    case["x"][1], case["x"][2], case["x"][4] = float("nan"), float("inf"), -float("inf")
+    d = on_gpu(case)
+    got = call(ctx, d)
+    assert torch.equal(forward(ctx, d), clean[0])
+    assert all(torch.equal(a, b) for a, b in zip(got, clean))
+    assert not got[1][[1, 2, 4]].any()
+    case["x"][3] = float("nan")
+    got = call(ctx, on_gpu(case))
+    assert got[0][3].isnan() and torch.equal(got[0][:3], clean[0][:3])
+    assert got[1][3].isnan().any() and torch.equal(got[1][:3], clean[1][:3]) and got[2].isnan().any()
+    case["t"][:] = -1
+    got = call(ctx, on_gpu(case))
+    assert not any(g.any() for g in got)
+    ctx.check_policy()
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_no_boards(ctx, moves):
+    case = make(3, torch.float32, moves=moves)
+    d = on_gpu(case)
+    d["x"], d["t"], d["w"], d["lists"] = d["x"][:0], d["t"][:0], d["w"][:0], tuple(a[:0] for a in d["lists"])
+    assert forward(ctx, d).shape == (0,)
+    d["w"] = torch.ones(1, device="cuda")
+    loss, dx, dk = call(ctx, d)
+    assert loss.shape == (0,) and dx.shape == (0, 32, 8, 8) and dk.shape == (32, 73) and not dk.any()
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_layouts_and_weights(ctx, moves):
+    """Strided, misaligned and permuted inputs, a kernel with the blob's shape, one weight for all boards."""
+    case = make(10, torch.bfloat16, seed=6, moves=moves)
+    d = on_gpu(case)
+    want = call(ctx, d)
+    other = dict(d)
+    other["x"] = d["x"].to(memory_format=torch.channels_last)
+    assert not other["x"].is_contiguous()
+    other["t"] = torch.stack([d["t"], d["t"]], 1)[:, 0]
+    room = torch.empty(d["k"].numel() + 1, dtype=torch.bfloat16, device="cuda")
+    room[1:] = d["k"].flatten()
+    other["k"] = room[1:].view(1, 1, 32, 73)
+    got = call(ctx, other)
+    assert got[2].shape == (1, 1, 32, 73)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[2].view(32, 73), want[2])
+    other["x"] = d["x"].reshape(10, 32, 64)
+    got = call(ctx, other)
+    assert got[1].shape == (10, 32, 64) and torch.equal(got[1].view_as(want[1]), want[1])
+    room = torch.empty(d["x"].numel() + 3, dtype=torch.bfloat16, device="cuda")
+    room[3:] = d["x"].flatten()
+    other["x"], other["k"] = room[3:].view_as(d["x"]), d["k"].t().contiguous().t()
+    assert all(torch.equal(a, b) for a, b in zip(call(ctx, other), want))
+    d["w"] = torch.tensor([0.25], device="cuda")
+    want = call(ctx, d)
+    d["w"] = d["w"].expand(10)
+    assert all(torch.equal(a, b) for a, b in zip(call(ctx, d), want))
+    d["w"] = torch.full((10,), 0.25, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(call(ctx, d), want))
+    only = call(ctx, d, kernel_grad=False)
+    assert torch.equal(only[1], want[1]) and only[2].numel() == 0
+    only = call(ctx, d, features_grad=False)
+    assert torch.equal(only[2], want[2]) and only[1].numel() == 0
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_autograd(ctx, dtype, moves):
+    case = make(21, dtype, seed=8, moves=moves)
+    d = on_gpu(case)
+    x, k = d["x"].clone().requires_grad_(), d["k"].clone().requires_grad_()
+    o = torch.ops.batchfirst
+    op = o.policy_move_loss if moves else o.policy_loss
+    (op(ctx.handle, x, k, *d["lists"], d["t"]) * d["w"]).sum().backward()
+    want = call(ctx, d)
+    assert torch.equal(x.grad, want[1]) and torch.equal(k.grad, want[2])
+    # a mean hands one expanded number down
+    k.grad = None
+    op(ctx.handle, d["x"], k, *d["lists"], d["t"]).mean().backward()
+    d["w"] = torch.full((1,), 1 / 21, device="cuda")
+    assert torch.equal(k.grad, call(ctx, d)[2])
+    loss = op(ctx.handle, x, k, *d["lists"], d["t"]).sum()
+    g, = torch.autograd.grad(loss, x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_gradient_is_the_difference_of_the_losses(ctx, moves):
+    """Along one direction, step h: the third derivative of a log-sum-exp along v is at most 0.2 r^3, r the spread of the
+    logits' change; the losses are known to their tolerance."""
+    case = make(6, torch.float32, seed=12, moves=moves)
+    ref = reference(case, torch.ones(1))
+    rng = np.random.default_rng(0)
+    v = torch.from_numpy(rng.standard_normal(case["x"].shape).astype(np.float32))
+    h = 2.0 ** -5
+    d = on_gpu(case)
+    d["w"] = torch.ones(1, device="cuda")
+    g = call(ctx, d)[1].cpu().double()
+    sides = []
+    for sign in (1, -1):
+        d["x"] = (case["x"] + sign * h * v).cuda()
+        sides.append(forward(ctx, d).cpu().double())
+    exactly = [losses.policy_loss((case["x"] + s * h * v).numpy(), case["k"].numpy(), case["t"].numpy(), np.ones(6), case["moves"]) for s in (1, -1)]
+    r = np.abs(np.einsum("cf,ncs->nfs", case["k"].double().numpy(), v.double().numpy().reshape(6, 32, 64))).max((1, 2)) * 2
+    tol = h * h / 6 * 0.2 * r ** 3 + (limits(exactly[0], case)[0] + limits(exactly[1], case)[0]) / (2 * h)
+    along = (g * v.double()).flatten(1).sum(1)
+    tol = tol + (limits(ref, case)[1] * np.abs(v.double().numpy().reshape(6, 32, 64))).sum((1, 2))
+    assert np.all(np.abs(((sides[0] - sides[1]) / (2 * h) - along).numpy()) <= tol)
+
+
+@gpu
+def test_out_of_range_inputs_are_reported_once(ctx):
+    case = make(4, torch.float32, seed=3)
+    case["t"] = torch.tensor([1, 4672, -2, 7])
+    d = on_gpu(case)
+    loss, dx, dk = call(ctx, d)
+    assert loss[1] == 0 and loss[2] == 0 and not dx[1:3].any()
+    with pytest.raises(ValueError, match="out of range"):
+        ctx.check_policy()
+    ctx.check_policy()
+    case["t"][1:3] = -1
+    assert all(torch.equal(a, b) for a, b in zip((loss, dx, dk), call(ctx, on_gpu(case))))
+    ctx.check_policy()
+
+    case = make(3, torch.float32, seed=3, moves=True)
+    case["moves"] = (np.array([1, 2, 3, 4, 5], np.uint8), np.array([0, 1, 2, 3, 4], np.uint8), np.array([2, 0, 3], np.uint8))
+    case["t"] = torch.tensor([0, -1, 2])
+    check_all(ctx, case)
+
+    def reported(change):
+        bad = dict(case)
+        bad["t"] = case["t"].clone()
+        bad["moves"] = tuple(a.copy() for a in case["moves"])
+        change(bad)
+        d = on_gpu(bad)
+        got = call(ctx, d)
+        with pytest.raises(ValueError, match="out of range"):
+            ctx.check_policy()
+        assert torch.equal(forward(ctx, d), got[0])
+        with pytest.raises(ValueError, match="out of range"):
+            ctx.check_policy()
+        return got
+
+    assert reported(lambda c: c["t"].__setitem__(2, 3))[0][2] == 0
+    assert reported(lambda c: c["t"].__setitem__(1, 0))[0][1] == 0
+    reported(lambda c: c["moves"][0].__setitem__(0, 64))
+    reported(lambda c: c["moves"][1].__setitem__(0, 73))
+    reported(lambda c: c["moves"][2].__setitem__(0, 1))        # one move too few
+    reported(lambda c: c["moves"][2].__setitem__(2, 200))      # far too many: absent ones end the list
+    ctx.check_policy()
+
+
+@gpu
+def test_ops_refuse(ctx):
+    o = torch.ops.batchfirst
+    x, k, t = torch.zeros(2, 32, 8, 8, device="cuda"), torch.zeros(32, 73, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    u8 = torch.zeros(2, dtype=torch.uint8, device="cuda")
+    w = torch.ones(2, device="cuda")
+    for bad, match in (((x[:, :31], k, t), "shape"), ((x, k[:31], t), "shape"), ((x, k.t(), t), "shape"), ((x, k.bfloat16(), t), "dtype"),
+                       ((x, k, t[:1]), "one entry"), ((x, k, t.int()), "dtype"), ((x.double(), k, t), "float32, bfloat16"),
+                       ((x.cpu(), k, t), "device tensor"), ((x, k, t.cpu()), "device tensor")):
+        with pytest.raises(ValueError, match=match):
+            o.policy_loss(ctx.handle, *bad)
+    for bad, match in ((w[:1].expand(2, 1), "board_weights"), (torch.ones(3, device="cuda"), "board_weights"), (w.double(), "dtype")):
+        with pytest.raises(ValueError, match=match):
+            o.policy_loss_grad(ctx.handle, x, k, t, bad)
+    for bad, match in (((u8, u8[:1], u8), "one per move"), ((u8, u8, u8[:1]), "one entry per board"), ((u8.int(), u8, u8), "dtype")):
+        with pytest.raises(ValueError, match=match):
+            o.policy_move_loss(ctx.handle, x, k, *bad, t)
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_captured_and_replayed(ctx, moves):
+    """Two graphs with their own workspaces, replayed in turn with other inputs and eager calls between."""
+    cases = [make(300, torch.bfloat16, seed=s, moves=moves) for s in (1, 2)]
+    if moves:      # a graph's lists keep their total
+        cases[1]["moves"], cases[1]["t"] = cases[0]["moves"], cases[0]["t"]
+    static = on_gpu(cases[0])
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        call(ctx, static)
+        side.synchronize()
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(call(ctx, static))
+            graphs.append(g)
+    torch.cuda.synchronize()
+    for turn in range(4):
+        d = on_gpu(cases[turn % 2])
+        want = call(ctx, d)
+        for name in ("x", "k", "w", "t"):
+            static[name].copy_(d[name])
+        for g, out in zip(graphs, outs):
+            for o in out:
+                o.fill_(7.0)
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+    ctx.check_policy()
+
+
+@gpu
+def test_streams_of_their_own(ctx):
+    """Calls on two streams at once, each with its own workspace, give what they give alone."""
+    cases = [on_gpu(make(700, torch.float32, seed=s, moves=s % 2 == 1, longest=30)) for s in range(4)]
+    want = [call(ctx, d) for d in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [None] * 4
+    for _ in range(5):
+        for i, (s, d) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i] = call(ctx, d)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@gpu
+def test_features_beyond_four_gib(ctx):
+    """More than 2^31 elements and 2^32 bytes of features: the last boards give what they give in a call of their own."""
+    n = (1 << 20) + 3
+    case = make(16, torch.bfloat16, seed=5)
+    d = on_gpu(case)
+    x = d["x"].repeat((n + 15) // 16, 1, 1, 1)[:n]
+    t = d["t"].repeat((n + 15) // 16)[:n]
+    one = torch.ones(1, device="cuda")
+    loss, dx, _ = torch.ops.batchfirst.policy_loss_grad(ctx.handle, x, d["k"], t, one, kernel_grad=False)
+    want = torch.ops.batchfirst.policy_loss_grad(ctx.handle, x[-16:].clone(), d["k"], t[-16:].clone(), one, kernel_grad=False)
+    assert torch.equal(loss[-16:], want[0]) and torch.equal(dx[-16:], want[1])
+    assert torch.equal(torch.ops.batchfirst.policy_loss(ctx.handle, x, d["k"], t)[-16:], want[0])
+    per = torch.full((n,), 2, dtype=torch.uint8, device="cuda")
+    frm = torch.arange(2 * n, device="cuda").remainder(64).to(torch.uint8)
+    flt = torch.arange(2 * n, device="cuda").remainder(73).to(torch.uint8)
+    t = torch.arange(n, device="cuda").remainder(3) - 1
+    args = (frm, flt, per, t)
+    loss, dx, _ = torch.ops.batchfirst.policy_move_loss_grad(ctx.handle, x, d["k"], *args, one, kernel_grad=False)
+    last = (frm[-32:].clone(), flt[-32:].clone(), per[-16:].clone(), t[-16:].clone())
+    want = torch.ops.batchfirst.policy_move_loss_grad(ctx.handle, x[-16:].clone(), d["k"], *last, one, kernel_grad=False)
+    assert torch.equal(loss[-16:], want[0]) and torch.equal(dx[-16:], want[1])
+    ctx.check_policy()
