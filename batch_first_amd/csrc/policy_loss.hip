@@ -10,6 +10,8 @@
 // (k_policy_move_loss).  A board without a target has loss 0 and no part in the gradients.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/batchfirst.h"
 #include "bf_train.h"
 
@@ -40,54 +42,418 @@ __device__ __forceinline__ float block_reduce(float v, float* red) {
     return MAX ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-template <typename T, bool GRAD>
-__global__ __launch_bounds__(kThreads) void k_policy_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
-                                                          const int64_t* __restrict__ targets, const float* __restrict__ weights,
-                                                          unsigned weight_step, float* __restrict__ loss, T* __restrict__ dx,
-                                                          float* __restrict__ dw_part, int* __restrict__ err) {
-    __shared__ float sx[kC * kS], sw[kXW], sp[kVocab], red[4];
-    const int tid = threadIdx.x;
-    for (int i = tid; i < kXW; i += kThreads) sw[i] = (float)w[i];
-    float acc[(kXW + kThreads - 1) / kThreads] = {};
-    for (size_t b = blockIdx.x; b < n; b += gridDim.x) {
-        __syncthreads();
-        for (int i = tid; i < kC * kS; i += kThreads) sx[i] = (float)x[b * (kC * kS) + i];
-        __syncthreads();
-        float top = -INFINITY;
-        for (int i = tid; i < kVocab; i += kThreads) {
-            float l = 0.0f;
-            for (int c = 0; c < kC; ++c) l = fmaf(sw[c * kF + (i >> 6)], sx[c * kS + (i & 63)], l);
-            sp[i] = l;
-            top = fmaxf(top, l);
-        }
-        top = block_reduce<true>(top, red);
-        float z = 0.0f;
-        for (int i = tid; i < kVocab; i += kThreads) z += expf(sp[i] - top);
-        z = block_reduce<false>(z, red);
-        const int64_t t = targets[b];
-        const bool has = t >= 0 && t < kVocab;
-        if (tid == 0) {
-            if (t < -1 || t >= kVocab) atomicOr(err, 8);
-            if (loss) loss[b] = has ? logf(z) + top - sp[t] : 0.0f;
-        }
-        if (!GRAD) continue;
-        __syncthreads();
-        const float wb = has ? weights[b * weight_step] : 0.0f;
-        for (int i = tid; i < kVocab; i += kThreads) sp[i] = has ? (expf(sp[i] - top) / z - (i == t ? 1.0f : 0.0f)) * wb : 0.0f;
-        __syncthreads();
-        if (dx)
-            for (int i = tid; i < kC * kS; i += kThreads) {
-                float a = 0.0f;
-                for (int f = 0; f < kF; ++f) a = fmaf(sw[(i >> 6) * kF + f], sp[f * kS + (i & 63)], a);
-                dx[b * (kC * kS) + i] = (T)a;
-            }
-        if (dw_part && has)
-            for (int k = 0, i = tid; i < kXW; i += kThreads, ++k)
-                for (int s = 0; s < kS; ++s) acc[k] = fmaf(sx[(i / kF) * kS + s], sp[(i % kF) * kS + s], acc[k]);
+// ---- the whole vocabulary --------------------------------------------------------------------------------------------
+//
+// One wave a board, everything between the features and the gradients in its registers, on 16x16x32 MFMAs with float32
+// sums.  Lane l = (n = l & 15, q = l >> 4) of an operand holds eight k (8 q ... 8 q + 7) of row or column n, of a result
+// the rows 4 q ... 4 q + 3 of column n.
+//
+//   logits   rows filter (five tiles of 16, 73 padded to 80), columns square, k channel.  Column n of tile j is square
+//            4 n + j, so that a lane's features are four neighbours in memory.
+//   dX       rows channel, columns square, k filter.  k is numbered so that a lane's eight are the filters whose logits
+//            it holds already: the probabilities become an operand where they are.
+//   dW       rows channel, columns filter, k square: the probabilities cross the lanes through LDS, 32 filters at a time;
+//            the sums stay in registers over all the wave's boards.
+//
+// float32 operands travel as two float16 terms (22 bits), scaled by a power of two, the kernel's by its largest element
+// and the features' by the board's, so that the larger term stays normal down to 2^-29 of the largest; of the four products of terms the
+// least is left out (2^-22).  bfloat16 and float16 operands are exact as they are.  The logits' gradients d (before the
+// weight) travel as two terms: bfloat16 ones for bfloat16 features, else float16 ones, scaled like the features.  Their
+// largest is the target's, which is the negative sum of all the others.
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Arith {                                   // float32 and float16 features: float16 terms
+    static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
+    static constexpr bool kScaled = true;
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
     }
-    if (GRAD && dw_part)
-        for (int k = 0, i = tid; i < kXW; i += kThreads, ++k) dw_part[(size_t)blockIdx.x * kXW + i] = acc[k];
+    // (a, b) = terms hi + lo, each packed with a in the low half; rounded towards zero, so lo has hi's sign
+    static __device__ __forceinline__ void split(float a, float b, unsigned& hi, unsigned& lo) {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+        hi = __builtin_bit_cast(unsigned, h);
+        lo = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+    }
+};
+template <>
+struct Arith<__bf16> {
+    static constexpr int kTerms = 1;
+    static constexpr bool kScaled = false;
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void split(float a, float b, unsigned& hi, unsigned& lo) {
+        hi = __builtin_bit_cast(unsigned, bf2{(__bf16)a, (__bf16)b});
+        lo = __builtin_bit_cast(unsigned, bf2{(__bf16)(a - __uint_as_float(hi << 16)), (__bf16)(b - __uint_as_float(hi & 0xffff0000u))});
+    }
+};
+
+// The larger, or NaN if either is: one instruction of three operands, without the quieting that fmaxf's takes each.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Over the 64 lanes, in fixed order; the result is uniform.
+template <bool MAX>
+__device__ __forceinline__ float lanes_reduce(float v) {
+    auto step = [](float a, float b) { return MAX ? larger(a, b) : a + b; };
+#define BF_DPP(ctrl) v = step(v, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), ctrl, 0xf, 0xf, true)))
+    BF_DPP(0xb1);    // quad_perm [1, 0, 3, 2]
+    BF_DPP(0x4e);    // quad_perm [2, 3, 0, 1]
+    BF_DPP(0x141);   // row_half_mirror
+    BF_DPP(0x140);   // row_mirror
+#undef BF_DPP
+    auto at = [&](int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); };
+    return step(step(at(0), at(16)), step(at(32), at(48)));
 }
+
+// 2^(13 - e) for a largest magnitude in [2^e, 2^(e+1)), and its reciprocal; magnitudes below 2^least count as that.
+__device__ __forceinline__ void scale_of(float largest, int least, float& scale, float& back) {
+    const int e = max((int)(__float_as_uint(largest) >> 23 & 255u) - 127, least);
+    scale = __uint_as_float((unsigned)(127 + 13 - e) << 23);
+    back = __uint_as_float((unsigned)(127 - 13 + e) << 23);
+}
+
+constexpr int kTiles = 5;                        // of filters
+constexpr int kRow = 72;                         // 16-bit elements a row of the crossing: 16 rows start in 16 different bank groups
+constexpr int kCross = 2 * 32 * kRow * 2;        // bytes: two terms of 32 filters
+constexpr int kWaveLds = 64 * 40 * 4;            // bytes a wave: the crossing, at the end its kernel gradient
+static_assert(kCross <= kWaveLds, "the crossing fits");
+
+template <typename T>
+struct HeadLds {                                 // the kernel as operands, 16 bytes a lane
+    u32x4 logit[kTiles][Arith<T>::kTerms][64];   // rows filter, k channel
+    u32x4 back[3][2][Arith<T>::kTerms][64];      // rows channel, k filter as the logits' results hold them
+    float red[8];
+};
+
+// Eight values as an operand of one or two terms.
+template <typename T>
+__device__ __forceinline__ void operand(const float (&v)[8], float scale, u32x4 (&out)[Arith<T>::kTerms]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (Arith<T>::kTerms == 2) {
+            unsigned hi, lo;
+            Arith<T>::split(v[2 * i] * scale, v[2 * i + 1] * scale, hi, lo);
+            out[0][i] = hi;
+            out[1][i] = lo;
+        } else if constexpr (sizeof(T) == 2) {
+            typedef T pair __attribute__((ext_vector_type(2)));
+            out[0][i] = __builtin_bit_cast(unsigned, pair{(T)v[2 * i], (T)v[2 * i + 1]});
+        }
+    }
+}
+
+// Fills the kernel's operands; returns the factor that takes a product of scaled operands' kernel part back.
+template <typename T, bool GRAD>
+__device__ __forceinline__ float load_head(const T* __restrict__ w, HeadLds<T>& lds) {
+    float scale = 1.0f, back = 1.0f;
+    const int tid = threadIdx.x, waves = blockDim.x >> 6;
+    if constexpr (Arith<T>::kTerms == 2) {
+        float largest = 0.0f;
+        for (int i = tid; i < kXW; i += blockDim.x) largest = fmaxf(largest, fabsf((float)w[i]));
+        largest = lanes_reduce<true>(largest);
+        if ((tid & 63) == 0) lds.red[tid >> 6] = largest;
+        __syncthreads();
+        for (int i = 0; i < waves; ++i) largest = fmaxf(largest, lds.red[i]);
+        scale_of(largest, -100, scale, back);
+    }
+    for (int i = tid; i < kTiles * 64; i += blockDim.x) {
+        const int f = (i >> 6) * 16 + (i & 15), q = i >> 4 & 3;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = f < kF ? (float)w[(8 * q + k) * kF + f] : 0.0f;
+        u32x4 out[Arith<T>::kTerms];
+        operand<T>(v, scale, out);
+#pragma unroll
+        for (int k = 0; k < Arith<T>::kTerms; ++k) lds.logit[i >> 6][k][i & 63] = out[k];
+    }
+    if (GRAD)
+        for (int i = tid; i < 6 * 64; i += blockDim.x) {
+            const int u = i >> 7, a = i >> 6 & 1, c = a * 16 + (i & 15), q = i >> 4 & 3;
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int f = 32 * u + 16 * (k >> 2) + 4 * q + (k & 3);
+                v[k] = f < kF ? (float)w[c * kF + f] : 0.0f;
+            }
+            u32x4 out[Arith<T>::kTerms];
+            operand<T>(v, scale, out);
+#pragma unroll
+            for (int k = 0; k < Arith<T>::kTerms; ++k) lds.back[u][a][k][i & 63] = out[k];
+        }
+    __syncthreads();
+    return back;
+}
+
+// A product of operands of one or two terms each, the least of four left out.
+template <typename T, int TA, int TB>
+__device__ __forceinline__ f32x4 products(const u32x4 (&a)[TA], const u32x4 (&b)[TB], f32x4 c) {
+    if constexpr (TB == 2) c = Arith<T>::mfma(a[0], b[1], c);
+    if constexpr (TA == 2) c = Arith<T>::mfma(a[1], b[0], c);
+    return Arith<T>::mfma(a[0], b[0], c);
+}
+
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
+                                                     const int64_t* __restrict__ targets, const float* __restrict__ weights,
+                                                     unsigned weight_step, float* __restrict__ loss, T* __restrict__ dx,
+                                                     float* __restrict__ dw_part, int* __restrict__ err) {
+    constexpr int NT = Arith<T>::kTerms;
+    extern __shared__ __align__(16) unsigned char smem[];
+    HeadLds<T>& lds = *reinterpret_cast<HeadLds<T>*>(smem);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int col = lane & 15, q = lane >> 4;
+    unsigned char* mine = smem + sizeof(HeadLds<T>) + wave * kWaveLds;   // gradient calls only
+    const float w_back = load_head<T, GRAD>(w, lds);
+
+    f32x4 dw[2][kTiles];
+    if (GRAD)
+#pragma unroll
+        for (int i = 0; i < 2 * kTiles; ++i) dw[i / kTiles][i % kTiles] = f32x4{0, 0, 0, 0};
+
+    for (size_t b = (size_t)blockIdx.x * waves + wave; b < n; b += (size_t)gridDim.x * waves) {
+        const T* xb = x + b * (kC * kS);
+        const int64_t t64 = targets[b];
+        const int target = __builtin_amdgcn_readfirstlane(t64 >= 0 && t64 < kVocab ? (int)t64 : -1);
+        if (target < 0) {                        // no part in anything, whatever the features hold
+            if (lane == 0) {
+                if (t64 != -1) atomicOr(err, 8);
+                if (loss) loss[b] = 0.0f;
+            }
+            if (GRAD && dx) {
+                u32x4* out = reinterpret_cast<u32x4*>(dx + b * (kC * kS));
+#pragma unroll
+                for (int i = 0; i < (int)(kC * kS * sizeof(T) / 1024); ++i) out[i * 64 + lane] = u32x4{0, 0, 0, 0};
+            }
+            continue;
+        }
+
+        // features as columns: square 4 col + j, channels 8 q ... 8 q + 7
+        u32x4 xc[4][NT];
+        float x_scale = 1.0f, x_back = 1.0f;
+        if constexpr (sizeof(T) == 4) {
+            f32x4 raw[8];
+            float largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const f32x4*>(xb + (8 * q + i) * kS + 4 * col);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) largest = larger(largest, fabsf(raw[i][j]));
+            scale_of(lanes_reduce<true>(largest), -100, x_scale, x_back);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = raw[i][j];
+                operand<T>(v, x_scale, xc[j]);
+            }
+        } else {
+            u32x2 raw[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const u32x2*>(xb + (8 * q + i) * kS + 4 * col);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    xc[j][0][i] = __builtin_amdgcn_perm(raw[2 * i + 1][j >> 1], raw[2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+        }
+
+        // logits, in units of 2^-(scales)
+        f32x16 v[kTiles];                        // [tile of filters][4 * square + row]
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            u32x4 a[NT];
+#pragma unroll
+            for (int k = 0; k < NT; ++k) a[k] = lds.logit[t][k][lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 l = products<T>(a, xc[j], f32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[t][4 * j + r] = l[r];
+            }
+        }
+        // the padding's filters 73 ... 79
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (64 + 4 * q + r >= kF) v[kTiles - 1][4 * j + r] = -INFINITY;
+
+        // the target's place: tile, register and lane are uniform
+        const int tf = target >> 6, ts = target & 63;
+        const int t_tile = tf >> 4, t_reg = (ts & 3) * 4 + (tf & 3), t_lane = (tf >> 2 & 3) * 16 + (ts >> 2);
+        auto at_target = [&](auto&& change) {    // returns what the target's lane then holds
+            float e = 0.0f;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+                if (t == t_tile) {
+                    e = change(v[t][t_reg]);
+                    v[t][t_reg] = e;
+                    asm volatile("" : "+v"(e));  // keeps the branch
+                }
+            return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), t_lane));
+        };
+        const float l_target = at_target([&](float e) { return e; });
+
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) top = larger(top, larger(v[t][k], v[t][k + 1]));
+        top = lanes_reduce<true>(top);
+        // exp(l - top) = 2^(l unit - top unit); an error of the rounded second product is common to all of the board
+        const float unit = fminf(fmaxf(w_back * x_back, 1e-36f), 1e38f);
+        const float unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
+        float z4[4] = {};
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                v[t][k] = __builtin_amdgcn_exp2f(fmaf(v[t][k], unit2, top2));
+                z4[k & 3] += v[t][k];
+            }
+        const float z = lanes_reduce<false>((z4[0] + z4[1]) + (z4[2] + z4[3]));
+        if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
+        if (!GRAD) continue;
+
+        // the logits' gradients: probabilities, less one at the target.  The target's is the largest but for rounding:
+        // z's own, up to 90 * 2^-24, can make the target's smaller than another by as much, which the least scale covers.
+        const float rz = __builtin_amdgcn_rcpf(z);
+        const float d_target = at_target([&](float e) { return e - (lane == t_lane ? z : 0.0f); }) * rz;
+        float d_scale = 1.0f, d_back = 1.0f;
+        if constexpr (Arith<T>::kScaled) scale_of(fabsf(d_target), -17, d_scale, d_back);
+        const float inv = d_scale * rz;
+        const float wb = weights[b * weight_step] * d_back;
+
+        // features as rows: channel col of each half, squares 8 q ... 8 q + 7 of each half
+        u32x4 xr[2][2][NT];
+        if (dw_part) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const T* p = xb + (16 * a + col) * kS + 32 * h + 8 * q;
+                    if constexpr (sizeof(T) == 4) {
+                        const f32x4 lo = reinterpret_cast<const f32x4*>(p)[0], hi = reinterpret_cast<const f32x4*>(p)[1];
+                        const float e[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                        operand<T>(e, x_scale, xr[a][h]);
+                    } else {
+                        xr[a][h][0] = *reinterpret_cast<const u32x4*>(p);
+                    }
+                }
+        }
+
+        f32x4 g[2][4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i >> 2][i & 3] = f32x4{0, 0, 0, 0};
+        const float w_scale = wb * x_back;
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+            const int tiles = u < 2 ? 2 : 1;
+            u32x4 d[4][2];                       // [square of four][term]: eight filters
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unsigned hi = 0, lo = 0;
+                    if (i < 2 * tiles) {
+                        const f32x16& p = v[2 * u + (i >> 1)];
+                        const int k = 4 * j + 2 * (i & 1);
+                        Arith<T>::split(p[k] * inv, p[k + 1] * inv, hi, lo);
+                    }
+                    d[j][0][i] = hi;
+                    d[j][1][i] = lo;
+                }
+            if (dw_part) {
+                // across the lanes: row filter, four squares at a time
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2 * tiles; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const unsigned pick = h ? 0x07060302u : 0x05040100u;
+                            const u32x2 four = {__builtin_amdgcn_perm(d[1][k][i], d[0][k][i], pick), __builtin_amdgcn_perm(d[3][k][i], d[2][k][i], pick)};
+                            const int row = 16 * (i >> 1) + 4 * q + 2 * (i & 1) + h;
+                            *reinterpret_cast<u32x2*>(mine + ((k * 32 + row) * kRow + 4 * col) * 2) = four;
+                        }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+            if (dx) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    u32x4 wk[NT];
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) wk[k] = lds.back[u][a][k][lane];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) g[a][j] = products<T>(wk, d[j], g[a][j]);
+                }
+            }
+            if (dw_part) {
+#pragma unroll
+                for (int t = 0; t < tiles; ++t) {
+                    f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        u32x4 dk[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            dk[k] = *reinterpret_cast<const u32x4*>(mine + ((k * 32 + 16 * t + col) * kRow + 32 * h + 8 * q) * 2);
+#pragma unroll
+                        for (int a = 0; a < 2; ++a) s[a] = products<T>(xr[a][h], dk, s[a]);
+                    }
+#pragma unroll
+                    for (int a = 0; a < 2; ++a)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) dw[a][2 * u + t][r] = fmaf(s[a][r], w_scale, dw[a][2 * u + t][r]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        if (dx) {
+            const float back = wb * w_back;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    typedef T four_t __attribute__((ext_vector_type(4)));
+                    const four_t out = {(T)(g[a][0][r] * back), (T)(g[a][1][r] * back), (T)(g[a][2][r] * back), (T)(g[a][3][r] * back)};
+                    *reinterpret_cast<four_t*>(dx + b * (kC * kS) + (16 * a + 4 * q + r) * kS + 4 * col) = out;
+                }
+        }
+    }
+
+    if (GRAD && dw_part) {
+        float* part = reinterpret_cast<float*>(mine);
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) part[((16 * a + 4 * q + r) * kTiles + t) * 16 + col] = dw[a][t][r];
+        __syncthreads();
+        const float* all = reinterpret_cast<const float*>(smem + sizeof(HeadLds<T>));
+        for (int i = threadIdx.x; i < kXW; i += blockDim.x) {
+            const int c = i / kF, f = i % kF;
+            float a = 0.0f;
+            for (int k = 0; k < waves; ++k) a += all[k * (kWaveLds / 4) + c * 80 + f];
+            dw_part[(size_t)blockIdx.x * kXW + i] = a;
+        }
+    }
+}
+
+// ---- the boards' own moves -------------------------------------------------------------------------------------------
 
 // start[b] = moves of the boards before b, start[n] = all moves; one workgroup.
 __global__ __launch_bounds__(1024) void k_move_starts(const uint8_t* __restrict__ per, size_t n, size_t n_moves,
@@ -172,14 +538,46 @@ __global__ __launch_bounds__(kThreads) void k_policy_move_loss(const T* __restri
         for (int k = 0, i = tid; i < kXW; i += kThreads, ++k) dw_part[(size_t)blockIdx.x * kXW + i] = acc[k];
 }
 
-// The partial kernel gradients of the workgroups, added up in fixed order.
+// The partial kernel gradients of the workgroups, added up in fixed order: a workgroup 32 elements, eight threads each.
 template <typename T>
-__global__ __launch_bounds__(64) void k_sum_parts(const float* __restrict__ part, unsigned parts, T* __restrict__ dw) {
-    const int i = blockIdx.x * 64 + threadIdx.x;
-    if (i >= kXW) return;
+__global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ part, unsigned parts, T* __restrict__ dw) {
+    __shared__ double sums[8][32];
+    const int i = blockIdx.x * 32 + (threadIdx.x & 31), j = threadIdx.x >> 5;
     double a = 0.0;
-    for (unsigned p = 0; p < parts; ++p) a += part[(size_t)p * kXW + i];
-    dw[i] = (T)(float)a;
+#pragma unroll 8
+    for (unsigned p = j; p < parts; p += 8) a += part[(size_t)p * kXW + i];
+    sums[j][threadIdx.x & 31] = a;
+    __syncthreads();
+    if (j == 0) {
+        for (int k = 1; k < 8; ++k) a += sums[k][threadIdx.x];
+        dw[i] = (T)(float)a;
+    }
+}
+static_assert(kXW % 32 == 0, "k_sum_parts needs no bounds check");
+
+constexpr unsigned kGroups = 256;   // workgroups of a gradient call over the vocabulary: one a compute unit
+
+// Waves a workgroup: small calls are spread over the compute units.
+unsigned waves_for(size_t n, unsigned most) {
+    unsigned waves = 1;
+    while (waves < most && (size_t)waves * kGroups < n) waves *= 2;
+    return waves;
+}
+
+template <typename T>
+hipError_t launch_vocabulary(const PolicyLossArgs& a, float* part, unsigned* parts, hipStream_t s) {
+    const T *x = static_cast<const T*>(a.features), *w = static_cast<const T*>(a.kernel);
+    if (a.d_features || part) {
+        const unsigned waves = waves_for(a.n, 8), lds = sizeof(HeadLds<T>) + waves * kWaveLds;
+        *parts = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, kGroups);
+        hipLaunchKernelGGL((k_policy_loss<T, true>), dim3(*parts), dim3(waves * 64), lds, s, x, w, a.n, a.targets, a.weights,
+                           a.n_weights > 1 ? 1u : 0u, a.loss, static_cast<T*>(a.d_features), part, a.err);
+    } else {
+        const unsigned waves = waves_for(a.n, 4);
+        hipLaunchKernelGGL((k_policy_loss<T, false>), dim3((unsigned)std::min<size_t>((a.n + waves - 1) / waves, 4 * kGroups)),
+                           dim3(waves * 64), sizeof(HeadLds<T>), s, x, w, a.n, a.targets, nullptr, 0u, a.loss, nullptr, nullptr, a.err);
+    }
+    return hipGetLastError();
 }
 
 unsigned grid_for(size_t n) { return (unsigned)(n < kMaxGrid ? n : kMaxGrid); }
@@ -189,7 +587,7 @@ hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
     const T *x = static_cast<const T*>(a.features), *w = static_cast<const T*>(a.kernel);
     T* dx = static_cast<T*>(a.d_features);
     const bool grad = a.d_features || a.d_kernel;
-    const unsigned grid = grid_for(a.n);
+    unsigned grid = grid_for(a.n);
     const unsigned step = a.n_weights > 1 ? 1u : 0u;
     uint64_t* start = static_cast<uint64_t*>(a.workspace);
     float* part = a.d_kernel ? reinterpret_cast<float*>(a.per_board ? start + (a.n + 2) / 2 * 2 : start) : nullptr;
@@ -202,15 +600,11 @@ hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
             hipLaunchKernelGGL((k_policy_move_loss<T, false>), dim3(grid), dim3(kThreads), 0, s, x, w, a.n, a.from, a.filter, a.n_moves,
                                start, a.targets, nullptr, 0u, a.loss, nullptr, nullptr, a.err);
     } else if (grid) {
-        if (grad)
-            hipLaunchKernelGGL((k_policy_loss<T, true>), dim3(grid), dim3(kThreads), 0, s, x, w, a.n, a.targets, a.weights, step, a.loss,
-                               dx, part, a.err);
-        else
-            hipLaunchKernelGGL((k_policy_loss<T, false>), dim3(grid), dim3(kThreads), 0, s, x, w, a.n, a.targets, nullptr, 0u, a.loss,
-                               nullptr, nullptr, a.err);
+        hipError_t e = launch_vocabulary<T>(a, part, &grid, s);
+        if (e != hipSuccess) return e;
     }
     if (a.d_kernel)
-        hipLaunchKernelGGL(k_sum_parts<T>, dim3((kXW + 63) / 64), dim3(64), 0, s, part, grid, static_cast<T*>(a.d_kernel));
+        hipLaunchKernelGGL(k_sum_parts<T>, dim3(kXW / 32), dim3(256), 0, s, part, grid, static_cast<T*>(a.d_kernel));
     return hipGetLastError();
 }
 

@@ -10,6 +10,11 @@ Tolerances, with u = 2^-24 (half a step of float32), eps(t) / 2 half a step of t
                                         split = 2^-17 where the probabilities travel as two bf16 terms (16-bit types)
   A probability below float32's smallest normal number 2^-126, or a bf16 term of one, may be flushed to zero: up to three
   flushes a product, 3 * 2^-126 * weight * |factor|, summed over the 73 filters / the boards' 64 squares.
+  Operands in two float16 terms are scaled so that the largest lies in [2^13, 2^14) or above and end at float16's last
+  step, 2^-24: what is below 2^-37 of the largest is lost.  The largest gradient of a board's logits is the target's, 1 - exp(-loss)
+  (counted as 2^-17 where smaller); their magnitudes sum to at most twice that.  So a gradient may miss 2^-37 times
+  2 weight (1 - exp(-loss)) times the largest factor, for either operand's loss, and for the logits' gradients as many
+  times as there are terms: 73 or 64.
 """
 import ctypes
 
@@ -61,14 +66,17 @@ def limits(ref, case):
     dtype = case["x"].dtype
     flush = 3 * 2.0 ** -126 * float(case["w"].max())
     dl = 40 * U * ref["logit_size"]
+    x, k = np.abs(case["x"].double().numpy().reshape(-1, 32, 64)), float(case["k"].abs().max())
+    x = np.nan_to_num(x, posinf=0.0).max((1, 2), initial=0.0)
+    lost = 2.0 ** -37 * np.broadcast_to(case["w"].double().numpy(), len(x)) * np.maximum(-np.expm1(-ref["loss"]), 2.0 ** -17)
     p = 2 * dl + U * (2 * ref["spread"] + 100)
     split = 0.0 if dtype == torch.float32 else 2.0 ** -17
     half, least = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     return (2 * dl + 16 * U * (1 + np.abs(ref["loss"]) + ref["top"]),
             (p[:, None, None] + U * 80 + split) * ref["d_features_size"] + half * np.abs(ref["d_features"]) + least
-            + flush * 73 * float(case["k"].abs().max()),
+            + flush * 73 * k + (lost * 75 * k)[:, None, None],
             (p.max(initial=0.0) + U * 600 + split) * ref["d_kernel_size"] + half * np.abs(ref["d_kernel"]) + least
-            + flush * 64 * len(case["t"]) * float(case["x"].nan_to_num().abs().max()))
+            + flush * 64 * len(x) * x.max(initial=0.0) + (lost * 66 * x).sum())
 
 
 def close(got, want, tol, what):
