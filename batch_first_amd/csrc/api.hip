@@ -978,7 +978,7 @@ int check_loss(bf_ctx* c, bf::PolicyLossArgs* a, bool grad, size_t workspace_byt
         if (a->n_moves && (!a->from || !a->filter)) return bf::fail(BF_E_ARG, "%s: null pointer", who);
         if (a->n == 0 && a->n_moves) return bf::fail(BF_E_ARG, "%s: moves given without boards", who);
     }
-    const size_t need = bf::policy_loss_workspace(a->n, a->per_board != nullptr, a->d_kernel != nullptr);
+    const size_t need = a->d_kernel ? bf::policy_loss_workspace(a->n) : 0;
     if (workspace_bytes < need || (need && !a->workspace))
         return bf::fail(BF_E_ARG, "%s: the workspace has %zu bytes, %zu are needed", who, a->workspace ? workspace_bytes : 0, need);
     a->err = c->policy.d_err;
@@ -1013,8 +1013,7 @@ int check_norm(const bf_ctx* c, const void* const* ptrs, const size_t* counts, c
 
 }  // namespace
 
-extern "C" size_t bf_policy_loss_workspace(size_t n) { return bf::policy_loss_workspace(n, false, true); }
-extern "C" size_t bf_policy_move_loss_workspace(size_t n) { return bf::policy_loss_workspace(n, true, true); }
+extern "C" size_t bf_policy_loss_workspace(size_t n) { return bf::policy_loss_workspace(n); }
 
 extern "C" int bf_policy_loss(bf_ctx* c, const void* d_features, int type, size_t n, const void* d_kernel, const int64_t* d_targets,
                               float* d_loss, void* stream) {
@@ -1036,12 +1035,12 @@ extern "C" int bf_policy_loss_grad(bf_ctx* c, const void* d_features, int type, 
 
 extern "C" int bf_policy_move_loss(bf_ctx* c, const void* d_features, int type, size_t n, const void* d_kernel, const uint8_t* d_from,
                                    const uint8_t* d_filter, const uint8_t* d_per_board, size_t n_moves, const int64_t* d_targets,
-                                   float* d_loss, void* d_workspace, size_t workspace_bytes, void* stream) {
+                                   float* d_loss, void* stream) {
     bf::PolicyLossArgs a{};
     a.features = d_features, a.type = type, a.n = n, a.kernel = d_kernel, a.targets = d_targets, a.loss = d_loss;
-    a.from = d_from, a.filter = d_filter, a.per_board = d_per_board, a.n_moves = n_moves, a.workspace = d_workspace;
+    a.from = d_from, a.filter = d_filter, a.per_board = d_per_board, a.n_moves = n_moves;
     if (n && !d_per_board) return bf::fail(BF_E_ARG, "bf_policy_move_loss: null pointer");
-    if (int r = check_loss(c, &a, false, workspace_bytes, "bf_policy_move_loss")) return r;
+    if (int r = check_loss(c, &a, false, 0, "bf_policy_move_loss")) return r;
     return run_loss(c, a, stream);
 }
 

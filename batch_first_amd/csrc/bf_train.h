@@ -23,10 +23,10 @@ struct PolicyLossArgs {
     float* loss;                  // [n], may be null beside a gradient
     void* d_features;
     void* d_kernel;
-    void* workspace;              // policy_loss_workspace bytes, 16-byte aligned
+    void* workspace;              // with d_kernel: policy_loss_workspace bytes, 16-byte aligned
     int* err;                     // sticky flag, bit 8: target or move list out of range
 };
-size_t policy_loss_workspace(size_t n, bool moves, bool kernel_grad);
+size_t policy_loss_workspace(size_t n);
 hipError_t launch_policy_loss(const PolicyLossArgs& args, hipStream_t stream);
 
 // The norm over tensors of mixed types, and with `clip` scaling them in place to `limit` (grad_norm.hip).

@@ -7,7 +7,9 @@
 //     dX[c][s] = sum_f W[c][f] d[f][s]                     dW[c][f] = sum over boards and s of X[c][s] d[f][s]
 //
 // where the softmax runs over the whole vocabulary (k_policy_loss) or over the board's own list of moves
-// (k_policy_move_loss).  A board without a target has loss 0 and no part in the gradients.
+// (k_policy_move_loss).  A board without a target has loss 0 and no part in the gradients.  Both keep one board in one
+// wave, so that its result does not depend on its place in the batch, and sum dW over a wave's boards, then over a
+// workgroup's waves, then over the workgroups (k_sum_parts), each in fixed order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -19,29 +21,6 @@ namespace bf {
 namespace {
 
 constexpr int kC = 32, kS = 64, kF = 73, kVocab = kF * kS, kXW = kC * kF;
-constexpr int kThreads = 256;
-constexpr unsigned kMaxGrid = 1024;   // workgroups of a gradient call: as many partial kernel gradients
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-// Over the workgroup's four waves, in fixed order; `red` holds four floats.
-template <bool MAX>
-__device__ __forceinline__ float block_reduce(float v, float* red) {
-    v = MAX ? wave_max(v) : wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return MAX ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
-}
-
 // ---- the whole vocabulary --------------------------------------------------------------------------------------------
 //
 // One wave a board, everything between the features and the gradients in its registers, on 16x16x32 MFMAs with float32
@@ -454,88 +433,244 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
 }
 
 // ---- the boards' own moves -------------------------------------------------------------------------------------------
+//
+// One wave a board, one lane a move (64 at a time), the board's features and the kernel in LDS.  A list of 32 moves needs
+// a hundredth of the vocabulary's products, so they are plain float32 sums; what bounds the kernel is reading the features and
+// writing their gradient, and next to it LDS.  A lane holds a move's logit; then 32 lanes a move, two moves at a time,
+// add the move's part to the kernel's gradient (kept in LDS over all the wave's boards) and to the features' gradient
+// (which takes the features' place).  LDS adds of one wave happen in order, and two moves that would meet in one
+// instruction take turns, so the sums are the same every time.
+//
+// A wave's boards are neighbours: it finds where its lists begin by adding up the counts of all boards before it, a
+// byte a board beside the 8 to 16 KB that each board costs, and needs no pass over them beforehand.
 
-// start[b] = moves of the boards before b, start[n] = all moves; one workgroup.
-__global__ __launch_bounds__(1024) void k_move_starts(const uint8_t* __restrict__ per, size_t n, size_t n_moves,
-                                                      uint64_t* __restrict__ start, int* __restrict__ err) {
-    __shared__ unsigned s[1024];
-    uint64_t base = 0;
-    for (size_t lo = 0; lo < n; lo += 1024) {
-        const unsigned mine = lo + threadIdx.x < n ? per[lo + threadIdx.x] : 0u;
-        s[threadIdx.x] = mine;
-        __syncthreads();
-        for (int o = 1; o < 1024; o <<= 1) {
-            const unsigned v = (int)threadIdx.x >= o ? s[threadIdx.x - o] : 0u;
-            __syncthreads();
-            s[threadIdx.x] += v;
-            __syncthreads();
-        }
-        if (lo + threadIdx.x < n) start[lo + threadIdx.x] = base + s[threadIdx.x] - mine;
-        base += s[1023];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        start[n] = base;
-        if (base != n_moves) atomicOr(err, 8);
-    }
+constexpr int kHeadRow = 36;                     // floats a filter of the kernel in LDS
+constexpr int kXRow = 68;                        // floats a channel of the features, from square to square
+constexpr int kGRow = 33;                        // floats a square of their gradient, from channel to channel
+constexpr int kMoveHeadBytes = kF * kHeadRow * 4 + 16 * 8;
+constexpr int kMoveWaveBytes = kC * kXRow * 4 + 64 * 8;
+constexpr int kMoveGradBytes = kMoveWaveBytes + kF * kC * 4;
+static_assert(kS * kGRow <= kC * kXRow, "the gradient takes the features' place");
+
+struct __attribute__((packed)) Bytes16 { unsigned v[4]; };
+
+template <typename T>
+struct Raw;                                      // four neighbours as they lie
+template <> struct Raw<float> { typedef f32x4 type; };
+template <> struct Raw<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
+template <> struct Raw<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
+
+__device__ __forceinline__ unsigned lanes_add(unsigned v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ void lds_fence() {    // orders a wave's own LDS accesses for the compiler; the hardware keeps order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 template <typename T, bool GRAD>
-__global__ __launch_bounds__(kThreads) void k_policy_move_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
-                                                               const uint8_t* __restrict__ from, const uint8_t* __restrict__ filter,
-                                                               size_t n_moves, const uint64_t* __restrict__ start,
-                                                               const int64_t* __restrict__ targets, const float* __restrict__ weights,
-                                                               unsigned weight_step, float* __restrict__ loss, T* __restrict__ dx,
-                                                               float* __restrict__ dw_part, int* __restrict__ err) {
-    __shared__ float sx[kC * kS], sw[kXW], sd[kThreads], red[4];
-    __shared__ int ss[kThreads], sf[kThreads];
-    const int tid = threadIdx.x;
-    for (int i = tid; i < kXW; i += kThreads) sw[i] = (float)w[i];
-    float acc[(kXW + kThreads - 1) / kThreads] = {};
-    for (size_t b = blockIdx.x; b < n; b += gridDim.x) {
-        __syncthreads();
-        for (int i = tid; i < kC * kS; i += kThreads) sx[i] = (float)x[b * (kC * kS) + i];
-        __syncthreads();
-        const uint64_t lo = min(start[b], (uint64_t)n_moves), hi = min(start[b + 1], (uint64_t)n_moves);
-        const int cnt = (int)(hi - lo);   // at most 255
-        float l = -INFINITY;
-        if (tid < cnt) {
-            int s = from[lo + tid], f = filter[lo + tid];
-            if (s >= kS || f >= kF) atomicOr(err, 8);
-            s = min(s, kS - 1);
-            f = min(f, kF - 1);
-            l = 0.0f;
-            for (int c = 0; c < kC; ++c) l = fmaf(sw[c * kF + f], sx[c * kS + s], l);
-            ss[tid] = s;
-            sf[tid] = f;
+__global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
+                                                          const uint8_t* __restrict__ from, const uint8_t* __restrict__ filter,
+                                                          const uint8_t* __restrict__ per, size_t n_moves,
+                                                          const int64_t* __restrict__ targets, const float* __restrict__ weights,
+                                                          unsigned weight_step, float* __restrict__ loss, T* __restrict__ dx,
+                                                          float* __restrict__ dw_part, int* __restrict__ err) {
+    typedef typename Raw<T>::type raw_t;
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* head = reinterpret_cast<float*>(smem);
+    uint64_t* red = reinterpret_cast<uint64_t*>(smem + kF * kHeadRow * 4);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int col = lane & 15, q = lane >> 4, chan = lane & 31, half = lane >> 5;
+    unsigned char* mine = smem + kMoveHeadBytes + wave * (GRAD ? kMoveGradBytes : kMoveWaveBytes);
+    float* xs = reinterpret_cast<float*>(mine);                                  // [32][68]
+    u32x2* entry = reinterpret_cast<u32x2*>(mine + kC * kXRow * 4);              // [64] (square | filter << 8, gradient)
+    float* dws = reinterpret_cast<float*>(mine + kMoveWaveBytes);                // [73][32], gradient calls only
+
+    const size_t all = (size_t)gridDim.x * waves, me = (size_t)blockIdx.x * waves + wave;
+    const size_t lo = n * me / all, hi = n * (me + 1) / all, group_lo = n * (me - wave) / all;
+
+    for (int i = tid; i < kXW; i += blockDim.x) head[(i % kF) * kHeadRow + i / kF] = (float)w[i];
+    if (GRAD)
+        for (int i = lane; i < kF * kC; i += 64) dws[i] = 0.0f;
+    unsigned before = 0;
+    for (size_t i = (size_t)tid * 16; i < group_lo; i += (size_t)blockDim.x * 16) {
+        if (i + 16 <= group_lo) {
+            const Bytes16 p = *reinterpret_cast<const Bytes16*>(per + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) before = __builtin_amdgcn_sad_u8(p.v[k], 0u, before);
+        } else {
+            for (size_t k = i; k < group_lo; ++k) before += per[k];
         }
-        const float top = block_reduce<true>(l, red);
-        const float e = tid < cnt ? expf(l - top) : 0.0f;
-        const float z = block_reduce<false>(e, red);
-        const int64_t t = targets[b];
-        const bool has = t >= 0 && t < cnt;
-        if (tid == 0) {
-            if (t < -1 || t >= cnt) atomicOr(err, 8);
-            if (loss && !has) loss[b] = 0.0f;
-        }
-        if (loss && has && tid == t) loss[b] = logf(z) + top - l;
-        if (!GRAD) continue;
-        sd[tid] = has ? (e / z - (tid == t ? 1.0f : 0.0f)) * weights[b * weight_step] : 0.0f;
-        __syncthreads();
-        if (dx)
-            for (int i = tid; i < kC * kS; i += kThreads) {
-                float a = 0.0f;
-                for (int m = 0; m < cnt; ++m)
-                    if (ss[m] == (i & 63)) a = fmaf(sw[(i >> 6) * kF + sf[m]], sd[m], a);
-                dx[b * (kC * kS) + i] = (T)a;
-            }
-        if (dw_part && has)
-            for (int k = 0, i = tid; i < kXW; i += kThreads, ++k)
-                for (int m = 0; m < cnt; ++m)
-                    if (sf[m] == i % kF) acc[k] = fmaf(sx[(i / kF) * kS + ss[m]], sd[m], acc[k]);
     }
-    if (GRAD && dw_part)
-        for (int k = 0, i = tid; i < kXW; i += kThreads, ++k) dw_part[(size_t)blockIdx.x * kXW + i] = acc[k];
+    before = lanes_add(before);
+    if (lane == 0) red[wave] = before;
+    before = 0;
+    for (size_t i = group_lo + lane; i < lo; i += 64) before += per[i];
+    uint64_t start = lanes_add(before);
+    __syncthreads();
+    for (int i = 0; i < waves; ++i) start += red[i];
+
+    raw_t raw[8];
+    auto load = [&](size_t b) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const raw_t*>(x + b * (kC * kS) + (4 * i + q) * kS + 4 * col);
+    };
+    if (lo < hi) load(lo);
+    unsigned counts = 0;
+    for (size_t b = lo; b < hi; ++b) {
+        if (((b - lo) & 63) == 0) counts = b + lane < hi ? per[b + lane] : 0u;
+        const unsigned listed = __builtin_amdgcn_readlane(counts, (int)((b - lo) & 63));
+        const uint64_t first = min(start, (uint64_t)n_moves);
+        const int cnt = (int)min((uint64_t)listed, n_moves - first);
+        start += listed;
+        const int64_t t64 = targets[b];
+        const int target = __builtin_amdgcn_readfirstlane(t64 >= 0 && t64 < cnt ? (int)t64 : -1);
+
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<f32x4*>(xs + (4 * i + q) * kXRow + 4 * col) = f32x4{(float)raw[i][0], (float)raw[i][1], (float)raw[i][2], (float)raw[i][3]};
+        if (b + 1 < hi) load(b + 1);
+        lds_fence();
+
+        float l[4];                              // [pass of 64 moves]
+        unsigned place[4];
+        float top = -INFINITY, l_target = 0.0f;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            l[p] = -INFINITY;
+            place[p] = 0;
+            if (64 * p >= cnt) continue;
+            if (64 * p + lane < cnt) {
+                unsigned s = from[first + 64 * p + lane], f = filter[first + 64 * p + lane];
+                if (s >= kS || f >= kF) atomicOr(err, 8);
+                s = min(s, kS - 1u);
+                f = min(f, kF - 1u);
+                place[p] = s | f << 8;
+                float a = 0.0f;
+#pragma unroll
+                for (int c = 0; c < kC; c += 4) {
+                    const f32x4 k = *reinterpret_cast<const f32x4*>(head + f * kHeadRow + c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) a = fmaf(k[i], xs[(c + i) * kXRow + s], a);
+                }
+                l[p] = a;
+            }
+            top = larger(top, l[p]);
+            if (target >> 6 == p) l_target = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l[p]), target & 63));
+        }
+        if (target < 0) {                        // no part in anything, whatever the features hold
+            if (lane == 0) {
+                if (t64 != -1) atomicOr(err, 8);
+                if (loss) loss[b] = 0.0f;
+            }
+            if (GRAD && dx) {
+                u32x4* out = reinterpret_cast<u32x4*>(dx + b * (kC * kS));
+#pragma unroll
+                for (int i = 0; i < (int)(kC * kS * sizeof(T) / 1024); ++i) out[i * 64 + lane] = u32x4{0, 0, 0, 0};
+            }
+            lds_fence();
+            continue;
+        }
+        top = lanes_reduce<true>(top);
+        float z = 0.0f;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            if (64 * p >= cnt) continue;
+            l[p] = __builtin_amdgcn_exp2f((l[p] - top) * 1.44269504088896341f);
+            z += l[p];
+        }
+        z = lanes_reduce<false>(z);
+        if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, top - l_target);
+        if (!GRAD) {
+            lds_fence();
+            continue;
+        }
+
+        const float wb = weights[b * weight_step], rz = __builtin_amdgcn_rcpf(z);
+        // entries k and k + `apart` of a pass are taken together
+        auto lay_out = [&](int p, int& pairs, uint64_t& same_square, uint64_t& same_filter) {
+            const float one = target == 64 * p + lane ? z : 0.0f;
+            lds_fence();
+            entry[lane] = u32x2{place[p], __float_as_uint((l[p] - one) * rz * wb)};
+            lds_fence();
+            const int here = min(cnt - 64 * p, 64);
+            pairs = (here + 1) >> 1;
+            const unsigned other = entry[(lane + pairs) & 63][0] ^ place[p];
+            const bool pair = lane < pairs && lane + pairs < here;
+            same_square = __ballot(pair && (other & 0xff) == 0);
+            same_filter = __ballot(pair && other >> 8 == 0);
+        };
+        int pairs;
+        uint64_t same_square, same_filter;
+        if (dw_part) {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                if (64 * p >= cnt) continue;
+                lay_out(p, pairs, same_square, same_filter);
+                const int here = min(cnt - 64 * p, 64);
+                for (int k = 0; k < pairs; ++k) {
+                    const int m = k + half * pairs;
+                    const u32x2 e = entry[min(m, 63)];
+                    const float v = xs[chan * kXRow + (e[0] & 0xff)] * __uint_as_float(e[1]);
+                    float* at = dws + (e[0] >> 8) * kC + chan;
+                    if (same_filter >> k & 1) {
+                        if (half == 0) unsafeAtomicAdd(at, v);
+                        __builtin_amdgcn_wave_barrier();
+                        if (half == 1) unsafeAtomicAdd(at, v);
+                    } else if (m < here) {
+                        unsafeAtomicAdd(at, v);
+                    }
+                }
+            }
+        }
+        if (dx) {
+            lds_fence();
+            float* g = xs;                       // [64][33]
+            for (int i = lane; i < kS * kGRow; i += 64) g[i] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                if (64 * p >= cnt) continue;
+                lay_out(p, pairs, same_square, same_filter);
+                const int here = min(cnt - 64 * p, 64);
+                for (int k = 0; k < pairs; ++k) {
+                    const int m = k + half * pairs;
+                    const u32x2 e = entry[min(m, 63)];
+                    const float v = head[(e[0] >> 8) * kHeadRow + chan] * __uint_as_float(e[1]);
+                    float* at = g + (e[0] & 0xff) * kGRow + chan;
+                    if (same_square >> k & 1) {
+                        if (half == 0) unsafeAtomicAdd(at, v);
+                        __builtin_amdgcn_wave_barrier();
+                        if (half == 1) unsafeAtomicAdd(at, v);
+                    } else if (m < here) {
+                        unsafeAtomicAdd(at, v);
+                    }
+                }
+            }
+            lds_fence();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                raw_t out;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) out[j] = (T)g[(4 * col + j) * kGRow + 4 * i + q];
+                *reinterpret_cast<raw_t*>(dx + b * (kC * kS) + (4 * i + q) * kS + 4 * col) = out;
+            }
+        }
+        lds_fence();
+    }
+    if (lo < hi && hi == n && lane == 0 && start != n_moves) atomicOr(err, 8);
+
+    if (GRAD && dw_part) {
+        __syncthreads();
+        for (int i = tid; i < kXW; i += blockDim.x) {
+            const int c = i / kF, f = i % kF;
+            float a = 0.0f;
+            for (int k = 0; k < waves; ++k)
+                a += reinterpret_cast<const float*>(smem + kMoveHeadBytes + k * kMoveGradBytes + kMoveWaveBytes)[f * kC + c];
+            dw_part[(size_t)blockIdx.x * kXW + i] = a;
+        }
+    }
 }
 
 // The partial kernel gradients of the workgroups, added up in fixed order: a workgroup 32 elements, eight threads each.
@@ -555,7 +690,7 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ par
 }
 static_assert(kXW % 32 == 0, "k_sum_parts needs no bounds check");
 
-constexpr unsigned kGroups = 256;   // workgroups of a gradient call over the vocabulary: one a compute unit
+constexpr unsigned kGroups = 256;   // workgroups of a gradient call: one a compute unit, each with a part of the kernel's gradient
 
 // Waves a workgroup: small calls are spread over the compute units.
 unsigned waves_for(size_t n, unsigned most) {
@@ -564,55 +699,33 @@ unsigned waves_for(size_t n, unsigned most) {
     return waves;
 }
 
-template <typename T>
-hipError_t launch_vocabulary(const PolicyLossArgs& a, float* part, unsigned* parts, hipStream_t s) {
-    const T *x = static_cast<const T*>(a.features), *w = static_cast<const T*>(a.kernel);
-    if (a.d_features || part) {
-        const unsigned waves = waves_for(a.n, 8), lds = sizeof(HeadLds<T>) + waves * kWaveLds;
-        *parts = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, kGroups);
-        hipLaunchKernelGGL((k_policy_loss<T, true>), dim3(*parts), dim3(waves * 64), lds, s, x, w, a.n, a.targets, a.weights,
-                           a.n_weights > 1 ? 1u : 0u, a.loss, static_cast<T*>(a.d_features), part, a.err);
-    } else {
-        const unsigned waves = waves_for(a.n, 4);
-        hipLaunchKernelGGL((k_policy_loss<T, false>), dim3((unsigned)std::min<size_t>((a.n + waves - 1) / waves, 4 * kGroups)),
-                           dim3(waves * 64), sizeof(HeadLds<T>), s, x, w, a.n, a.targets, nullptr, 0u, a.loss, nullptr, nullptr, a.err);
-    }
-    return hipGetLastError();
-}
-
-unsigned grid_for(size_t n) { return (unsigned)(n < kMaxGrid ? n : kMaxGrid); }
-
-template <typename T>
+template <typename T, bool GRAD>
 hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
     const T *x = static_cast<const T*>(a.features), *w = static_cast<const T*>(a.kernel);
     T* dx = static_cast<T*>(a.d_features);
-    const bool grad = a.d_features || a.d_kernel;
-    unsigned grid = grid_for(a.n);
-    const unsigned step = a.n_weights > 1 ? 1u : 0u;
-    uint64_t* start = static_cast<uint64_t*>(a.workspace);
-    float* part = a.d_kernel ? reinterpret_cast<float*>(a.per_board ? start + (a.n + 2) / 2 * 2 : start) : nullptr;
-    if (grid && a.per_board) {
-        hipLaunchKernelGGL(k_move_starts, dim3(1), dim3(1024), 0, s, a.per_board, a.n, a.n_moves, start, a.err);
-        if (grad)
-            hipLaunchKernelGGL((k_policy_move_loss<T, true>), dim3(grid), dim3(kThreads), 0, s, x, w, a.n, a.from, a.filter, a.n_moves,
-                               start, a.targets, a.weights, step, a.loss, dx, part, a.err);
-        else
-            hipLaunchKernelGGL((k_policy_move_loss<T, false>), dim3(grid), dim3(kThreads), 0, s, x, w, a.n, a.from, a.filter, a.n_moves,
-                               start, a.targets, nullptr, 0u, a.loss, nullptr, nullptr, a.err);
-    } else if (grid) {
-        hipError_t e = launch_vocabulary<T>(a, part, &grid, s);
-        if (e != hipSuccess) return e;
-    }
-    if (a.d_kernel)
-        hipLaunchKernelGGL(k_sum_parts<T>, dim3(kXW / 32), dim3(256), 0, s, part, grid, static_cast<T*>(a.d_kernel));
+    float* part = a.d_kernel ? static_cast<float*>(a.workspace) : nullptr;
+    const unsigned waves = waves_for(a.n, GRAD ? 8 : 4), step = a.n_weights > 1 ? 1u : 0u;
+    const unsigned grid = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, GRAD ? kGroups : 4 * kGroups);
+    if (grid && a.per_board)
+        hipLaunchKernelGGL((k_policy_move_loss<T, GRAD>), dim3(grid), dim3(waves * 64),
+                           kMoveHeadBytes + waves * (GRAD ? kMoveGradBytes : kMoveWaveBytes), s, x, w, a.n, a.from, a.filter, a.per_board,
+                           a.n_moves, a.targets, a.weights, step, a.loss, dx, part, a.err);
+    else if (grid)
+        hipLaunchKernelGGL((k_policy_loss<T, GRAD>), dim3(grid), dim3(waves * 64), sizeof(HeadLds<T>) + (GRAD ? waves * kWaveLds : 0), s,
+                           x, w, a.n, a.targets, a.weights, step, a.loss, dx, part, a.err);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (a.d_kernel) hipLaunchKernelGGL(k_sum_parts<T>, dim3(kXW / 32), dim3(256), 0, s, part, grid, static_cast<T*>(a.d_kernel));
     return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
+    return a.d_features || a.d_kernel ? launch<T, true>(a, s) : launch<T, false>(a, s);
 }
 
 }  // namespace
 
-size_t policy_loss_workspace(size_t n, bool moves, bool kernel_grad) {
-    return (moves ? (n + 2) / 2 * 2 * sizeof(uint64_t) : 0) + (kernel_grad ? (size_t)grid_for(n) * kXW * sizeof(float) : 0);
-}
+size_t policy_loss_workspace(size_t n) { return std::min<size_t>(n, kGroups) * kXW * sizeof(float); }
 
 hipError_t launch_policy_loss(const PolicyLossArgs& a, hipStream_t stream) {
     if (a.type == BF_TYPE_F32) return launch<float>(a, stream);

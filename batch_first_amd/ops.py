@@ -265,11 +265,8 @@ def _board_weights(c, board_weights, n):
 def _loss(name, c, x, w, t, lists):
     n = x.shape[0]
     loss = torch.empty(n, dtype=torch.float32, device=x.device)
-    args = [c._ctx, x.data_ptr(), _TYPES[x.dtype], n, w.data_ptr(), *lists, t.data_ptr(), loss.data_ptr()]
-    if lists:
-        work = torch.empty(c._lib.bf_policy_move_loss_workspace(n), dtype=torch.uint8, device=x.device)
-        args += [work.data_ptr(), work.numel()]
-    _lib.check(getattr(c._lib, name)(*args, _stream(x.device)))
+    _lib.check(getattr(c._lib, name)(c._ctx, x.data_ptr(), _TYPES[x.dtype], n, w.data_ptr(), *lists, t.data_ptr(), loss.data_ptr(),
+                                     _stream(x.device)))
     return loss
 
 
@@ -279,7 +276,7 @@ def _loss_grad(name, c, x, w, t, lists, board_weights, features_grad, kernel_gra
     loss = torch.empty(n, dtype=torch.float32, device=x.device)
     dx = torch.empty_like(x) if features_grad else x.new_empty(0)
     dw = torch.empty_like(w) if kernel_grad else w.new_empty(0)
-    work = torch.empty(getattr(c._lib, name + "_workspace")(n), dtype=torch.uint8, device=x.device)
+    work = torch.empty(c._lib.bf_policy_loss_workspace(n) if kernel_grad else 0, dtype=torch.uint8, device=x.device)
     _lib.check(getattr(c._lib, name + "_grad")(
         c._ctx, x.data_ptr(), _TYPES[x.dtype], n, w.data_ptr(), *lists, t.data_ptr(), g.data_ptr(), g.numel(), loss.data_ptr(),
         dx.data_ptr() if features_grad else None, dw.data_ptr() if kernel_grad else None, work.data_ptr(), work.numel(),

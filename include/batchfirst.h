@@ -312,7 +312,7 @@ int bf_policy_loss(bf_ctx* ctx, const void* d_features, int type, size_t n, cons
 /* The same with the gradients of sum_b weights[b] * loss[b], in one pass over the features.  d_weights holds n_weights
  * floats: n, or one for all boards.  d_loss, d_features_grad and d_kernel_grad may be NULL (not wanted), not all three.
  * A board without a target leaves zeros in its rows of d_features_grad, whatever its features hold.
- * d_workspace: bf_policy_loss_workspace(n) bytes. */
+ * d_workspace: bf_policy_loss_workspace(n) bytes; not needed without d_kernel_grad. */
 size_t bf_policy_loss_workspace(size_t n);
 int bf_policy_loss_grad(bf_ctx* ctx, const void* d_features, int type, size_t n, const void* d_logit_kernel,
                         const int64_t* d_targets, const float* d_weights, size_t n_weights, float* d_loss,
@@ -322,13 +322,10 @@ int bf_policy_loss_grad(bf_ctx* ctx, const void* d_features, int type, size_t n,
  * d_from_square and d_move_filter uint8 [n_moves], boards back to back, d_moves_per_board uint8 [n].  A target is a place
  * in the board's own list, or -1; a board with no moves has none.  A move listed twice counts twice.  Out-of-range
  * squares and filters are clamped, targets beyond the list count as -1, moves beyond n_moves are absent; each of these,
- * and a sum of d_moves_per_board other than n_moves, is reported by bf_policy_check().
- * d_workspace: bf_policy_move_loss_workspace(n) bytes, for both. */
-size_t bf_policy_move_loss_workspace(size_t n);
+ * and a sum of d_moves_per_board other than n_moves, is reported by bf_policy_check(). */
 int bf_policy_move_loss(bf_ctx* ctx, const void* d_features, int type, size_t n, const void* d_logit_kernel,
                         const uint8_t* d_from_square, const uint8_t* d_move_filter, const uint8_t* d_moves_per_board,
-                        size_t n_moves, const int64_t* d_targets, float* d_loss, void* d_workspace, size_t workspace_bytes,
-                        void* stream);
+                        size_t n_moves, const int64_t* d_targets, float* d_loss, void* stream);
 int bf_policy_move_loss_grad(bf_ctx* ctx, const void* d_features, int type, size_t n, const void* d_logit_kernel,
                              const uint8_t* d_from_square, const uint8_t* d_move_filter, const uint8_t* d_moves_per_board,
                              size_t n_moves, const int64_t* d_targets, const float* d_weights, size_t n_weights, float* d_loss,

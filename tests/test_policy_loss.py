@@ -114,7 +114,7 @@ def test_refusals_of_the_c_entry_points():
     lib, ctx = _lib.load(), _fake_context()
     buf = ctypes.create_string_buffer(1 << 16)
     p = (ctypes.addressof(buf) + 255) & ~255
-    big = lib.bf_policy_move_loss_workspace(2)
+    big = lib.bf_policy_loss_workspace(2)
 
     def refused(rc, text):
         assert rc == _lib.BF_E_ARG and text in lib.bf_last_error().decode(), lib.bf_last_error()
@@ -140,19 +140,18 @@ def test_refusals_of_the_c_entry_points():
     refused(grad(out=None, dx=None, dk=None), "no output")
     refused(grad(dx=p + 2), "aligned")
     refused(grad(ws=p + 8), "aligned")
-    refused(grad(size=lib.bf_policy_loss_workspace(2) - 1), "workspace")
+    refused(grad(size=big - 1), "workspace")
     refused(grad(ws=None), "workspace")
 
-    def moves(n=2, frm=p, flt=p, per=p, m=4, ws=p, size=big):
-        return lib.bf_policy_move_loss(ctx, p, 0, n, p, frm, flt, per, m, p, p, ws, size, None)
+    def moves(n=2, frm=p, flt=p, per=p, m=4):
+        return lib.bf_policy_move_loss(ctx, p, 0, n, p, frm, flt, per, m, p, p, None)
 
     refused(moves(frm=None), "null pointer")
     refused(moves(flt=None), "null pointer")
     refused(moves(per=None), "null pointer")
     refused(moves(m=(1 << 31) + 1), "2^31")
     refused(moves(n=0, per=None), "moves given without boards")
-    refused(moves(size=0), "workspace")
-    refused(lib.bf_policy_move_loss_grad(ctx, p, 0, 2, p, p, p, p, 4, p, p, 2, p, p, p, p, lib.bf_policy_move_loss_workspace(2) - 1, None),
+    refused(lib.bf_policy_move_loss_grad(ctx, p, 0, 2, p, p, p, p, 4, p, p, 2, p, p, p, p, big - 1, None),
             "workspace")
 
 
