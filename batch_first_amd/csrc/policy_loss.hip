@@ -438,8 +438,9 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
 // a hundredth of the vocabulary's products, so they are plain float32 sums; what bounds the kernel is reading the features and
 // writing their gradient, and next to it LDS.  A lane holds a move's logit; then 32 lanes a move, two moves at a time,
 // add the move's part to the kernel's gradient (kept in LDS over all the wave's boards) and to the features' gradient
-// (which takes the features' place).  LDS adds of one wave happen in order, and two moves that would meet in one
-// instruction take turns, so the sums are the same every time.
+// (which takes the features' place).  Two moves that would meet take turns, so the sums are the same
+// every time.  (LDS's own float adds do the same in one instruction, but take 200 cycles each: 0.88 ms in place of
+// 0.35 for 65 536 boards.)
 //
 // A wave's boards are neighbours: it finds where its lists begin by adding up the counts of all boards before it, a
 // byte a board beside the 8 to 16 KB that each board costs, and needs no pass over them beforehand.
@@ -589,65 +590,48 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
         }
 
         const float wb = weights[b * weight_step], rz = __builtin_amdgcn_rcpf(z);
-        // entries k and k + `apart` of a pass are taken together
-        auto lay_out = [&](int p, int& pairs, uint64_t& same_square, uint64_t& same_filter) {
+        // One pass's moves, two at a time: move k by the lower lanes, move k + pairs by the upper ones.  to(place) is where
+        // a lane adds to, of(place) what of times the logit's gradient it adds; meet(a, b): two moves add to the same.
+        auto add_up = [&](int p, auto&& to, auto&& of, auto&& meet) {
+            const int here = min(cnt - 64 * p, 64), pairs = (here + 1) >> 1;
             const float one = target == 64 * p + lane ? z : 0.0f;
             lds_fence();
             entry[lane] = u32x2{place[p], __float_as_uint((l[p] - one) * rz * wb)};
             lds_fence();
-            const int here = min(cnt - 64 * p, 64);
-            pairs = (here + 1) >> 1;
-            const unsigned other = entry[(lane + pairs) & 63][0] ^ place[p];
-            const bool pair = lane < pairs && lane + pairs < here;
-            same_square = __ballot(pair && (other & 0xff) == 0);
-            same_filter = __ballot(pair && other >> 8 == 0);
-        };
-        int pairs;
-        uint64_t same_square, same_filter;
-        if (dw_part) {
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                if (64 * p >= cnt) continue;
-                lay_out(p, pairs, same_square, same_filter);
-                const int here = min(cnt - 64 * p, 64);
-                for (int k = 0; k < pairs; ++k) {
-                    const int m = k + half * pairs;
-                    const u32x2 e = entry[min(m, 63)];
-                    const float v = xs[chan * kXRow + (e[0] & 0xff)] * __uint_as_float(e[1]);
-                    float* at = dws + (e[0] >> 8) * kC + chan;
-                    if (same_filter >> k & 1) {
-                        if (half == 0) unsafeAtomicAdd(at, v);
-                        __builtin_amdgcn_wave_barrier();
-                        if (half == 1) unsafeAtomicAdd(at, v);
-                    } else if (m < here) {
-                        unsafeAtomicAdd(at, v);
-                    }
+            const uint64_t turns = __ballot(lane + pairs < here && meet(entry[(lane + pairs) & 63][0], place[p]));
+            u32x2 e = entry[half * pairs];
+            float v = of(e[0]) * __uint_as_float(e[1]);
+            for (int k = 0; k < pairs; ++k) {
+                float* at = to(e[0]);
+                const float was = *at;
+                e = entry[min(k + 1 + half * pairs, 63)];
+                const float next = of(e[0]) * __uint_as_float(e[1]);   // in flight while this one is added
+                if (turns >> k & 1) {
+                    if (half == 0) *at = was + v;
+                    lds_fence();
+                    if (half == 1) *at += v;
+                } else if (k + half * pairs < here) {
+                    *at = was + v;
                 }
+                lds_fence();
+                v = next;
             }
-        }
+        };
+        if (dw_part)
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+                if (64 * p < cnt)
+                    add_up(p, [&](unsigned m) { return dws + (m >> 8) * kC + chan; }, [&](unsigned m) { return xs[chan * kXRow + (m & 0xff)]; },
+                           [](unsigned a, unsigned b) { return a >> 8 == b >> 8; });
         if (dx) {
             lds_fence();
             float* g = xs;                       // [64][33]
             for (int i = lane; i < kS * kGRow; i += 64) g[i] = 0.0f;
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                if (64 * p >= cnt) continue;
-                lay_out(p, pairs, same_square, same_filter);
-                const int here = min(cnt - 64 * p, 64);
-                for (int k = 0; k < pairs; ++k) {
-                    const int m = k + half * pairs;
-                    const u32x2 e = entry[min(m, 63)];
-                    const float v = head[(e[0] >> 8) * kHeadRow + chan] * __uint_as_float(e[1]);
-                    float* at = g + (e[0] & 0xff) * kGRow + chan;
-                    if (same_square >> k & 1) {
-                        if (half == 0) unsafeAtomicAdd(at, v);
-                        __builtin_amdgcn_wave_barrier();
-                        if (half == 1) unsafeAtomicAdd(at, v);
-                    } else if (m < here) {
-                        unsafeAtomicAdd(at, v);
-                    }
-                }
-            }
+            for (int p = 0; p < 4; ++p)
+                if (64 * p < cnt)
+                    add_up(p, [&](unsigned m) { return g + (m & 0xff) * kGRow + chan; }, [&](unsigned m) { return head[(m >> 8) * kHeadRow + chan]; },
+                           [](unsigned a, unsigned b) { return (a & 0xff) == (b & 0xff); });
             lds_fence();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
