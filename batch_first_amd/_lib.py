@@ -80,7 +80,7 @@ SIGNATURES = {
     "bf_policy_loss_grad": (_int, [_vp, _vp, _int, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
     "bf_policy_move_loss": (_int, [_vp, _vp, _int, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp]),
     "bf_policy_move_loss_grad": (_int, [_vp, _vp, _int, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "bf_grad_norm_workspace": (_sz, [_vp, _sz]),
+    "bf_grad_norm_workspace": (_sz, [_sz]),
     "bf_global_norm": (_int, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp]),
     "bf_clip_grad_norm": (_int, [_vp, _vp, _vp, _vp, _sz, _c.c_float, _vp, _vp, _sz, _vp]),
     "bf_packed_t16_bytes": (_sz, []),

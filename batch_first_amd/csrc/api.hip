@@ -996,17 +996,18 @@ int check_norm(const bf_ctx* c, const void* const* ptrs, const size_t* counts, c
                const void* workspace, size_t workspace_bytes, const char* who) {
     if (!c) return bf::fail(BF_E_ARG, "%s: null context", who);
     if (!d_norm || !workspace || (n && (!ptrs || !counts || !types))) return bf::fail(BF_E_ARG, "%s: null pointer", who);
+    if (n > ((size_t)1 << 20)) return bf::fail(BF_E_ARG, "%s: %zu tensors exceeds the limit of 2^20", who, n);
     for (size_t i = 0; i < n; ++i) {
         if (types[i] != BF_TYPE_F32 && types[i] != BF_TYPE_BF16 && types[i] != BF_TYPE_F16)
             return bf::fail(BF_E_ARG, "%s: tensor %zu has unknown element type %d", who, i, types[i]);
         if (!counts[i]) continue;
-        if (counts[i] > ((size_t)1 << 40)) return bf::fail(BF_E_ARG, "%s: tensor %zu has %zu elements, more than 2^40", who, i, counts[i]);
+        if (counts[i] > ((size_t)1 << 37)) return bf::fail(BF_E_ARG, "%s: tensor %zu has %zu elements, more than 2^37", who, i, counts[i]);
         if (!ptrs[i]) return bf::fail(BF_E_ARG, "%s: tensor %zu is a null pointer", who, i);
         if (reinterpret_cast<uintptr_t>(ptrs[i]) & (types[i] == BF_TYPE_F32 ? 3u : 1u))
             return bf::fail(BF_E_ARG, "%s: tensor %zu is not aligned to its elements", who, i);
     }
     if (!aligned16(workspace)) return bf::fail(BF_E_ARG, "%s: the workspace must be 16-byte aligned", who);
-    const size_t need = bf::grad_norm_workspace(counts, n);
+    const size_t need = bf::grad_norm_workspace(n);
     if (workspace_bytes < need) return bf::fail(BF_E_ARG, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, need);
     return BF_OK;
 }
@@ -1057,9 +1058,7 @@ extern "C" int bf_policy_move_loss_grad(bf_ctx* c, const void* d_features, int t
     return run_loss(c, a, stream);
 }
 
-extern "C" size_t bf_grad_norm_workspace(const size_t* h_counts, size_t n_tensors) {
-    return bf::grad_norm_workspace(h_counts, h_counts ? n_tensors : 0);
-}
+extern "C" size_t bf_grad_norm_workspace(size_t n_tensors) { return bf::grad_norm_workspace(n_tensors); }
 
 extern "C" int bf_global_norm(bf_ctx* c, const void* const* h_tensors, const size_t* h_counts, const int* h_types, size_t n_tensors,
                               float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream) {

@@ -30,7 +30,7 @@ size_t policy_loss_workspace(size_t n);
 hipError_t launch_policy_loss(const PolicyLossArgs& args, hipStream_t stream);
 
 // The norm over tensors of mixed types, and with `clip` scaling them in place to `limit` (grad_norm.hip).
-size_t grad_norm_workspace(const size_t* counts, size_t n_tensors);
+size_t grad_norm_workspace(size_t n_tensors);
 hipError_t launch_grad_norm(void* const* ptrs, const size_t* counts, const int* types, size_t n_tensors, bool clip, float limit,
                             float* d_norm, void* workspace, hipStream_t stream);
 

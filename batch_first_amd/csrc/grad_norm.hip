@@ -3,7 +3,13 @@
 //     norm = sqrt(sum over tensors and elements of g^2)        g <- g * min(1, limit / (norm + 1e-6))
 //
 // Squares and sums are float64: float32 would overflow from 1.8e19 on and lose the small tensors beside the large.
+// Bound by reading (and, to scale, reading again and writing): a workgroup walks a run of 16 KB chunks, through however
+// many tensors it spans, with 16-byte accesses and four of them in flight a thread, and leaves one partial sum; every
+// workgroup of the scaling pass adds the partial sums up by itself, in the same fixed order, which spares a launch between the two.
+// The scaling pass walks its run backwards, so that it begins with what the first pass has left in the caches.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "../../include/batchfirst.h"
 #include "bf_train.h"
@@ -12,17 +18,92 @@ namespace bf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr size_t kChunk = 65536;   // elements a workgroup
-constexpr int kTable = 96;         // tensors a launch: the table travels in the kernel's arguments
+constexpr int kInFlight = 4;                                        // 16-byte accesses a thread and chunk
+constexpr size_t kChunkBytes = (size_t)kThreads * kInFlight * 16;
+constexpr int kTable = 160;        // tensors a launch: their table travels in the kernel's arguments, of which there are 4 KB
+constexpr unsigned kGroups = 2048; // workgroups a launch: eight a compute unit
+constexpr int kTypeShift = 56;
 
 struct Table {
-    void* ptr[kTable];
-    unsigned long long count[kTable];
-    unsigned first[kTable];        // first workgroup of the tensor, within the launch
-    unsigned char type[kTable];
+    char* ptr[kTable];
+    unsigned long long count[kTable];      // elements; the type in the top byte
+    unsigned first[kTable + 1];            // first chunk of each tensor, and the end
     int n;
 };
+static_assert(sizeof(Table) <= 3600, "kernel arguments");
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// A tensor of elements T as 16-byte pieces of memory; the pieces at its ends may lie partly outside.
+template <typename T>
+struct Pieces {
+    static constexpr int kPer = 16 / sizeof(T);
+    T* base;                 // 16-byte aligned, at or before the tensor
+    long long lo, hi;        // the tensor's elements are base[lo ... hi)
+    __device__ __forceinline__ Pieces(char* p, unsigned long long count) {
+        const unsigned skip = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15u);
+        base = reinterpret_cast<T*>(p - skip);
+        lo = skip / sizeof(T);
+        hi = lo + (long long)count;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ double square(T v) {
+    const double d = (double)(float)v;
+    return d * d;
+}
+
+// Pieces [at, at + kThreads * kInFlight) of a tensor: whole(i, piece) for those inside it, part(element) for the
+// elements of those that its ends cut.
+template <typename T, typename Whole, typename Part>
+__device__ __forceinline__ void chunk_of(char* p, unsigned long long count, unsigned chunk, Whole&& whole, Part&& part) {
+    typedef T piece_t __attribute__((ext_vector_type(16 / sizeof(T))));
+    constexpr int kPer = Pieces<T>::kPer;
+    const Pieces<T> t(p, count);
+    const long long at = (long long)chunk * (kThreads * kInFlight) + threadIdx.x;
+    piece_t v[kInFlight];
+    bool in[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+        const long long e = (at + i * kThreads) * kPer;
+        in[i] = e >= t.lo && e + kPer <= t.hi;
+        if (in[i]) v[i] = *reinterpret_cast<const piece_t*>(t.base + e);
+    }
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+        const long long e = (at + i * kThreads) * kPer;
+        if (in[i]) whole(reinterpret_cast<piece_t*>(t.base + e), v[i]);
+        else if (e < t.hi)
+            for (long long k = max(e, t.lo); k < min(e + kPer, t.hi); ++k) part(t.base + k);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ double squares(char* p, unsigned long long count, unsigned chunk) {
+    constexpr int kPer = Pieces<T>::kPer;
+    double a[2] = {0.0, 0.0};
+    chunk_of<T>(p, count, chunk,
+                [&](auto*, auto& v) {
+#pragma unroll
+                    for (int k = 0; k < kPer; ++k) a[k & 1] = fma((double)(float)v[k], (double)(float)v[k], a[k & 1]);
+                },
+                [&](T* e) { a[0] += square(*e); });
+    return a[0] + a[1];
+}
+
+template <typename T>
+__device__ __forceinline__ void scale(char* p, unsigned long long count, unsigned chunk, float f) {
+    chunk_of<T>(p, count, chunk,
+                [&](auto* at, auto& v) {
+#pragma unroll
+                    for (int k = 0; k < Pieces<T>::kPer; ++k) v[k] = (T)((float)v[k] * f);
+                    *at = v;
+                },
+                [&](T* e) { *e = (T)((float)*e * f); });
+}
+
+// The workgroup's sum, the same in every thread.
 __device__ __forceinline__ double block_sum(double v) {
     __shared__ double red[kThreads / 64];
 #pragma unroll
@@ -32,86 +113,93 @@ __device__ __forceinline__ double block_sum(double v) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__device__ __forceinline__ int find(const Table& t, unsigned block) {
+// The tensor that a chunk belongs to.
+__device__ __forceinline__ int find(const Table& t, unsigned chunk) {
     int lo = 0, hi = t.n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (t.first[mid] <= block) lo = mid; else hi = mid - 1;
+        if (t.first[mid] <= chunk) lo = mid; else hi = mid - 1;
     }
     return lo;
 }
 
-template <typename T>
-__device__ __forceinline__ double squares(const T* g, size_t n) {
-    double a = 0.0;
-    for (size_t i = threadIdx.x; i < n; i += kThreads) {
-        const double v = (double)(float)g[i];
-        a = fma(v, v, a);
-    }
-    return a;
+__device__ __forceinline__ void run_of(const Table& t, unsigned& lo, unsigned& hi) {
+    const unsigned long long chunks = t.first[t.n];
+    lo = (unsigned)(chunks * blockIdx.x / gridDim.x);
+    hi = (unsigned)(chunks * (blockIdx.x + 1) / gridDim.x);
 }
 
 __global__ __launch_bounds__(kThreads) void k_squares(Table t, double* __restrict__ part) {
-    const int k = find(t, blockIdx.x);
-    const size_t at = (size_t)(blockIdx.x - t.first[k]) * kChunk;
-    const size_t n = min((size_t)t.count[k] - at, kChunk);
-    double a;
-    if (t.type[k] == BF_TYPE_F32) a = squares(static_cast<const float*>(t.ptr[k]) + at, n);
-    else if (t.type[k] == BF_TYPE_BF16) a = squares(static_cast<const __bf16*>(t.ptr[k]) + at, n);
-    else a = squares(static_cast<const _Float16*>(t.ptr[k]) + at, n);
+    unsigned lo, hi;
+    run_of(t, lo, hi);
+    double a = 0.0;
+    int k = find(t, lo);
+    for (unsigned c = lo; c < hi; ++c) {
+        while (c >= t.first[k + 1]) ++k;
+        const unsigned long long count = t.count[k] & ((1ull << kTypeShift) - 1);
+        const int type = (int)(t.count[k] >> kTypeShift);
+        if (type == BF_TYPE_F32) a += squares<float>(t.ptr[k], count, c - t.first[k]);
+        else if (type == BF_TYPE_BF16) a += squares<__bf16>(t.ptr[k], count, c - t.first[k]);
+        else a += squares<_Float16>(t.ptr[k], count, c - t.first[k]);
+    }
     a = block_sum(a);
     if (threadIdx.x == 0) part[blockIdx.x] = a;
 }
 
-__global__ __launch_bounds__(kThreads) void k_norm(const double* __restrict__ part, size_t parts, float limit,
-                                                   float* __restrict__ norm, float* __restrict__ scale) {
+__device__ __forceinline__ float norm_of(const double* __restrict__ part, unsigned parts) {
     double a = 0.0;
-    for (size_t i = threadIdx.x; i < parts; i += kThreads) a += part[i];
-    a = block_sum(a);
-    if (threadIdx.x == 0) {
-        const float v = (float)sqrt(a);
-        *norm = v;
-        // a norm of NaN gives a scale of NaN, one of infinity a scale of 0, as the formula has it
-        const float f = limit / (v + 1e-6f);
-        *scale = f > 1.0f ? 1.0f : f;
+    for (unsigned i = threadIdx.x; i < parts; i += kThreads) a += part[i];
+    return (float)sqrt(block_sum(a));
+}
+
+__global__ __launch_bounds__(kThreads) void k_norm(const double* __restrict__ part, unsigned parts, float* __restrict__ norm) {
+    const float v = norm_of(part, parts);
+    if (threadIdx.x == 0) *norm = v;
+}
+
+__global__ __launch_bounds__(kThreads) void k_scale(Table t, const double* __restrict__ part, unsigned parts, float limit,
+                                                    float* __restrict__ norm) {
+    const float v = norm_of(part, parts);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
+    // a norm of NaN gives a factor of NaN, one of infinity a factor of 0, as the formula has it
+    const float f = limit / (v + 1e-6f);
+    if (f >= 1.0f) return;   // within the limit: every product would be the value itself
+    unsigned lo, hi;
+    run_of(t, lo, hi);
+    if (lo == hi) return;
+    int k = find(t, hi - 1);
+    for (unsigned c = hi; c-- > lo;) {
+        while (c < t.first[k]) --k;
+        const unsigned long long count = t.count[k] & ((1ull << kTypeShift) - 1);
+        const int type = (int)(t.count[k] >> kTypeShift);
+        if (type == BF_TYPE_F32) scale<float>(t.ptr[k], count, c - t.first[k], f);
+        else if (type == BF_TYPE_BF16) scale<__bf16>(t.ptr[k], count, c - t.first[k], f);
+        else scale<_Float16>(t.ptr[k], count, c - t.first[k], f);
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void scale_all(T* g, size_t n, float f) {
-    for (size_t i = threadIdx.x; i < n; i += kThreads) g[i] = (T)((float)g[i] * f);
+size_t chunks_of(const void* ptr, size_t count, int type) {
+    const size_t bytes = (reinterpret_cast<uintptr_t>(ptr) & 15u) + count * (type == BF_TYPE_F32 ? 4 : 2);
+    return (bytes + kChunkBytes - 1) / kChunkBytes;
 }
 
-__global__ __launch_bounds__(kThreads) void k_scale(Table t, const float* __restrict__ scale) {
-    const float f = *scale;
-    if (f == 1.0f) return;   // within the limit: every product would be the value itself
-    const int k = find(t, blockIdx.x);
-    const size_t at = (size_t)(blockIdx.x - t.first[k]) * kChunk;
-    const size_t n = min((size_t)t.count[k] - at, kChunk);
-    if (t.type[k] == BF_TYPE_F32) scale_all(static_cast<float*>(t.ptr[k]) + at, n, f);
-    else if (t.type[k] == BF_TYPE_BF16) scale_all(static_cast<__bf16*>(t.ptr[k]) + at, n, f);
-    else scale_all(static_cast<_Float16*>(t.ptr[k]) + at, n, f);
-}
-
-// Calls launch(table, workgroups) for the non-empty tensors, kTable at a time.
+// Calls launch(table, workgroups) for the non-empty tensors, kTable at a time; returns the first error.
 template <typename F>
 hipError_t tables(void* const* ptrs, const size_t* counts, const int* types, size_t n_tensors, F launch) {
     Table t;
     t.n = 0;
-    unsigned blocks = 0;
+    t.first[0] = 0;
     for (size_t i = 0; i < n_tensors; ++i) {
         if (counts[i]) {
-            t.ptr[t.n] = ptrs[i];
-            t.count[t.n] = counts[i];
-            t.type[t.n] = (unsigned char)types[i];
-            t.first[t.n++] = blocks;
-            blocks += (unsigned)((counts[i] + kChunk - 1) / kChunk);
+            t.ptr[t.n] = static_cast<char*>(ptrs[i]);
+            t.count[t.n] = (unsigned long long)counts[i] | (unsigned long long)types[i] << kTypeShift;
+            t.first[t.n + 1] = t.first[t.n] + (unsigned)chunks_of(ptrs[i], counts[i], types[i]);
+            ++t.n;
         }
         if (t.n && (t.n == kTable || i + 1 == n_tensors)) {
-            launch(t, blocks);
+            launch(t, std::min(t.first[t.n], kGroups));
             if (hipError_t e = hipGetLastError()) return e;
             t.n = 0;
-            blocks = 0;
         }
     }
     return hipSuccess;
@@ -119,26 +207,24 @@ hipError_t tables(void* const* ptrs, const size_t* counts, const int* types, siz
 
 }  // namespace
 
-size_t grad_norm_workspace(const size_t* counts, size_t n_tensors) {
-    size_t parts = 0;
-    for (size_t i = 0; i < n_tensors; ++i) parts += (counts[i] + kChunk - 1) / kChunk;
-    return 16 + parts * sizeof(double);
-}
+size_t grad_norm_workspace(size_t n_tensors) { return std::max<size_t>((n_tensors + kTable - 1) / kTable, 1) * kGroups * sizeof(double); }
 
 hipError_t launch_grad_norm(void* const* ptrs, const size_t* counts, const int* types, size_t n_tensors, bool clip, float limit,
                             float* d_norm, void* workspace, hipStream_t s) {
-    float* scale = static_cast<float*>(workspace);
-    double* part = reinterpret_cast<double*>(static_cast<char*>(workspace) + 16);
-    size_t parts = 0;
-    hipError_t e = tables(ptrs, counts, types, n_tensors, [&](const Table& t, unsigned blocks) {
-        hipLaunchKernelGGL(k_squares, dim3(blocks), dim3(kThreads), 0, s, t, part + parts);
-        parts += blocks;
+    double* part = static_cast<double*>(workspace);
+    unsigned parts = 0;
+    hipError_t e = tables(ptrs, counts, types, n_tensors, [&](const Table& t, unsigned groups) {
+        hipLaunchKernelGGL(k_squares, dim3(groups), dim3(kThreads), 0, s, t, part + parts);
+        parts += groups;
     });
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_norm, dim3(1), dim3(kThreads), 0, s, part, parts, limit, d_norm, scale);
-    if ((e = hipGetLastError()) != hipSuccess || !clip) return e;
-    return tables(ptrs, counts, types, n_tensors, [&](const Table& t, unsigned blocks) {
-        hipLaunchKernelGGL(k_scale, dim3(blocks), dim3(kThreads), 0, s, t, scale);
+    if (!clip || !parts) {
+        hipLaunchKernelGGL(k_norm, dim3(1), dim3(kThreads), 0, s, part, parts, d_norm);
+        return hipGetLastError();
+    }
+    return tables(ptrs, counts, types, n_tensors, [&](const Table& t, unsigned groups) {
+        hipLaunchKernelGGL(k_scale, dim3(groups), dim3(kThreads), 0, s, t, part, parts, limit, d_norm);
+        d_norm = nullptr;    // the first launch writes it
     });
 }
 

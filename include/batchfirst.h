@@ -334,8 +334,8 @@ int bf_policy_move_loss_grad(bf_ctx* ctx, const void* d_features, int type, size
 /* *d_norm = sqrt of the sum of squares over n_tensors tensors: h_tensors holds their device pointers, h_counts their
  * element counts (0 is allowed, its pointer is then not read), h_types their BF_TYPE_*; host arrays, read before the
  * call returns.  Each tensor is one contiguous range, aligned to its element.  Squares are summed in float64.
- * d_workspace: bf_grad_norm_workspace(h_counts, n_tensors) bytes. */
-size_t bf_grad_norm_workspace(const size_t* h_counts, size_t n_tensors);
+ * d_workspace: bf_grad_norm_workspace(n_tensors) bytes. */
+size_t bf_grad_norm_workspace(size_t n_tensors);
 int bf_global_norm(bf_ctx* ctx, const void* const* h_tensors, const size_t* h_counts, const int* h_types, size_t n_tensors,
                    float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream);
 

@@ -35,10 +35,10 @@ def check_against(norm, tensors, before, limit):
 def test_refusals_of_the_c_entry_points():
     lib = _lib.load()
     ctx = ctypes.cast(ctypes.create_string_buffer(1 << 16), ctypes.c_void_p)    # the checks look at nothing in it
-    buf = ctypes.create_string_buffer(1 << 16)
+    buf = ctypes.create_string_buffer(1 << 17)
     p = (ctypes.addressof(buf) + 255) & ~255
 
-    def clip(ctx=ctx, ptrs=(p, p + 4096), counts=(8, 8), types=(0, 1), limit=1.0, norm=p + 8192, ws=p + 16384, size=4096):
+    def clip(ctx=ctx, ptrs=(p, p + 4096), counts=(8, 8), types=(0, 1), limit=1.0, norm=p + 8192, ws=p + 16384, size=1 << 15):
         n = len(ptrs)
         return lib.bf_clip_grad_norm(ctx, (ctypes.c_void_p * n)(*ptrs), (ctypes.c_size_t * n)(*counts), (ctypes.c_int * n)(*types), n,
                                      limit, norm, ws, size, None)
@@ -55,7 +55,8 @@ def test_refusals_of_the_c_entry_points():
     refused(clip(ptrs=(p, None)), "tensor 1 is a null pointer")
     refused(clip(ptrs=(p + 2, p + 4096)), "tensor 0 is not aligned")
     refused(clip(ptrs=(p, p + 4097)), "tensor 1 is not aligned")
-    refused(clip(counts=(8, (1 << 40) + 1)), "2^40")
+    refused(clip(counts=(8, (1 << 37) + 1)), "2^37")
+    refused(lib.bf_global_norm(ctx, p, p, p, (1 << 20) + 1, p, p, 4096, None), "2^20")
     for limit in (-1.0, float("nan")):
         refused(clip(limit=limit), "max_norm")
     refused(clip(ptrs=(p, p)), "overlap")
@@ -111,7 +112,7 @@ def test_one_tensor(ctx, n, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("count", [2, 27, 95, 96, 97, 193, 1000])
+@pytest.mark.parametrize("count", [2, 27, 159, 160, 161, 321, 1000])
 def test_many_tensors_of_mixed_types_and_sizes(ctx, count):
     rng = np.random.default_rng(count)
     tensors = [randn(int(k), TYPES[i % 3], i, 0.1) for i, k in enumerate(np.exp(rng.uniform(0, 10, count)).astype(int))]
@@ -212,6 +213,15 @@ def test_refusals(ctx):
         o.clip_grad_norm_(ctx.handle, [x.double()], 1.0)
     with pytest.raises(ValueError, match="device tensor"):
         o.global_norm(ctx.handle, [x, torch.ones(3)])
+    with pytest.raises(ValueError, match="device tensor"):
+        o.clip_grad_norm_(ctx.handle, [torch.ones(3)], 1.0)
+    with pytest.raises(ValueError, match="require grad"):
+        o.clip_grad_norm_(ctx.handle, [x, torch.ones(3, device="cuda", requires_grad=True)], 1.0)
+    version = x._version
+    o.global_norm(ctx.handle, [x])
+    assert x._version == version
+    o.clip_grad_norm_(ctx.handle, [x], 100.0)
+    assert x._version == version + 1
     assert torch.equal(x, torch.ones(64, device="cuda"))
     assert float(o.global_norm(ctx.handle, [x, x])) == pytest.approx(128 ** 0.5)    # reading twice is fine
 
