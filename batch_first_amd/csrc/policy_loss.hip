@@ -31,8 +31,9 @@ constexpr int kC = 32, kS = 64, kF = 73, kVocab = kF * kS, kXW = kC * kF;
 //            4 n + j, so that a lane's features are four neighbours in memory.
 //   dX       rows channel, columns square, k filter.  k is numbered so that a lane's eight are the filters whose logits
 //            it holds already: the probabilities become an operand where they are.
-//   dW       rows channel, columns filter, k square: the probabilities cross the lanes through LDS, 32 filters at a time;
-//            the sums stay in registers over all the wave's boards.
+//   dW       rows channel, columns filter, k square: features and probabilities are written to LDS a square's channels
+//            or filters at a time, as they lie in the lanes, and read transposed (32 filters at a time); the sums stay
+//            in registers over all the wave's boards.
 //
 // float32 operands travel as two float16 terms (22 bits), scaled by a power of two, the kernel's by its largest element
 // and the features' by the board's, so that the larger term stays normal down to 2^-29 of the largest; of the four products of terms the
@@ -46,13 +47,14 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short short4v __attribute__((__vector_size__(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T>
 struct Arith {                                   // float32 and float16 features: float16 terms
     static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
-    static constexpr bool kScaled = true;
+    static constexpr bool kScaled = true;         // the gradients' terms need scaling
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
     }
@@ -75,6 +77,17 @@ struct Arith<__bf16> {
         lo = __builtin_bit_cast(unsigned, bf2{(__bf16)(a - __uint_as_float(hi << 16)), (__bf16)(b - __uint_as_float(hi & 0xffff0000u))});
     }
 };
+
+template <typename T>
+struct Raw;                                      // four neighbours as they lie
+template <> struct Raw<float> { typedef f32x4 type; };
+template <> struct Raw<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
+template <> struct Raw<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
+
+__device__ __forceinline__ void lds_fence() {    // orders a wave's own LDS accesses for the compiler; the hardware keeps order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
 // The larger, or NaN if either is: one instruction of three operands, without the quieting that fmaxf's takes each.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -101,10 +114,10 @@ __device__ __forceinline__ void scale_of(float largest, int least, float& scale,
 }
 
 constexpr int kTiles = 5;                        // of filters
-constexpr int kRow = 72;                         // 16-bit elements a row of the crossing: 16 rows start in 16 different bank groups
-constexpr int kCross = 2 * 32 * kRow * 2;        // bytes: two terms of 32 filters
-constexpr int kWaveLds = 64 * 40 * 4;            // bytes a wave: the crossing, at the end its kernel gradient
-static_assert(kCross <= kWaveLds, "the crossing fits");
+constexpr int kRow = 40;                         // 16-bit elements a square of the crossing: 32, and 16 rows in 16 different bank groups
+constexpr int kTerm = kS * kRow;                 // elements a term
+constexpr int kWaveLds = 2 * kTerm * 2;          // bytes a wave
+static_assert(kWaveLds >= 64 * 40 * 4, "at the end it takes the wave's kernel gradient");
 
 template <typename T>
 struct HeadLds {                                 // the kernel as operands, 16 bytes a lane
@@ -172,78 +185,129 @@ __device__ __forceinline__ float load_head(const T* __restrict__ w, HeadLds<T>& 
     return back;
 }
 
-// A product of operands of one or two terms each, the least of four left out.
-template <typename T, int TA, int TB>
-__device__ __forceinline__ f32x4 products(const u32x4 (&a)[TA], const u32x4 (&b)[TB], f32x4 c) {
-    if constexpr (TB == 2) c = Arith<T>::mfma(a[0], b[1], c);
-    if constexpr (TA == 2) c = Arith<T>::mfma(a[1], b[0], c);
-    return Arith<T>::mfma(a[0], b[0], c);
+// c[i] += a(i) b(i) for products of operands of one or two terms each, the least of four left out.  An MFMA that waits for
+// the one before it takes twice as long, so the N sums take turns; the barriers keep the compiler from undoing that.
+template <typename T, int TA, int TB, int N, typename A, typename B>
+__device__ __forceinline__ void products(f32x4 (&c)[N], A&& a, B&& b) {
+#pragma unroll
+    for (int k = (TA - 1) + (TB - 1); k >= 0; --k) {
+        const int ka = k == 2 ? 1 : TB == 1 ? k : 0, kb = k == 2 ? 0 : TB == 1 ? 0 : k;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = Arith<T>::mfma(a(i, ka), b(i, kb), c[i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
-template <typename T, bool GRAD>
+// What a call asks for beside the loss.
+enum { kFeaturesGrad = 1, kKernelGrad = 2 };
+
+template <typename T, int WANT>
 __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
                                                      const int64_t* __restrict__ targets, const float* __restrict__ weights,
                                                      unsigned weight_step, float* __restrict__ loss, T* __restrict__ dx,
                                                      float* __restrict__ dw_part, int* __restrict__ err) {
     constexpr int NT = Arith<T>::kTerms;
+    typedef typename Raw<T>::type raw_t;
     extern __shared__ __align__(16) unsigned char smem[];
     HeadLds<T>& lds = *reinterpret_cast<HeadLds<T>*>(smem);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int col = lane & 15, q = lane >> 4;
-    unsigned char* mine = smem + sizeof(HeadLds<T>) + wave * kWaveLds;   // gradient calls only
-    const float w_back = load_head<T, GRAD>(w, lds);
+    // Crossing: square 4 col + j is row 16 j + col.  A lane of a transposed read names four elements of one row and gets
+    // one column's element of four rows; two make an operand's eight k.
+    typedef __attribute__((address_space(3))) short4v* lds_short4;
+    short* mine = reinterpret_cast<short*>(smem + sizeof(HeadLds<T>) + wave * kWaveLds);   // kernel gradients only
+    short* write_at = mine + col * kRow + 8 * q;
+    short* read_at = mine + (8 * q + (col >> 2)) * kRow + 4 * (col & 3);
+    auto transposed = [&](int term, int h, int tile) {   // columns 16 tile ..., rows 32 h + 8 q ...
+        short* p = read_at + term * kTerm + 32 * h * kRow + 16 * tile;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)p));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(p + 4 * kRow)));
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+
+    const size_t step = (size_t)gridDim.x * waves;
+    size_t base = (size_t)blockIdx.x * waves + wave;     // lane i looks after board base + i step
+    const float w_back = load_head<T, (WANT & kFeaturesGrad) != 0>(w, lds);
+    raw_t raw[8];                                // channels 8 q ... 8 q + 7, squares 4 col ... 4 col + 3
+    auto load = [&](size_t board) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const raw_t*>(x + board * (kC * kS) + (8 * q + i) * kS + 4 * col);
+    };
 
     f32x4 dw[2][kTiles];
-    if (GRAD)
+    if (WANT & kKernelGrad)
 #pragma unroll
         for (int i = 0; i < 2 * kTiles; ++i) dw[i / kTiles][i % kTiles] = f32x4{0, 0, 0, 0};
 
-    for (size_t b = (size_t)blockIdx.x * waves + wave; b < n; b += (size_t)gridDim.x * waves) {
-        const T* xb = x + b * (kC * kS);
-        const int64_t t64 = targets[b];
-        const int target = __builtin_amdgcn_readfirstlane(t64 >= 0 && t64 < kVocab ? (int)t64 : -1);
-        if (target < 0) {                        // no part in anything, whatever the features hold
-            if (lane == 0) {
-                if (t64 != -1) atomicOr(err, 8);
-                if (loss) loss[b] = 0.0f;
-            }
-            if (GRAD && dx) {
-                u32x4* out = reinterpret_cast<u32x4*>(dx + b * (kC * kS));
+    for (; base < n; base += 64 * step) {
+        const bool in = base + lane * step < n;
+        const int64_t t64 = in ? targets[base + lane * step] : 0;
+        const bool valid = in && t64 >= 0 && t64 < kVocab;
+        const float my_weight = WANT && valid ? weights[(base + lane * step) * weight_step] : 0.0f;
+        const int my_target = (int)t64;
+        if (in && !valid) {                      // no part in anything, whatever the features hold
+            if (t64 != -1) atomicOr(err, 8);
+            if (loss) loss[base + lane * step] = 0.0f;
+        }
+        if (WANT & kFeaturesGrad)
+            for (uint64_t left = __ballot(in && !valid); left; left &= left - 1) {
+                u32x4* out = reinterpret_cast<u32x4*>(dx + (base + __builtin_ctzll(left) * step) * (kC * kS));
 #pragma unroll
                 for (int i = 0; i < (int)(kC * kS * sizeof(T) / 1024); ++i) out[i * 64 + lane] = u32x4{0, 0, 0, 0};
             }
-            continue;
-        }
+        uint64_t left = __ballot(valid);
+        if (left) load(base + __builtin_ctzll(left) * step);
+      while (left) {
+        const int who = __builtin_ctzll(left);
+        const size_t b = base + who * step;
+        left &= left - 1;
+        const size_t next = base + (left ? __builtin_ctzll(left) : 0) * step;   // read ahead; after the last, in vain
+        const int target = __builtin_amdgcn_readlane(my_target, who);
 
-        // features as columns: square 4 col + j, channels 8 q ... 8 q + 7
-        u32x4 xc[4][NT];
+        // features in their terms, pairs of squares packed
+        u32x2 rows[NT][8];
         float x_scale = 1.0f, x_back = 1.0f;
         if constexpr (sizeof(T) == 4) {
-            f32x4 raw[8];
             float largest = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const f32x4*>(xb + (8 * q + i) * kS + 4 * col);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) largest = larger(largest, fabsf(raw[i][j]));
             scale_of(lanes_reduce<true>(largest), -100, x_scale, x_back);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float v[8];
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = raw[i][j];
-                operand<T>(v, x_scale, xc[j]);
-            }
+                for (int j = 0; j < 2; ++j) {
+                    unsigned hi, lo;
+                    Arith<T>::split(raw[i][2 * j] * x_scale, raw[i][2 * j + 1] * x_scale, hi, lo);
+                    rows[0][i][j] = hi;
+                    rows[1][i][j] = lo;
+                }
         } else {
-            u32x2 raw[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const u32x2*>(xb + (8 * q + i) * kS + 4 * col);
+            for (int i = 0; i < 8; ++i) rows[0][i] = __builtin_bit_cast(u32x2, raw[i]);
+        }
+        if (WANT == 0) load(next);
+
+        // as columns (square 4 col + j, channels 8 q ... 8 q + 7)
+        u32x4 xc[4][NT];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    xc[j][0][i] = __builtin_amdgcn_perm(raw[2 * i + 1][j >> 1], raw[2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+                    xc[j][k][i] = __builtin_amdgcn_perm(rows[k][2 * i + 1][j >> 1], rows[k][2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+
+        // and as rows (channel, squares by row of the crossing) for dW
+        u32x4 xr[2][2][NT];
+        if (WANT & kKernelGrad) {
+#pragma unroll
+            for (int i = 0; i < 4 * NT; ++i) *reinterpret_cast<u32x4*>(write_at + (i % NT) * kTerm + 16 * (i / NT) * kRow) = xc[i / NT][i % NT];
+            lds_fence();
+#pragma unroll
+            for (int i = 0; i < 4 * NT; ++i) xr[i / NT >> 1][i / NT & 1][i % NT] = transposed(i % NT, i / NT & 1, i / NT >> 1);
+            lds_fence();
         }
 
         // logits, in units of 2^-(scales)
@@ -253,12 +317,10 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
             u32x4 a[NT];
 #pragma unroll
             for (int k = 0; k < NT; ++k) a[k] = lds.logit[t][k][lane];
+            f32x4 l[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+            products<T, NT, NT>(l, [&](int, int k) { return a[k]; }, [&](int j, int k) { return xc[j][k]; });
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 l = products<T>(a, xc[j], f32x4{0, 0, 0, 0});
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[t][4 * j + r] = l[r];
-            }
+            for (int k = 0; k < 16; ++k) v[t][k] = l[k >> 2][k & 3];
         }
         // the padding's filters 73 ... 79
 #pragma unroll
@@ -302,38 +364,26 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
             }
         const float z = lanes_reduce<false>((z4[0] + z4[1]) + (z4[2] + z4[3]));
         if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
-        if (!GRAD) continue;
+        if (!WANT) continue;
 
-        // the logits' gradients: probabilities, less one at the target.  The target's is the largest but for rounding:
-        // z's own, up to 90 * 2^-24, can make the target's smaller than another by as much, which the least scale covers.
+        // the logits' gradients times z: exponentials, less z at the target.  The target's is the largest but for
+        // rounding: z's own, up to 90 * 2^-24, can make the target's smaller than another by as much, which the least
+        // scale covers.
         const float rz = __builtin_amdgcn_rcpf(z);
         const float d_target = at_target([&](float e) { return e - (lane == t_lane ? z : 0.0f); }) * rz;
-        float d_scale = 1.0f, d_back = 1.0f;
-        if constexpr (Arith<T>::kScaled) scale_of(fabsf(d_target), -17, d_scale, d_back);
-        const float inv = d_scale * rz;
-        const float wb = weights[b * weight_step] * d_back;
-
-        // features as rows: channel col of each half, squares 8 q ... 8 q + 7 of each half
-        u32x4 xr[2][2][NT];
-        if (dw_part) {
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const T* p = xb + (16 * a + col) * kS + 32 * h + 8 * q;
-                    if constexpr (sizeof(T) == 4) {
-                        const f32x4 lo = reinterpret_cast<const f32x4*>(p)[0], hi = reinterpret_cast<const f32x4*>(p)[1];
-                        const float e[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                        operand<T>(e, x_scale, xr[a][h]);
-                    } else {
-                        xr[a][h][0] = *reinterpret_cast<const u32x4*>(p);
-                    }
-                }
+        float inv = 1.0f, wb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
+        if constexpr (Arith<T>::kScaled) {
+            float d_scale, d_back;
+            scale_of(fabsf(d_target), -17, d_scale, d_back);
+            inv = d_scale * rz;
+            wb *= d_back;
+        } else {
+            wb *= rz;
         }
 
-        f32x4 g[2][4];
+        f32x4 g[8];                              // [4 * half of channels + square of four]
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i >> 2][i & 3] = f32x4{0, 0, 0, 0};
+        for (int i = 0; i < 8; ++i) g[i] = f32x4{0, 0, 0, 0};
         const float w_scale = wb * x_back;
 #pragma unroll
         for (int u = 0; u < 3; ++u) {
@@ -347,80 +397,78 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
                     if (i < 2 * tiles) {
                         const f32x16& p = v[2 * u + (i >> 1)];
                         const int k = 4 * j + 2 * (i & 1);
-                        Arith<T>::split(p[k] * inv, p[k + 1] * inv, hi, lo);
+                        if constexpr (Arith<T>::kScaled) Arith<T>::split(p[k] * inv, p[k + 1] * inv, hi, lo);
+                        else Arith<T>::split(p[k], p[k + 1], hi, lo);
                     }
                     d[j][0][i] = hi;
                     d[j][1][i] = lo;
                 }
-            if (dw_part) {
-                // across the lanes: row filter, four squares at a time
+            if (u == 0) load(next);              // the first two tiles' registers are free
+            if (WANT & kKernelGrad) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int i = 0; i < 8; ++i) {
+                    short* p = write_at + (i & 1) * kTerm + 16 * (i >> 1) * kRow;
+                    if (tiles == 2) *reinterpret_cast<u32x4*>(p) = d[i >> 1][i & 1];
+                    else *reinterpret_cast<u32x2*>(p - 4 * q) = u32x2{d[i >> 1][i & 1][0], d[i >> 1][i & 1][1]};
+                }
+                lds_fence();
+            }
+            if (WANT & kFeaturesGrad) {
+                u32x4 wk[2][NT];
+#pragma unroll
+                for (int i = 0; i < 2 * NT; ++i) wk[i / NT][i % NT] = lds.back[u][i / NT][i % NT][lane];
+                products<T, NT, 2>(g, [&](int i, int k) { return wk[i >> 2][k]; }, [&](int i, int k) { return d[i & 3][k]; });
+            }
+            if (WANT & kKernelGrad) {
+                auto sums = [&](auto& s) {       // [2 * tile + half of channels]
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        u32x4 dk[2][2];
+#pragma unroll
+                        for (int i = 0; i < 2 * tiles; ++i)
+                            dk[i >> 1][i & 1] = transposed(i & 1, h, i >> 1);
+                        products<T, NT, 2>(s, [&](int i, int k) { return xr[i & 1][h][k]; }, [&](int i, int k) { return dk[i >> 1][k]; });
+                    }
 #pragma unroll
                     for (int i = 0; i < 2 * tiles; ++i)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const unsigned pick = h ? 0x07060302u : 0x05040100u;
-                            const u32x2 four = {__builtin_amdgcn_perm(d[1][k][i], d[0][k][i], pick), __builtin_amdgcn_perm(d[3][k][i], d[2][k][i], pick)};
-                            const int row = 16 * (i >> 1) + 4 * q + 2 * (i & 1) + h;
-                            *reinterpret_cast<u32x2*>(mine + ((k * 32 + row) * kRow + 4 * col) * 2) = four;
-                        }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-            }
-            if (dx) {
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    u32x4 wk[NT];
-#pragma unroll
-                    for (int k = 0; k < NT; ++k) wk[k] = lds.back[u][a][k][lane];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) g[a][j] = products<T>(wk, d[j], g[a][j]);
-                }
-            }
-            if (dw_part) {
-#pragma unroll
-                for (int t = 0; t < tiles; ++t) {
+                        for (int r = 0; r < 4; ++r) dw[i & 1][2 * u + (i >> 1)][r] = fmaf(s[i][r], w_scale, dw[i & 1][2 * u + (i >> 1)][r]);
+                };
+                if (tiles == 2) {
+                    f32x4 s[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+                    sums(s);
+                } else {
                     f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        u32x4 dk[2];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            dk[k] = *reinterpret_cast<const u32x4*>(mine + ((k * 32 + 16 * t + col) * kRow + 32 * h + 8 * q) * 2);
-#pragma unroll
-                        for (int a = 0; a < 2; ++a) s[a] = products<T>(xr[a][h], dk, s[a]);
-                    }
-#pragma unroll
-                    for (int a = 0; a < 2; ++a)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) dw[a][2 * u + t][r] = fmaf(s[a][r], w_scale, dw[a][2 * u + t][r]);
+                    sums(s);
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+                lds_fence();
             }
         }
-        if (dx) {
+        if (WANT & kFeaturesGrad) {
             const float back = wb * w_back;
 #pragma unroll
             for (int a = 0; a < 2; ++a)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    typedef T four_t __attribute__((ext_vector_type(4)));
-                    const four_t out = {(T)(g[a][0][r] * back), (T)(g[a][1][r] * back), (T)(g[a][2][r] * back), (T)(g[a][3][r] * back)};
-                    *reinterpret_cast<four_t*>(dx + b * (kC * kS) + (16 * a + 4 * q + r) * kS + 4 * col) = out;
+                    const raw_t out = {(T)(g[4 * a][r] * back), (T)(g[4 * a + 1][r] * back), (T)(g[4 * a + 2][r] * back), (T)(g[4 * a + 3][r] * back)};
+                    *reinterpret_cast<raw_t*>(dx + b * (kC * kS) + (16 * a + 4 * q + r) * kS + 4 * col) = out;
                 }
         }
+      }
     }
 
-    if (GRAD && dw_part) {
+    if (WANT & kKernelGrad) {
         float* part = reinterpret_cast<float*>(mine);
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) part[((16 * a + 4 * q + r) * kTiles + t) * 16 + col] = dw[a][t][r];
+                for (int r = 0; r < 4; ++r) {
+                    // column c of a pair of tiles is filter 16 (c >> 2 & 1) + 4 (c >> 3) + (c & 3) of the pair's 32
+                    const int c = 16 * (t & 1) + col, f = t == 4 ? 64 + col : 32 * (t >> 1) + 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
+                    part[(16 * a + 4 * q + r) * (16 * kTiles) + f] = dw[a][t][r];
+                }
         __syncthreads();
         const float* all = reinterpret_cast<const float*>(smem + sizeof(HeadLds<T>));
         for (int i = threadIdx.x; i < kXW; i += blockDim.x) {
@@ -455,23 +503,12 @@ static_assert(kS * kGRow <= kC * kXRow, "the gradient takes the features' place"
 
 struct __attribute__((packed)) Bytes16 { unsigned v[4]; };
 
-template <typename T>
-struct Raw;                                      // four neighbours as they lie
-template <> struct Raw<float> { typedef f32x4 type; };
-template <> struct Raw<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
-template <> struct Raw<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
-
 __device__ __forceinline__ unsigned lanes_add(unsigned v) {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
-__device__ __forceinline__ void lds_fence() {    // orders a wave's own LDS accesses for the compiler; the hardware keeps order
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-template <typename T, bool GRAD>
+template <typename T, int WANT>
 __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
                                                           const uint8_t* __restrict__ from, const uint8_t* __restrict__ filter,
                                                           const uint8_t* __restrict__ per, size_t n_moves,
@@ -482,9 +519,9 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
     extern __shared__ __align__(16) unsigned char smem[];
     float* head = reinterpret_cast<float*>(smem);
     uint64_t* red = reinterpret_cast<uint64_t*>(smem + kF * kHeadRow * 4);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
     const int col = lane & 15, q = lane >> 4, chan = lane & 31, half = lane >> 5;
-    unsigned char* mine = smem + kMoveHeadBytes + wave * (GRAD ? kMoveGradBytes : kMoveWaveBytes);
+    unsigned char* mine = smem + kMoveHeadBytes + wave * (WANT & kKernelGrad ? kMoveGradBytes : kMoveWaveBytes);
     float* xs = reinterpret_cast<float*>(mine);                                  // [32][68]
     u32x2* entry = reinterpret_cast<u32x2*>(mine + kC * kXRow * 4);              // [64] (square | filter << 8, gradient)
     float* dws = reinterpret_cast<float*>(mine + kMoveWaveBytes);                // [73][32], gradient calls only
@@ -493,7 +530,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
     const size_t lo = n * me / all, hi = n * (me + 1) / all, group_lo = n * (me - wave) / all;
 
     for (int i = tid; i < kXW; i += blockDim.x) head[(i % kF) * kHeadRow + i / kF] = (float)w[i];
-    if (GRAD)
+    if (WANT & kKernelGrad)
         for (int i = lane; i < kF * kC; i += 64) dws[i] = 0.0f;
     unsigned before = 0;
     for (size_t i = (size_t)tid * 16; i < group_lo; i += (size_t)blockDim.x * 16) {
@@ -566,7 +603,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                 if (t64 != -1) atomicOr(err, 8);
                 if (loss) loss[b] = 0.0f;
             }
-            if (GRAD && dx) {
+            if (WANT & kFeaturesGrad) {
                 u32x4* out = reinterpret_cast<u32x4*>(dx + b * (kC * kS));
 #pragma unroll
                 for (int i = 0; i < (int)(kC * kS * sizeof(T) / 1024); ++i) out[i * 64 + lane] = u32x4{0, 0, 0, 0};
@@ -584,7 +621,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
         }
         z = lanes_reduce<false>(z);
         if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, top - l_target);
-        if (!GRAD) {
+        if (!WANT) {
             lds_fence();
             continue;
         }
@@ -617,13 +654,13 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                 v = next;
             }
         };
-        if (dw_part)
+        if (WANT & kKernelGrad)
 #pragma unroll
             for (int p = 0; p < 4; ++p)
                 if (64 * p < cnt)
                     add_up(p, [&](unsigned m) { return dws + (m >> 8) * kC + chan; }, [&](unsigned m) { return xs[chan * kXRow + (m & 0xff)]; },
                            [](unsigned a, unsigned b) { return a >> 8 == b >> 8; });
-        if (dx) {
+        if (WANT & kFeaturesGrad) {
             lds_fence();
             float* g = xs;                       // [64][33]
             for (int i = lane; i < kS * kGRow; i += 64) g[i] = 0.0f;
@@ -645,7 +682,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
     }
     if (lo < hi && hi == n && lane == 0 && start != n_moves) atomicOr(err, 8);
 
-    if (GRAD && dw_part) {
+    if (WANT & kKernelGrad) {
         __syncthreads();
         for (int i = tid; i < kXW; i += blockDim.x) {
             const int c = i / kF, f = i % kF;
@@ -683,28 +720,30 @@ unsigned waves_for(size_t n, unsigned most) {
     return waves;
 }
 
-template <typename T, bool GRAD>
+template <typename T, int WANT>
 hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
     const T *x = static_cast<const T*>(a.features), *w = static_cast<const T*>(a.kernel);
     T* dx = static_cast<T*>(a.d_features);
-    float* part = a.d_kernel ? static_cast<float*>(a.workspace) : nullptr;
-    const unsigned waves = waves_for(a.n, GRAD ? 8 : 4), step = a.n_weights > 1 ? 1u : 0u;
-    const unsigned grid = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, GRAD ? kGroups : 4 * kGroups);
+    float* part = static_cast<float*>(a.workspace);
+    const unsigned waves = waves_for(a.n, WANT ? 8 : 4), step = a.n_weights > 1 ? 1u : 0u;
+    const unsigned grid = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, WANT ? kGroups : 4 * kGroups);
     if (grid && a.per_board)
-        hipLaunchKernelGGL((k_policy_move_loss<T, GRAD>), dim3(grid), dim3(waves * 64),
-                           kMoveHeadBytes + waves * (GRAD ? kMoveGradBytes : kMoveWaveBytes), s, x, w, a.n, a.from, a.filter, a.per_board,
-                           a.n_moves, a.targets, a.weights, step, a.loss, dx, part, a.err);
+        hipLaunchKernelGGL((k_policy_move_loss<T, WANT>), dim3(grid), dim3(waves * 64),
+                           kMoveHeadBytes + waves * (WANT & kKernelGrad ? kMoveGradBytes : kMoveWaveBytes), s, x, w, a.n, a.from,
+                           a.filter, a.per_board, a.n_moves, a.targets, a.weights, step, a.loss, dx, part, a.err);
     else if (grid)
-        hipLaunchKernelGGL((k_policy_loss<T, GRAD>), dim3(grid), dim3(waves * 64), sizeof(HeadLds<T>) + (GRAD ? waves * kWaveLds : 0), s,
-                           x, w, a.n, a.targets, a.weights, step, a.loss, dx, part, a.err);
+        hipLaunchKernelGGL((k_policy_loss<T, WANT>), dim3(grid), dim3(waves * 64),
+                           sizeof(HeadLds<T>) + (WANT & kKernelGrad ? waves * kWaveLds : 0), s, x, w, a.n, a.targets, a.weights, step,
+                           a.loss, dx, part, a.err);
     if (hipError_t e = hipGetLastError()) return e;
-    if (a.d_kernel) hipLaunchKernelGGL(k_sum_parts<T>, dim3(kXW / 32), dim3(256), 0, s, part, grid, static_cast<T*>(a.d_kernel));
+    if (WANT & kKernelGrad) hipLaunchKernelGGL(k_sum_parts<T>, dim3(kXW / 32), dim3(256), 0, s, part, grid, static_cast<T*>(a.d_kernel));
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
-    return a.d_features || a.d_kernel ? launch<T, true>(a, s) : launch<T, false>(a, s);
+    if (a.d_features) return a.d_kernel ? launch<T, kFeaturesGrad | kKernelGrad>(a, s) : launch<T, kFeaturesGrad>(a, s);
+    return a.d_kernel ? launch<T, kKernelGrad>(a, s) : launch<T, 0>(a, s);
 }
 
 }  // namespace
