@@ -112,21 +112,150 @@ __device__ __forceinline__ void scale_of(float largest, int least, float& scale,
     scale = __uint_as_float((unsigned)(127 + 13 - e) << 23);
     back = __uint_as_float((unsigned)(127 - 13 + e) << 23);
 }
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
-constexpr int kTiles = 5;                        // of filters
-constexpr int kRow = 40;                         // 16-bit elements a square of the crossing: 32, and 16 rows in 16 different bank groups
-constexpr int kTerm = kS * kRow;                 // elements a term
-constexpr int kWaveLds = 2 * kTerm * 2;          // bytes a wave
-static_assert(kWaveLds >= 64 * 40 * 4, "at the end it takes the wave's kernel gradient");
+constexpr int kTiles = 5;                        // of 16 filters
+constexpr int kRow = 40;                         // 16-bit elements of a row of 32 in LDS: 16 rows start in 16 different bank groups
+constexpr int kTerm = kS * kRow;                 // elements of 64 rows
+constexpr int kPartBytes = 64 * 40 * 4;          // a wave's kernel gradient in LDS, when its boards are done
+constexpr int kStageBytes = kXW * 4;             // the kernel on its way to its operands
 
+// A board's features: a lane holds channels 8 q ... 8 q + 7 of squares 4 col ... 4 col + 3 and turns them into operands
+// of columns square (4 col + j), k channel.  The scale goes by the largest finite one, so that squares that a list of
+// moves leaves out may hold anything.
 template <typename T>
-struct HeadLds {                                 // the kernel as operands, 16 bytes a lane
-    u32x4 logit[kTiles][Arith<T>::kTerms][64];   // rows filter, k channel
-    u32x4 back[3][2][Arith<T>::kTerms][64];      // rows channel, k filter as the logits' results hold them
-    float red[8];
+struct Features {
+    static constexpr int kTerms = Arith<T>::kTerms;
+    typename Raw<T>::type raw[8];
+    u32x4 column[4][kTerms];
+    float scale, back;
+
+    __device__ __forceinline__ void load(const T* board, int col, int q) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const typename Raw<T>::type*>(board + (8 * q + i) * kS + 4 * col);
+    }
+    __device__ __forceinline__ void convert() {
+        u32x2 rows[kTerms][8];                   // pairs of squares
+        scale = back = 1.0f;
+        if constexpr (kTerms == 2) {
+            float largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) largest = larger(largest, fabsf(raw[i >> 2][i & 3]));
+            largest = lanes_reduce<true>(largest);
+            if (!finite(largest)) {
+                largest = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) largest = larger(largest, finite(raw[i >> 2][i & 3]) ? fabsf(raw[i >> 2][i & 3]) : 0.0f);
+                largest = lanes_reduce<true>(largest);
+            }
+            scale_of(largest, -100, scale, back);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                unsigned hi, lo;
+                Arith<T>::split(raw[i >> 1][2 * (i & 1)] * scale, raw[i >> 1][2 * (i & 1) + 1] * scale, hi, lo);
+                rows[0][i >> 1][i & 1] = hi;
+                rows[1][i >> 1][i & 1] = lo;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rows[0][i] = __builtin_bit_cast(u32x2, raw[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int k = 0; k < kTerms; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    column[j][k][i] = __builtin_amdgcn_perm(rows[k][2 * i + 1][j >> 1], rows[k][2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+    }
 };
 
-// Eight values as an operand of one or two terms.
+// Square 4 col + j is row 16 j + col of 64 rows of channels or filters in LDS.
+template <int TERMS>
+__device__ __forceinline__ void write_rows(short* rows, int col, int q, const u32x4 (&v)[4][TERMS]) {
+#pragma unroll
+    for (int i = 0; i < 4 * TERMS; ++i)
+        *reinterpret_cast<u32x4*>(rows + (i % TERMS) * kTerm + (16 * (i / TERMS) + col) * kRow + 8 * q) = v[i / TERMS][i % TERMS];
+}
+
+// A transposed read: a lane names four elements of one row (group of 16 lanes: four rows) and gets one column's element of
+// the four rows.  Two make the eight k of an operand of 16 rows or columns; lo and hi are the lane's row of the first and
+// of the second four.
+__device__ __forceinline__ u32x4 transposed(const short* lo, const short* hi) {
+    typedef __attribute__((address_space(3))) short4v* lds_short4;
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)lo));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)hi));
+    return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// Boards without a target: loss 0, gradient 0.
+template <typename T>
+__device__ __forceinline__ void zero_features_grad(T* board, int lane) {
+    u32x4* out = reinterpret_cast<u32x4*>(board);
+#pragma unroll
+    for (int i = 0; i < (int)(kC * kS * sizeof(T) / 1024); ++i) out[i * 64 + lane] = u32x4{0, 0, 0, 0};
+}
+
+// g[4 a + j]: rows channel 16 a + 4 q + r, columns square 4 col + j
+template <typename T>
+__device__ __forceinline__ void store_features_grad(T* board, int col, int q, const f32x4 (&g)[8], float back) {
+    typedef typename Raw<T>::type raw_t;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int a = i >> 2, r = i & 3;
+        *reinterpret_cast<raw_t*>(board + (16 * a + 4 * q + r) * kS + 4 * col) =
+            raw_t{(T)(g[4 * a][r] * back), (T)(g[4 * a + 1][r] * back), (T)(g[4 * a + 2][r] * back), (T)(g[4 * a + 3][r] * back)};
+    }
+}
+
+// The workgroup's part of the kernel's gradient: dw[a][t] of every wave, rows channel 16 a + 4 q + r, columns the filters
+// that filter_of(t, col) says; `mine` and `stride` bytes further on the other waves' LDS.
+template <typename F>
+__device__ __forceinline__ void store_part(const f32x4 (&dw)[2][kTiles], unsigned char* first, int stride, int wave, int waves, int col, int q,
+                                           float* __restrict__ part, F&& filter_of) {
+    float* mine = reinterpret_cast<float*>(first + wave * stride);
+#pragma unroll
+    for (int i = 0; i < 8 * kTiles; ++i) {
+        const int a = i / (4 * kTiles), t = i / 4 % kTiles, r = i & 3;
+        mine[(16 * a + 4 * q + r) * (16 * kTiles) + filter_of(t, col)] = dw[a][t][r];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kXW; i += blockDim.x) {
+        float a = 0.0f;
+        for (int k = 0; k < waves; ++k) a += reinterpret_cast<const float*>(first + k * stride)[i / kF * (16 * kTiles) + i % kF];
+        part[i] = a;
+    }
+}
+
+// The kernel as float32 in `stage`, and its scale, which is by the largest finite element.
+template <typename T>
+__device__ __forceinline__ void stage_head(const T* __restrict__ w, float* stage, float* red, float& scale, float& back) {
+    typedef T piece_t __attribute__((ext_vector_type(16 / sizeof(T))));
+    constexpr int kPer = 16 / sizeof(T);
+    static_assert(kXW % kPer == 0, "whole pieces");
+    float largest = 0.0f;
+#pragma unroll 3
+    for (int i = threadIdx.x; i < kXW / kPer; i += blockDim.x) {
+        const piece_t v = reinterpret_cast<const piece_t*>(w)[i];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            stage[i * kPer + k] = (float)v[k];
+            if (finite((float)v[k])) largest = fmaxf(largest, fabsf((float)v[k]));
+        }
+    }
+    scale = back = 1.0f;
+    if constexpr (Arith<T>::kTerms == 2) {
+        largest = lanes_reduce<true>(largest);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = largest;
+        __syncthreads();
+        for (int i = 0; i < (int)blockDim.x >> 6; ++i) largest = fmaxf(largest, red[i]);
+        scale_of(largest, -100, scale, back);
+    } else {
+        __syncthreads();
+    }
+}
+
+// Eight values as an operand.
 template <typename T>
 __device__ __forceinline__ void operand(const float (&v)[8], float scale, u32x4 (&out)[Arith<T>::kTerms]) {
 #pragma unroll
@@ -136,53 +265,11 @@ __device__ __forceinline__ void operand(const float (&v)[8], float scale, u32x4 
             Arith<T>::split(v[2 * i] * scale, v[2 * i + 1] * scale, hi, lo);
             out[0][i] = hi;
             out[1][i] = lo;
-        } else if constexpr (sizeof(T) == 2) {
+        } else {
             typedef T pair __attribute__((ext_vector_type(2)));
             out[0][i] = __builtin_bit_cast(unsigned, pair{(T)v[2 * i], (T)v[2 * i + 1]});
         }
     }
-}
-
-// Fills the kernel's operands; returns the factor that takes a product of scaled operands' kernel part back.
-template <typename T, bool GRAD>
-__device__ __forceinline__ float load_head(const T* __restrict__ w, HeadLds<T>& lds) {
-    float scale = 1.0f, back = 1.0f;
-    const int tid = threadIdx.x, waves = blockDim.x >> 6;
-    if constexpr (Arith<T>::kTerms == 2) {
-        float largest = 0.0f;
-        for (int i = tid; i < kXW; i += blockDim.x) largest = fmaxf(largest, fabsf((float)w[i]));
-        largest = lanes_reduce<true>(largest);
-        if ((tid & 63) == 0) lds.red[tid >> 6] = largest;
-        __syncthreads();
-        for (int i = 0; i < waves; ++i) largest = fmaxf(largest, lds.red[i]);
-        scale_of(largest, -100, scale, back);
-    }
-    for (int i = tid; i < kTiles * 64; i += blockDim.x) {
-        const int f = (i >> 6) * 16 + (i & 15), q = i >> 4 & 3;
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = f < kF ? (float)w[(8 * q + k) * kF + f] : 0.0f;
-        u32x4 out[Arith<T>::kTerms];
-        operand<T>(v, scale, out);
-#pragma unroll
-        for (int k = 0; k < Arith<T>::kTerms; ++k) lds.logit[i >> 6][k][i & 63] = out[k];
-    }
-    if (GRAD)
-        for (int i = tid; i < 6 * 64; i += blockDim.x) {
-            const int u = i >> 7, a = i >> 6 & 1, c = a * 16 + (i & 15), q = i >> 4 & 3;
-            float v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int f = 32 * u + 16 * (k >> 2) + 4 * q + (k & 3);
-                v[k] = f < kF ? (float)w[c * kF + f] : 0.0f;
-            }
-            u32x4 out[Arith<T>::kTerms];
-            operand<T>(v, scale, out);
-#pragma unroll
-            for (int k = 0; k < Arith<T>::kTerms; ++k) lds.back[u][a][k][i & 63] = out[k];
-        }
-    __syncthreads();
-    return back;
 }
 
 // c[i] += a(i) b(i) for products of operands of one or two terms each, the least of four left out.  An MFMA that waits for
@@ -201,45 +288,72 @@ __device__ __forceinline__ void products(f32x4 (&c)[N], A&& a, B&& b) {
 // What a call asks for beside the loss.
 enum { kFeaturesGrad = 1, kKernelGrad = 2 };
 
+template <typename T>
+struct HeadLds {                                 // the kernel as operands, 16 bytes a lane
+    u32x4 logit[kTiles][Arith<T>::kTerms][64];   // rows filter, k channel
+    u32x4 back[3][2][Arith<T>::kTerms][64];      // rows channel, k filter as the logits' results hold them
+    float red[8];
+};
+constexpr int kWaveLds = 2 * kTerm * 2;          // bytes a wave: the crossing
+static_assert(kWaveLds >= kPartBytes, "at the end it takes the wave's kernel gradient");
+
 template <typename T, int WANT>
 __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
                                                      const int64_t* __restrict__ targets, const float* __restrict__ weights,
                                                      unsigned weight_step, float* __restrict__ loss, T* __restrict__ dx,
                                                      float* __restrict__ dw_part, int* __restrict__ err) {
     constexpr int NT = Arith<T>::kTerms;
-    typedef typename Raw<T>::type raw_t;
     extern __shared__ __align__(16) unsigned char smem[];
     HeadLds<T>& lds = *reinterpret_cast<HeadLds<T>*>(smem);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int col = lane & 15, q = lane >> 4;
-    // Crossing: square 4 col + j is row 16 j + col.  A lane of a transposed read names four elements of one row and gets
-    // one column's element of four rows; two make an operand's eight k.
-    typedef __attribute__((address_space(3))) short4v* lds_short4;
     short* mine = reinterpret_cast<short*>(smem + sizeof(HeadLds<T>) + wave * kWaveLds);   // kernel gradients only
-    short* write_at = mine + col * kRow + 8 * q;
-    short* read_at = mine + (8 * q + (col >> 2)) * kRow + 4 * (col & 3);
-    auto transposed = [&](int term, int h, int tile) {   // columns 16 tile ..., rows 32 h + 8 q ...
-        short* p = read_at + term * kTerm + 32 * h * kRow + 16 * tile;
-        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)p));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(p + 4 * kRow)));
-        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    const short* read_at = mine + (8 * q + (col >> 2)) * kRow + 4 * (col & 3);
+    auto crossed = [&](int term, int h, int tile) {      // columns 16 tile ..., k the rows 32 h + 8 q ...
+        const short* p = read_at + term * kTerm + 32 * h * kRow + 16 * tile;
+        return transposed(p, p + 4 * kRow);
     };
 
-    const size_t step = (size_t)gridDim.x * waves;
-    size_t base = (size_t)blockIdx.x * waves + wave;     // lane i looks after board base + i step
-    const float w_back = load_head<T, (WANT & kFeaturesGrad) != 0>(w, lds);
-    raw_t raw[8];                                // channels 8 q ... 8 q + 7, squares 4 col ... 4 col + 3
-    auto load = [&](size_t board) {
+    float w_back;
+    {
+        float w_scale;
+        float* stage = reinterpret_cast<float*>(smem + sizeof(HeadLds<T>));
+        stage_head<T>(w, stage, lds.red, w_scale, w_back);
+        for (int i = threadIdx.x; i < kTiles * 64; i += blockDim.x) {
+            const int f = (i >> 6) * 16 + (i & 15);
+            float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const raw_t*>(x + board * (kC * kS) + (8 * q + i) * kS + 4 * col);
-    };
+            for (int k = 0; k < 8; ++k) v[k] = f < kF ? stage[(8 * (i >> 4 & 3) + k) * kF + f] : 0.0f;
+            u32x4 out[NT];
+            operand<T>(v, w_scale, out);
+#pragma unroll
+            for (int k = 0; k < NT; ++k) lds.logit[i >> 6][k][i & 63] = out[k];
+        }
+        if (WANT & kFeaturesGrad)
+            for (int i = threadIdx.x; i < 6 * 64; i += blockDim.x) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int f = 32 * (i >> 7) + 16 * (k >> 2) + 4 * (i >> 4 & 3) + (k & 3);
+                    v[k] = f < kF ? stage[(16 * (i >> 6 & 1) + (i & 15)) * kF + f] : 0.0f;
+                }
+                u32x4 out[NT];
+                operand<T>(v, w_scale, out);
+#pragma unroll
+                for (int k = 0; k < NT; ++k) lds.back[i >> 7][i >> 6 & 1][k][i & 63] = out[k];
+            }
+        __syncthreads();
+    }
 
     f32x4 dw[2][kTiles];
     if (WANT & kKernelGrad)
 #pragma unroll
         for (int i = 0; i < 2 * kTiles; ++i) dw[i / kTiles][i % kTiles] = f32x4{0, 0, 0, 0};
 
-    for (; base < n; base += 64 * step) {
+    Features<T> features;
+    const size_t step = (size_t)gridDim.x * waves;
+    // lane i looks after board base + i step; the boards of a small call go to different workgroups
+    for (size_t base = (size_t)wave * gridDim.x + blockIdx.x; base < n; base += 64 * step) {
         const bool in = base + lane * step < n;
         const int64_t t64 = in ? targets[base + lane * step] : 0;
         const bool valid = in && t64 >= 0 && t64 < kVocab;
@@ -250,63 +364,27 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
             if (loss) loss[base + lane * step] = 0.0f;
         }
         if (WANT & kFeaturesGrad)
-            for (uint64_t left = __ballot(in && !valid); left; left &= left - 1) {
-                u32x4* out = reinterpret_cast<u32x4*>(dx + (base + __builtin_ctzll(left) * step) * (kC * kS));
-#pragma unroll
-                for (int i = 0; i < (int)(kC * kS * sizeof(T) / 1024); ++i) out[i * 64 + lane] = u32x4{0, 0, 0, 0};
-            }
+            for (uint64_t left = __ballot(in && !valid); left; left &= left - 1)
+                zero_features_grad(dx + (base + __builtin_ctzll(left) * step) * (kC * kS), lane);
         uint64_t left = __ballot(valid);
-        if (left) load(base + __builtin_ctzll(left) * step);
+        if (left) features.load(x + (base + __builtin_ctzll(left) * step) * (kC * kS), col, q);
       while (left) {
         const int who = __builtin_ctzll(left);
         const size_t b = base + who * step;
         left &= left - 1;
-        const size_t next = base + (left ? __builtin_ctzll(left) : 0) * step;   // read ahead; after the last, in vain
+        const T* next = x + (base + (left ? __builtin_ctzll(left) : 0) * step) * (kC * kS);   // read ahead; after the last, in vain
         const int target = __builtin_amdgcn_readlane(my_target, who);
 
-        // features in their terms, pairs of squares packed
-        u32x2 rows[NT][8];
-        float x_scale = 1.0f, x_back = 1.0f;
-        if constexpr (sizeof(T) == 4) {
-            float largest = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) largest = larger(largest, fabsf(raw[i][j]));
-            scale_of(lanes_reduce<true>(largest), -100, x_scale, x_back);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    unsigned hi, lo;
-                    Arith<T>::split(raw[i][2 * j] * x_scale, raw[i][2 * j + 1] * x_scale, hi, lo);
-                    rows[0][i][j] = hi;
-                    rows[1][i][j] = lo;
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) rows[0][i] = __builtin_bit_cast(u32x2, raw[i]);
-        }
-        if (WANT == 0) load(next);
-
-        // as columns (square 4 col + j, channels 8 q ... 8 q + 7)
-        u32x4 xc[4][NT];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int k = 0; k < NT; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    xc[j][k][i] = __builtin_amdgcn_perm(rows[k][2 * i + 1][j >> 1], rows[k][2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
-
-        // and as rows (channel, squares by row of the crossing) for dW
-        u32x4 xr[2][2][NT];
+        features.convert();
+        const u32x4 (&xc)[4][NT] = features.column;
+        const float x_back = features.back;
+        if (WANT == 0) features.load(next, col, q);
+        u32x4 xr[2][2][NT];                      // and as rows (channel, k square) for dW
         if (WANT & kKernelGrad) {
-#pragma unroll
-            for (int i = 0; i < 4 * NT; ++i) *reinterpret_cast<u32x4*>(write_at + (i % NT) * kTerm + 16 * (i / NT) * kRow) = xc[i / NT][i % NT];
+            write_rows<NT>(mine, col, q, xc);
             lds_fence();
 #pragma unroll
-            for (int i = 0; i < 4 * NT; ++i) xr[i / NT >> 1][i / NT & 1][i % NT] = transposed(i % NT, i / NT & 1, i / NT >> 1);
+            for (int i = 0; i < 4 * NT; ++i) xr[i / NT >> 1][i / NT & 1][i % NT] = crossed(i % NT, i / NT & 1, i / NT >> 1);
             lds_fence();
         }
 
@@ -403,14 +481,14 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
                     d[j][0][i] = hi;
                     d[j][1][i] = lo;
                 }
-            if (u == 0) load(next);              // the first two tiles' registers are free
+            if (u == 0) features.load(next, col, q);   // the first two tiles' registers are free
             if (WANT & kKernelGrad) {
+                if (tiles == 2) write_rows<2>(mine, col, q, d);
+                else
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    short* p = write_at + (i & 1) * kTerm + 16 * (i >> 1) * kRow;
-                    if (tiles == 2) *reinterpret_cast<u32x4*>(p) = d[i >> 1][i & 1];
-                    else *reinterpret_cast<u32x2*>(p - 4 * q) = u32x2{d[i >> 1][i & 1][0], d[i >> 1][i & 1][1]};
-                }
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<u32x2*>(mine + (i & 1) * kTerm + (16 * (i >> 1) + col) * kRow + 4 * q) =
+                            u32x2{d[i >> 1][i & 1][0], d[i >> 1][i & 1][1]};
                 lds_fence();
             }
             if (WANT & kFeaturesGrad) {
@@ -426,7 +504,7 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
                         u32x4 dk[2][2];
 #pragma unroll
                         for (int i = 0; i < 2 * tiles; ++i)
-                            dk[i >> 1][i & 1] = transposed(i & 1, h, i >> 1);
+                            dk[i >> 1][i & 1] = crossed(i & 1, h, i >> 1);
                         products<T, NT, 2>(s, [&](int i, int k) { return xr[i & 1][h][k]; }, [&](int i, int k) { return dk[i >> 1][k]; });
                     }
 #pragma unroll
@@ -444,62 +522,51 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
                 lds_fence();
             }
         }
-        if (WANT & kFeaturesGrad) {
-            const float back = wb * w_back;
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const raw_t out = {(T)(g[4 * a][r] * back), (T)(g[4 * a + 1][r] * back), (T)(g[4 * a + 2][r] * back), (T)(g[4 * a + 3][r] * back)};
-                    *reinterpret_cast<raw_t*>(dx + b * (kC * kS) + (16 * a + 4 * q + r) * kS + 4 * col) = out;
-                }
-        }
+        if (WANT & kFeaturesGrad) store_features_grad(dx + b * (kC * kS), col, q, g, wb * w_back);
       }
     }
-
-    if (WANT & kKernelGrad) {
-        float* part = reinterpret_cast<float*>(mine);
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    // column c of a pair of tiles is filter 16 (c >> 2 & 1) + 4 (c >> 3) + (c & 3) of the pair's 32
-                    const int c = 16 * (t & 1) + col, f = t == 4 ? 64 + col : 32 * (t >> 1) + 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
-                    part[(16 * a + 4 * q + r) * (16 * kTiles) + f] = dw[a][t][r];
-                }
-        __syncthreads();
-        const float* all = reinterpret_cast<const float*>(smem + sizeof(HeadLds<T>));
-        for (int i = threadIdx.x; i < kXW; i += blockDim.x) {
-            const int c = i / kF, f = i % kF;
-            float a = 0.0f;
-            for (int k = 0; k < waves; ++k) a += all[k * (kWaveLds / 4) + c * 80 + f];
-            dw_part[(size_t)blockIdx.x * kXW + i] = a;
-        }
-    }
+    if (WANT & kKernelGrad)
+        store_part(dw, smem + sizeof(HeadLds<T>), kWaveLds, wave, waves, col, q, dw_part + (size_t)blockIdx.x * kXW, [](int t, int col) {
+            // column c of a pair of tiles is filter 16 (c >> 2 & 1) + 4 (c >> 3) + (c & 3) of the pair's 32
+            const int c = 16 * (t & 1) + col;
+            return t == 4 ? 64 + col : 32 * (t >> 1) + 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
+        });
 }
 
 // ---- the boards' own moves -------------------------------------------------------------------------------------------
 //
-// One wave a board, one lane a move (64 at a time), the board's features and the kernel in LDS.  A list of 32 moves needs
-// a hundredth of the vocabulary's products, so they are plain float32 sums; what bounds the kernel is reading the features and
-// writing their gradient, and next to it LDS.  A lane holds a move's logit; then 32 lanes a move, two moves at a time,
-// add the move's part to the kernel's gradient (kept in LDS over all the wave's boards) and to the features' gradient
-// (which takes the features' place).  Two moves that would meet take turns, so the sums are the same
-// every time.  (LDS's own float adds do the same in one instruction, but take 200 cycles each: 0.88 ms in place of
-// 0.35 for 65 536 boards.)
+// One wave a board again.  A list of 32 moves needs a hundredth of the vocabulary's products, and MFMAs make them nearly
+// free where the operands are cheap to gather: the features lie in LDS as rows of a square's channels, the kernel as rows of a
+// filter's, and a move names one of each.
 //
-// A wave's boards are neighbours: it finds where its lists begin by adding up the counts of all boards before it, a
-// byte a board beside the 8 to 16 KB that each board costs, and needs no pass over them beforehand.
+//   logits   16 moves' features times the same 16 moves' filters: the diagonal
+//   dX       rows channel, columns square, k move: the filters' rows by a transposed read, the gradients of the logits
+//            each in the column of its move's square, zero in the others
+//   dW       rows channel, columns filter, k move: the squares' rows, the gradients in the columns of their filters
+//
+// What bounds it is reading the features and writing their gradient.  A wave's boards are neighbours: it finds where its
+// lists begin by adding up the counts of all boards before its own, a byte a board beside the 8 to 16 KB that each
+// board costs, and needs no pass over them beforehand.
 
-constexpr int kHeadRow = 36;                     // floats a filter of the kernel in LDS
-constexpr int kXRow = 68;                        // floats a channel of the features, from square to square
-constexpr int kGRow = 33;                        // floats a square of their gradient, from channel to channel
-constexpr int kMoveHeadBytes = kF * kHeadRow * 4 + 16 * 8;
-constexpr int kMoveWaveBytes = kC * kXRow * 4 + 64 * 8;
-constexpr int kMoveGradBytes = kMoveWaveBytes + kF * kC * 4;
-static_assert(kS * kGRow <= kC * kXRow, "the gradient takes the features' place");
+template <typename T>
+struct MoveHeadLds {
+    short rows[Arith<T>::kTerms][kF][kRow];      // [filter][channel]
+    uint64_t sum[8];
+    float red[8];
+};
+static_assert(sizeof(MoveHeadLds<float>) % 16 == 0 && sizeof(MoveHeadLds<__bf16>) % 16 == 0, "the waves' parts are aligned");
+struct __attribute__((aligned(16))) MoveList {   // a board's moves, up to a multiple of 32; beyond its last, that again
+    float logit[256];
+    unsigned short hi[256], lo[256];             // terms of the logit's gradient
+    unsigned char square[256], filter[256];      // square: its row of features
+    unsigned square_tile[4][16];                 // for 32 moves, a pair a word: which of the pair is in the tile of columns
+    unsigned filter_tile[kTiles][16];
+};
+template <typename T>
+constexpr unsigned move_wave_bytes(int want) {
+    const unsigned rows = Arith<T>::kTerms * kTerm * 2, most = rows + sizeof(MoveList);
+    return (want & kKernelGrad) && most < (unsigned)kPartBytes ? kPartBytes : most;
+}
 
 struct __attribute__((packed)) Bytes16 { unsigned v[4]; };
 
@@ -508,6 +575,9 @@ __device__ __forceinline__ unsigned lanes_add(unsigned v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+// 0xffff in the half of each that is set
+__device__ __forceinline__ unsigned halves(bool low, bool high) { return (low ? 0xffffu : 0u) | (high ? 0xffff0000u : 0u); }
+
 template <typename T, int WANT>
 __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
                                                           const uint8_t* __restrict__ from, const uint8_t* __restrict__ filter,
@@ -515,23 +585,34 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                                                           const int64_t* __restrict__ targets, const float* __restrict__ weights,
                                                           unsigned weight_step, float* __restrict__ loss, T* __restrict__ dx,
                                                           float* __restrict__ dw_part, int* __restrict__ err) {
-    typedef typename Raw<T>::type raw_t;
+    constexpr int NT = Arith<T>::kTerms;
     extern __shared__ __align__(16) unsigned char smem[];
-    float* head = reinterpret_cast<float*>(smem);
-    uint64_t* red = reinterpret_cast<uint64_t*>(smem + kF * kHeadRow * 4);
+    MoveHeadLds<T>& head = *reinterpret_cast<MoveHeadLds<T>*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
-    const int col = lane & 15, q = lane >> 4, chan = lane & 31, half = lane >> 5;
-    unsigned char* mine = smem + kMoveHeadBytes + wave * (WANT & kKernelGrad ? kMoveGradBytes : kMoveWaveBytes);
-    float* xs = reinterpret_cast<float*>(mine);                                  // [32][68]
-    u32x2* entry = reinterpret_cast<u32x2*>(mine + kC * kXRow * 4);              // [64] (square | filter << 8, gradient)
-    float* dws = reinterpret_cast<float*>(mine + kMoveWaveBytes);                // [73][32], gradient calls only
+    const int col = lane & 15, q = lane >> 4;
+    unsigned char* const first_wave = smem + sizeof(MoveHeadLds<T>);
+    short* rows = reinterpret_cast<short*>(first_wave + wave * move_wave_bytes<T>(WANT));
+    MoveList& list = *reinterpret_cast<MoveList*>(rows + NT * kTerm);
 
+    float w_back;
+    {
+        float w_scale;
+        float* stage = reinterpret_cast<float*>(first_wave);
+        stage_head<T>(w, stage, head.red, w_scale, w_back);
+        for (int i = tid; i < kF * 4; i += blockDim.x) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = stage[(8 * (i & 3) + k) * kF + (i >> 2)];
+            u32x4 out[NT];
+            operand<T>(v, w_scale, out);
+#pragma unroll
+            for (int k = 0; k < NT; ++k) *reinterpret_cast<u32x4*>(&head.rows[k][i >> 2][8 * (i & 3)]) = out[k];
+        }
+    }
+
+    // the wave's boards [lo, hi), and where their lists begin
     const size_t all = (size_t)gridDim.x * waves, me = (size_t)blockIdx.x * waves + wave;
     const size_t lo = n * me / all, hi = n * (me + 1) / all, group_lo = n * (me - wave) / all;
-
-    for (int i = tid; i < kXW; i += blockDim.x) head[(i % kF) * kHeadRow + i / kF] = (float)w[i];
-    if (WANT & kKernelGrad)
-        for (int i = lane; i < kF * kC; i += 64) dws[i] = 0.0f;
     unsigned before = 0;
     for (size_t i = (size_t)tid * 16; i < group_lo; i += (size_t)blockDim.x * 16) {
         if (i + 16 <= group_lo) {
@@ -543,200 +624,278 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
         }
     }
     before = lanes_add(before);
-    if (lane == 0) red[wave] = before;
+    if (lane == 0) head.sum[wave] = before;
     before = 0;
     for (size_t i = group_lo + lane; i < lo; i += 64) before += per[i];
     uint64_t start = lanes_add(before);
     __syncthreads();
-    for (int i = 0; i < waves; ++i) start += red[i];
+    for (int i = 0; i < waves; ++i) start += head.sum[i];
 
-    raw_t raw[8];
-    auto load = [&](size_t b) {
+    f32x4 dw[2][kTiles];
+    if (WANT & kKernelGrad)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const raw_t*>(x + b * (kC * kS) + (4 * i + q) * kS + 4 * col);
-    };
-    if (lo < hi) load(lo);
-    unsigned counts = 0;
-    for (size_t b = lo; b < hi; ++b) {
-        if (((b - lo) & 63) == 0) counts = b + lane < hi ? per[b + lane] : 0u;
-        const unsigned listed = __builtin_amdgcn_readlane(counts, (int)((b - lo) & 63));
-        const uint64_t first = min(start, (uint64_t)n_moves);
-        const int cnt = (int)min((uint64_t)listed, n_moves - first);
-        start += listed;
-        const int64_t t64 = targets[b];
-        const int target = __builtin_amdgcn_readfirstlane(t64 >= 0 && t64 < cnt ? (int)t64 : -1);
+        for (int i = 0; i < 2 * kTiles; ++i) dw[i / kTiles][i % kTiles] = f32x4{0, 0, 0, 0};
 
+    Features<T> features;
+    for (size_t base = lo; base < hi; base += 64) {      // lane i looks after board base + i
+        const bool in = base + lane < hi;
+        const unsigned listed = in ? per[base + lane] : 0u;
+        unsigned upto = listed;                          // inclusive sum over the lanes
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<f32x4*>(xs + (4 * i + q) * kXRow + 4 * col) = f32x4{(float)raw[i][0], (float)raw[i][1], (float)raw[i][2], (float)raw[i][3]};
-        if (b + 1 < hi) load(b + 1);
-        lds_fence();
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned v = __shfl_up(upto, o);
+            upto += lane >= o ? v : 0u;
+        }
+        const uint64_t my_first = min(start + upto - listed, (uint64_t)n_moves);
+        const int my_count = (int)min((uint64_t)listed, n_moves - my_first);
+        start += (unsigned)__builtin_amdgcn_readlane(upto, 63);
+        const int64_t t64 = in ? targets[base + lane] : 0;
+        const bool valid = in && t64 >= 0 && t64 < my_count;
+        const float my_weight = WANT && valid ? weights[(base + lane) * weight_step] : 0.0f;
+        const int my_target = (int)t64;
+        if (in && !valid) {                      // no part in anything, whatever the features hold
+            if (t64 != -1) atomicOr(err, 8);
+            if (loss) loss[base + lane] = 0.0f;
+        }
+        for (uint64_t left = __ballot(in && !valid); left; left &= left - 1) {
+            const int who = __builtin_ctzll(left);
+            if (WANT & kFeaturesGrad) zero_features_grad(dx + (base + who) * (kC * kS), lane);
+            // its moves are looked over all the same
+            const uint64_t first = (uint64_t)(unsigned)__builtin_amdgcn_readlane((unsigned)my_first, who) |
+                                   (uint64_t)(unsigned)__builtin_amdgcn_readlane((unsigned)(my_first >> 32), who) << 32;
+            for (int m = lane; m < __builtin_amdgcn_readlane(my_count, who); m += 64)
+                if (from[first + m] >= kS || filter[first + m] >= kF) atomicOr(err, 8);
+        }
+        uint64_t left = __ballot(valid);
+        if (!left) continue;
 
-        float l[4];                              // [pass of 64 moves]
-        unsigned place[4];
-        float top = -INFINITY, l_target = 0.0f;
+        uint64_t first;                          // of the board at hand
+        int cnt;
+        unsigned square, filt;                   // its first 64 moves
+        auto look_up = [&](int who) {
+            first = (uint64_t)(unsigned)__builtin_amdgcn_readlane((unsigned)my_first, who) |
+                    (uint64_t)(unsigned)__builtin_amdgcn_readlane((unsigned)(my_first >> 32), who) << 32;
+            cnt = __builtin_amdgcn_readlane(my_count, who);
+            square = from[first + min(lane, cnt - 1)];
+            filt = filter[first + min(lane, cnt - 1)];
+            features.load(x + (base + who) * (kC * kS), col, q);
+        };
+        int who = __builtin_ctzll(left);
+        look_up(who);
+      while (true) {
+        const size_t b = base + who;
+        const int target = __builtin_amdgcn_readlane(my_target, who), count = cnt;
+        const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
+        features.convert();
+        const float x_back = features.back;
+        write_rows<NT>(rows, col, q, features.column);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-            l[p] = -INFINITY;
-            place[p] = 0;
-            if (64 * p >= cnt) continue;
-            if (64 * p + lane < cnt) {
-                unsigned s = from[first + 64 * p + lane], f = filter[first + 64 * p + lane];
-                if (s >= kS || f >= kF) atomicOr(err, 8);
-                s = min(s, kS - 1u);
-                f = min(f, kF - 1u);
-                place[p] = s | f << 8;
-                float a = 0.0f;
-#pragma unroll
-                for (int c = 0; c < kC; c += 4) {
-                    const f32x4 k = *reinterpret_cast<const f32x4*>(head + f * kHeadRow + c);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) a = fmaf(k[i], xs[(c + i) * kXRow + s], a);
-                }
-                l[p] = a;
+            if (64 * p >= count) continue;
+            if (p) {
+                square = from[first + min(64 * p + lane, count - 1)];
+                filt = filter[first + min(64 * p + lane, count - 1)];
             }
-            top = larger(top, l[p]);
-            if (target >> 6 == p) l_target = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l[p]), target & 63));
+            if (square >= kS || filt >= kF) atomicOr(err, 8);
+            square = min(square, kS - 1u);
+            list.square[64 * p + lane] = (unsigned char)(16 * (square & 3) + (square >> 2));
+            list.filter[64 * p + lane] = (unsigned char)min(filt, kF - 1u);
         }
-        if (target < 0) {                        // no part in anything, whatever the features hold
-            if (lane == 0) {
-                if (t64 != -1) atomicOr(err, 8);
-                if (loss) loss[b] = 0.0f;
-            }
-            if (WANT & kFeaturesGrad) {
-                u32x4* out = reinterpret_cast<u32x4*>(dx + b * (kC * kS));
+        left &= left - 1;
+        if (left) {
+            who = __builtin_ctzll(left);
+            look_up(who);
+        }
+        lds_fence();
+
+        // logits, in units of 2^-(scales)
+        for (int m = 0; m < count; m += 32) {
+            u32x4 a[2][NT], f[2][NT];
 #pragma unroll
-                for (int i = 0; i < (int)(kC * kS * sizeof(T) / 1024); ++i) out[i * 64 + lane] = u32x4{0, 0, 0, 0};
+            for (int i = 0; i < 2; ++i) {
+                const int sq = list.square[m + 16 * i + col], fl = list.filter[m + 16 * i + col];
+#pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    a[i][k] = *reinterpret_cast<const u32x4*>(rows + k * kTerm + sq * kRow + 8 * q);
+                    f[i][k] = *reinterpret_cast<const u32x4*>(&head.rows[k][fl][8 * q]);
+                }
             }
-            lds_fence();
-            continue;
+            f32x4 l[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            products<T, NT, NT>(l, [&](int i, int k) { return a[i][k]; }, [&](int i, int k) { return f[i][k]; });
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float even = col & 2 ? l[i][2] : l[i][0], odd = col & 2 ? l[i][3] : l[i][1];
+                if (q == col >> 2) list.logit[m + 16 * i + col] = col & 1 ? odd : even;
+            }
+        }
+        lds_fence();
+        const float l_target = list.logit[target];
+        float v[4], top = -INFINITY;             // [pass of 64 moves]
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            v[p] = -INFINITY;
+            if (64 * p >= count) continue;
+            if (64 * p + lane < count) v[p] = list.logit[64 * p + lane];
+            top = larger(top, v[p]);
         }
         top = lanes_reduce<true>(top);
+        const float unit = fminf(fmaxf(w_back * x_back, 1e-36f), 1e38f), unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
         float z = 0.0f;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-            if (64 * p >= cnt) continue;
-            l[p] = __builtin_amdgcn_exp2f((l[p] - top) * 1.44269504088896341f);
-            z += l[p];
+            if (64 * p >= count) continue;
+            v[p] = __builtin_amdgcn_exp2f(fmaf(v[p], unit2, top2));
+            z += v[p];
         }
         z = lanes_reduce<false>(z);
-        if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, top - l_target);
-        if (!WANT) {
-            lds_fence();
-            continue;
-        }
+        if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
 
-        const float wb = weights[b * weight_step], rz = __builtin_amdgcn_rcpf(z);
-        // One pass's moves, two at a time: move k by the lower lanes, move k + pairs by the upper ones.  to(place) is where
-        // a lane adds to, of(place) what of times the logit's gradient it adds; meet(a, b): two moves add to the same.
-        auto add_up = [&](int p, auto&& to, auto&& of, auto&& meet) {
-            const int here = min(cnt - 64 * p, 64), pairs = (here + 1) >> 1;
-            const float one = target == 64 * p + lane ? z : 0.0f;
-            lds_fence();
-            entry[lane] = u32x2{place[p], __float_as_uint((l[p] - one) * rz * wb)};
-            lds_fence();
-            const uint64_t turns = __ballot(lane + pairs < here && meet(entry[(lane + pairs) & 63][0], place[p]));
-            u32x2 e = entry[half * pairs];
-            float v = of(e[0]) * __uint_as_float(e[1]);
-            for (int k = 0; k < pairs; ++k) {
-                float* at = to(e[0]);
-                const float was = *at;
-                e = entry[min(k + 1 + half * pairs, 63)];
-                const float next = of(e[0]) * __uint_as_float(e[1]);   // in flight while this one is added
-                if (turns >> k & 1) {
-                    if (half == 0) *at = was + v;
-                    lds_fence();
-                    if (half == 1) *at += v;
-                } else if (k + half * pairs < here) {
-                    *at = was + v;
+        if (WANT) {
+            // the logits' gradients times z, as over the vocabulary
+            const float rz = __builtin_amdgcn_rcpf(z), e_target = __builtin_amdgcn_exp2f(fmaf(l_target, unit2, top2));
+            float inv = 1.0f, wb = weight;
+            if constexpr (Arith<T>::kScaled) {
+                float d_scale, d_back;
+                scale_of(fabsf(e_target - z) * rz, -17, d_scale, d_back);
+                inv = d_scale * rz;
+                wb *= d_back;
+            } else {
+                wb *= rz;
+            }
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                if (64 * p >= count) continue;
+                unsigned hi, lo;
+                Arith<T>::split((v[p] - (64 * p + lane == target ? z : 0.0f)) * inv, 0.0f, hi, lo);
+                list.hi[64 * p + lane] = (unsigned short)hi;
+                list.lo[64 * p + lane] = (unsigned short)lo;
+            }
+            f32x4 g[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[i] = f32x4{0, 0, 0, 0};
+            for (int m = 0; m < count; m += 32) {
+                {                                // pair `col`, tile q
+                    const unsigned s2 = *reinterpret_cast<const unsigned short*>(&list.square[m + 2 * col]);
+                    const unsigned f2 = *reinterpret_cast<const unsigned short*>(&list.filter[m + 2 * col]);
+                    list.square_tile[q][col] = halves((s2 >> 4 & 15) == (unsigned)q, s2 >> 12 == (unsigned)q);
+                    list.filter_tile[q][col] = halves((f2 >> 4 & 15) == (unsigned)q, f2 >> 12 == (unsigned)q);
+                    if (q == 0) list.filter_tile[4][col] = halves((f2 >> 4 & 15) == 4, f2 >> 12 == 4);
                 }
                 lds_fence();
-                v = next;
+                // the lane's eight moves m + 8 q ...: the terms, kept where the move's square or filter is in the lane's column
+                u32x4 d[2];
+                d[0] = *reinterpret_cast<const u32x4*>(&list.hi[m + 8 * q]);
+                d[1] = *reinterpret_cast<const u32x4*>(&list.lo[m + 8 * q]);
+                const int row_lo = m + 8 * q + (col >> 2), row_hi = row_lo + 4;   // whose row the lane names in a transposed read
+                auto in_column = [&](const unsigned char* of, u32x4 (&out)[2]) {
+                    const u32x2 s8 = *reinterpret_cast<const u32x2*>(of + m + 8 * q);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned pair = s8[i >> 1] >> 16 * (i & 1);
+                        const unsigned keep = halves((pair & 15) == (unsigned)col, (pair >> 8 & 15) == (unsigned)col);
+                        out[0][i] = d[0][i] & keep;
+                        out[1][i] = d[1][i] & keep;
+                    }
+                };
+                if (WANT & kFeaturesGrad) {
+                    u32x4 a[2][NT], mine[2], s[4][2];
+                    const short *w_lo = &head.rows[0][list.filter[row_lo]][4 * (col & 3)], *w_hi = &head.rows[0][list.filter[row_hi]][4 * (col & 3)];
+#pragma unroll
+                    for (int i = 0; i < 2 * NT; ++i) {
+                        const int at = (i % NT) * kF * kRow + 16 * (i / NT);
+                        a[i / NT][i % NT] = transposed(w_lo + at, w_hi + at);
+                    }
+                    in_column(list.square, mine);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.square_tile[j][4 * q]);
+                        s[j][0] = mine[0] & keep;
+                        s[j][1] = mine[1] & keep;
+                    }
+                    products<T, NT, 2>(g, [&](int i, int k) { return a[i >> 2][k]; }, [&](int i, int k) { return s[i & 3][k]; });
+                }
+                if (WANT & kKernelGrad) {
+                    u32x4 a[2][NT], mine[2];
+                    const short *x_lo = rows + list.square[row_lo] * kRow + 4 * (col & 3), *x_hi = rows + list.square[row_hi] * kRow + 4 * (col & 3);
+#pragma unroll
+                    for (int i = 0; i < 2 * NT; ++i) {
+                        const int at = (i % NT) * kTerm + 16 * (i / NT);
+                        a[i / NT][i % NT] = transposed(x_lo + at, x_hi + at);
+                    }
+                    in_column(list.filter, mine);
+                    const float w_scale = wb * x_back;
+                    f32x4 sum[2 * kTiles];
+                    u32x4 f[kTiles][2];
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.filter_tile[t][4 * q]);
+                        f[t][0] = mine[0] & keep;
+                        f[t][1] = mine[1] & keep;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2 * kTiles; ++i) sum[i] = f32x4{0, 0, 0, 0};
+                    products<T, NT, 2>(sum, [&](int i, int k) { return a[i & 1][k]; }, [&](int i, int k) { return f[i >> 1][k]; });
+#pragma unroll
+                    for (int i = 0; i < 8 * kTiles; ++i)
+                        dw[i >> 2 & 1][i >> 3][i & 3] = fmaf(sum[i >> 2][i & 3], w_scale, dw[i >> 2 & 1][i >> 3][i & 3]);
+                }
+                lds_fence();
             }
-        };
-        if (WANT & kKernelGrad)
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-                if (64 * p < cnt)
-                    add_up(p, [&](unsigned m) { return dws + (m >> 8) * kC + chan; }, [&](unsigned m) { return xs[chan * kXRow + (m & 0xff)]; },
-                           [](unsigned a, unsigned b) { return a >> 8 == b >> 8; });
-        if (WANT & kFeaturesGrad) {
-            lds_fence();
-            float* g = xs;                       // [64][33]
-            for (int i = lane; i < kS * kGRow; i += 64) g[i] = 0.0f;
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-                if (64 * p < cnt)
-                    add_up(p, [&](unsigned m) { return g + (m & 0xff) * kGRow + chan; }, [&](unsigned m) { return head[(m >> 8) * kHeadRow + chan]; },
-                           [](unsigned a, unsigned b) { return (a & 0xff) == (b & 0xff); });
-            lds_fence();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                raw_t out;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) out[j] = (T)g[(4 * col + j) * kGRow + 4 * i + q];
-                *reinterpret_cast<raw_t*>(dx + b * (kC * kS) + (4 * i + q) * kS + 4 * col) = out;
-            }
+            if (WANT & kFeaturesGrad) store_features_grad(dx + b * (kC * kS), col, q, g, wb * w_back);
         }
         lds_fence();
+        if (!left) break;
+      }
     }
     if (lo < hi && hi == n && lane == 0 && start != n_moves) atomicOr(err, 8);
-
     if (WANT & kKernelGrad) {
         __syncthreads();
-        for (int i = tid; i < kXW; i += blockDim.x) {
-            const int c = i / kF, f = i % kF;
-            float a = 0.0f;
-            for (int k = 0; k < waves; ++k)
-                a += reinterpret_cast<const float*>(smem + kMoveHeadBytes + k * kMoveGradBytes + kMoveWaveBytes)[f * kC + c];
-            dw_part[(size_t)blockIdx.x * kXW + i] = a;
-        }
+        store_part(dw, first_wave, move_wave_bytes<T>(WANT), wave, waves, col, q, dw_part + (size_t)blockIdx.x * kXW,
+                   [](int t, int col) { return 16 * t + col; });
     }
 }
 
-// The partial kernel gradients of the workgroups, added up in fixed order: a workgroup 32 elements, eight threads each.
+// The partial kernel gradients of the workgroups, added up in fixed order: a workgroup 32 elements, 32 threads each, whose
+// loads are all in flight at once.
+constexpr unsigned kGroups = 256;   // workgroups of a gradient call: one a compute unit, each with a part of the kernel's gradient
 template <typename T>
-__global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ part, unsigned parts, T* __restrict__ dw) {
-    __shared__ double sums[8][32];
-    const int i = blockIdx.x * 32 + (threadIdx.x & 31), j = threadIdx.x >> 5;
+__global__ __launch_bounds__(1024) void k_sum_parts(const float* __restrict__ part, unsigned parts, T* __restrict__ dw) {
+    __shared__ double sums[32][33];
+    const int i = threadIdx.x & 31, j = threadIdx.x >> 5;
     double a = 0.0;
-#pragma unroll 8
-    for (unsigned p = j; p < parts; p += 8) a += part[(size_t)p * kXW + i];
-    sums[j][threadIdx.x & 31] = a;
-    __syncthreads();
-    if (j == 0) {
-        for (int k = 1; k < 8; ++k) a += sums[k][threadIdx.x];
-        dw[i] = (T)(float)a;
+#pragma unroll
+    for (unsigned k = 0; k < kGroups / 32; ++k) {
+        const unsigned p = j + 32 * k;
+        a += p < parts ? part[(size_t)p * kXW + blockIdx.x * 32 + i] : 0.0f;
     }
+    sums[i][j] = a;
+    __syncthreads();
+    a = sums[j][i];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) a += __shfl_xor(a, o);
+    if (i == 0) dw[blockIdx.x * 32 + j] = (T)(float)a;
 }
 static_assert(kXW % 32 == 0, "k_sum_parts needs no bounds check");
-
-constexpr unsigned kGroups = 256;   // workgroups of a gradient call: one a compute unit, each with a part of the kernel's gradient
-
-// Waves a workgroup: small calls are spread over the compute units.
-unsigned waves_for(size_t n, unsigned most) {
-    unsigned waves = 1;
-    while (waves < most && (size_t)waves * kGroups < n) waves *= 2;
-    return waves;
-}
 
 template <typename T, int WANT>
 hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
     const T *x = static_cast<const T*>(a.features), *w = static_cast<const T*>(a.kernel);
     T* dx = static_cast<T*>(a.d_features);
     float* part = static_cast<float*>(a.workspace);
-    const unsigned waves = waves_for(a.n, WANT ? 8 : 4), step = a.n_weights > 1 ? 1u : 0u;
-    const unsigned grid = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, WANT ? kGroups : 4 * kGroups);
+    // At least four waves a workgroup, which share the work on the kernel; the boards of a call of up to 1024 are spread
+    // over the compute units.  Without gradients more workgroups fit a compute unit.
+    const unsigned waves = WANT && a.n > 4 * kGroups ? 8 : 4, step = a.n_weights > 1 ? 1u : 0u;
+    const unsigned grid = (unsigned)std::min<size_t>(a.n, WANT || a.n <= 4 * kGroups ? kGroups : 4 * kGroups);
     if (grid && a.per_board)
         hipLaunchKernelGGL((k_policy_move_loss<T, WANT>), dim3(grid), dim3(waves * 64),
-                           kMoveHeadBytes + waves * (WANT & kKernelGrad ? kMoveGradBytes : kMoveWaveBytes), s, x, w, a.n, a.from,
-                           a.filter, a.per_board, a.n_moves, a.targets, a.weights, step, a.loss, dx, part, a.err);
+                           sizeof(MoveHeadLds<T>) + std::max<unsigned>(waves * move_wave_bytes<T>(WANT), kStageBytes), s, x, w, a.n, a.from, a.filter, a.per_board,
+                           a.n_moves, a.targets, a.weights, step, a.loss, dx, part, a.err);
     else if (grid)
         hipLaunchKernelGGL((k_policy_loss<T, WANT>), dim3(grid), dim3(waves * 64),
-                           sizeof(HeadLds<T>) + (WANT & kKernelGrad ? waves * kWaveLds : 0), s, x, w, a.n, a.targets, a.weights, step,
-                           a.loss, dx, part, a.err);
+                           sizeof(HeadLds<T>) + std::max(WANT & kKernelGrad ? waves * kWaveLds : 0u, (unsigned)kStageBytes), s, x, w,
+                           a.n, a.targets, a.weights, step, a.loss, dx, part, a.err);
     if (hipError_t e = hipGetLastError()) return e;
-    if (WANT & kKernelGrad) hipLaunchKernelGGL(k_sum_parts<T>, dim3(kXW / 32), dim3(256), 0, s, part, grid, static_cast<T*>(a.d_kernel));
+    if (WANT & kKernelGrad) hipLaunchKernelGGL(k_sum_parts<T>, dim3(kXW / 32), dim3(1024), 0, s, part, grid, static_cast<T*>(a.d_kernel));
     return hipGetLastError();
 }
 
