@@ -10,6 +10,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # BATCHFIRST_LIB: another build of the same library (A/B timing and diagnostics, tools/build_variant.sh)
 LIB_PATH = os.environ.get("BATCHFIRST_LIB") or os.path.join(_HERE, "libbatchfirst_hip.so")
+TORCH_PATH = os.path.join(_HERE, "libbatchfirst_torch.so")
 
 BF_OK, BF_E_ARG, BF_E_HIP, BF_E_FORMAT, BF_E_NOGPU = 0, -1, -2, -3, -4
 BF_PRECISION_F32, BF_PRECISION_BF16, BF_PRECISION_F32_SPLIT, BF_PRECISION_F32_SPLIT3 = 0, 1, 2, 3
@@ -91,6 +92,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_torch = None
 
 
 class BatchFirstError(RuntimeError):
@@ -113,6 +115,25 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def load_torch():
+    """Load the training operators' torch registration (csrc/torch_ops.cpp) and bind it to the library."""
+    global _torch
+    if _torch is not None:
+        return _torch
+    if not os.path.exists(TORCH_PATH):
+        raise ImportError("%s is missing: the torch operators have not been built (run __graft_entry__.build())" % TORCH_PATH)
+    import torch
+    torch.ops.load_library(TORCH_PATH)
+    lib, ext = load(), ctypes.CDLL(TORCH_PATH)
+    ext.bf_torch_bind.argtypes, ext.bf_torch_bind.restype = [_c.POINTER(_vp)], None
+    ext.bf_torch_context.argtypes, ext.bf_torch_context.restype = [_vp, _int], None
+    names = ("bf_last_error", "bf_policy_loss", "bf_policy_loss_grad", "bf_policy_loss_workspace", "bf_policy_move_loss",
+             "bf_policy_move_loss_grad", "bf_global_norm", "bf_clip_grad_norm", "bf_grad_norm_workspace")
+    ext.bf_torch_bind((_vp * len(names))(*[_c.cast(getattr(lib, n), _vp) for n in names]))
+    _torch = ext
+    return ext
 
 
 def check(rc):

@@ -22,15 +22,20 @@ features' type):
     torch.ops.batchfirst.global_norm(ctx, tensors)                                 -> f32[]
     torch.ops.batchfirst.clip_grad_norm_(ctx, tensors, max_norm)                   -> f32[], tensors scaled in place
 
-The two losses are differentiable in the features and the kernel; the ``_grad`` forms give loss and gradients in one
-pass where the boards' weights in the total are known beforehand.
+``policy_loss`` is the softmax cross entropy of one target a board over the 73 x 64 move vocabulary; a target is
+move_filter * 64 + from_square in the mover's frame, or -1 (none: loss 0).  ``policy_move_loss`` is the same over each
+board's own moves, as ``policy_scores`` takes them; a target is a place in the board's list, or -1.  Both are
+differentiable in the features and the kernel; the ``_grad`` forms give the losses and the gradients of
+sum(board_weights * loss) in one pass where the boards' weights (f32[N] or [1]) are known beforehand, and an empty tensor
+for a gradient that is not asked for.  No call waits for the device: targets, squares and filters out of range, and lists
+that do not add up, are reported by :meth:`DeviceContext.check_policy` afterwards (a target then counts as -1).
+``clip_grad_norm_`` scales by min(1, max_norm / (norm + 1e-6)) and returns the norm before.
 
 ``ctx`` is the integer handle of a :class:`DeviceContext`.  occupied_bbs travels as int64
 because torch has no first-class uint64; only the bits matter (the reference's placeholder is
 int64 too, ann_creation_helper.py:51).
 """
 import ctypes
-from typing import Tuple
 
 import numpy as np
 import torch
@@ -39,6 +44,7 @@ from . import _lib
 from .chestimator import _as_blob, _as_policy_blob
 
 _contexts = {}
+_torch = _lib.load_torch()
 
 
 class DeviceContext:
@@ -54,6 +60,7 @@ class DeviceContext:
         self.device = torch.device("cuda", int(device))
         self.handle = int(ctx.value)
         _contexts[self.handle] = self
+        _torch.bf_torch_context(ctx, int(device))
 
     def set_policy(self, policy_weights):
         blob = _as_policy_blob(policy_weights)
@@ -69,6 +76,7 @@ class DeviceContext:
     def close(self):
         if self._ctx is not None:
             _contexts.pop(self.handle, None)
+            _torch.bf_torch_context(self._ctx, -1)
             self._lib.bf_ctx_destroy(self._ctx)
             self._ctx = None
 
@@ -219,205 +227,14 @@ def policy_scores(ctx: int, features: torch.Tensor, from_squares: torch.Tensor, 
     return out
 
 
-_TYPES = {torch.float32: _lib.BF_TYPE_F32, torch.bfloat16: _lib.BF_TYPE_BF16, torch.float16: _lib.BF_TYPE_F16}
-
-
-def _aligned(t):
-    """The kernels load 16 bytes at a time; a view may start anywhere."""
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _head(c, features, logit_kernel, targets):
-    """Checked (features, kernel, targets) of a loss."""
-    if features.dtype not in _TYPES:
-        raise ValueError("features must be float32, bfloat16 or float16")
-    x = _dev(features, features.dtype, "features", c)
-    if tuple(x.shape[1:]) not in ((32, 8, 8), (32, 64)):
-        raise ValueError("features must have shape [N, 32, 8, 8] or [N, 32, 64]")
-    w = _dev(logit_kernel, features.dtype, "logit_kernel", c)
-    if tuple(w.shape) not in ((32, 73), (1, 1, 32, 73)):
-        raise ValueError("logit_kernel must have shape [32, 73] or [1, 1, 32, 73]")
-    t = _dev(targets, torch.int64, "targets", c)
-    if t.dim() != 1 or t.numel() != x.shape[0]:
-        raise ValueError("targets needs one entry per board")
-    return _aligned(x), _aligned(w), t
-
-
-def _move_lists(c, from_squares, move_filters, moves_per_board, n):
-    frm = _dev(from_squares, torch.uint8, "from_squares", c)
-    flt = _dev(move_filters, torch.uint8, "move_filters", c)
-    per = _dev(moves_per_board, torch.uint8, "moves_per_board", c)
-    if per.numel() != n or frm.numel() != flt.numel():
-        raise ValueError("moves_per_board needs one entry per board, from_squares and move_filters one per move")
-    return frm, flt, per
-
-
-def _board_weights(c, board_weights, n):
-    g = board_weights
-    if g.dim() == 1 and g.numel() > 1 and g.stride(0) == 0:
-        g = g[:1]                     # one weight for all boards: what a mean's or a sum's gradient is
-    g = _dev(g, torch.float32, "board_weights", c)
-    if g.dim() > 1 or g.numel() not in (1, n):
-        raise ValueError("board_weights needs one entry, or one per board")
-    return g
-
-
-def _loss(name, c, x, w, t, lists):
-    n = x.shape[0]
-    loss = torch.empty(n, dtype=torch.float32, device=x.device)
-    _lib.check(getattr(c._lib, name)(c._ctx, x.data_ptr(), _TYPES[x.dtype], n, w.data_ptr(), *lists, t.data_ptr(), loss.data_ptr(),
-                                     _stream(x.device)))
-    return loss
-
-
-def _loss_grad(name, c, x, w, t, lists, board_weights, features_grad, kernel_grad):
-    n = x.shape[0]
-    g = _board_weights(c, board_weights, n)
-    loss = torch.empty(n, dtype=torch.float32, device=x.device)
-    dx = torch.empty_like(x) if features_grad else x.new_empty(0)
-    dw = torch.empty_like(w) if kernel_grad else w.new_empty(0)
-    work = torch.empty(c._lib.bf_policy_loss_workspace(n) if kernel_grad else 0, dtype=torch.uint8, device=x.device)
-    _lib.check(getattr(c._lib, name + "_grad")(
-        c._ctx, x.data_ptr(), _TYPES[x.dtype], n, w.data_ptr(), *lists, t.data_ptr(), g.data_ptr(), g.numel(), loss.data_ptr(),
-        dx.data_ptr() if features_grad else None, dw.data_ptr() if kernel_grad else None, work.data_ptr(), work.numel(),
-        _stream(x.device)))
-    return loss, dx, dw
-
-
-@torch.library.custom_op("batchfirst::policy_loss", mutates_args=())
-def policy_loss(ctx: int, features: torch.Tensor, logit_kernel: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-    """Softmax cross entropy of one target a board over the 73 x 64 move vocabulary; a target is
-    move_filter * 64 + from_square in the mover's frame, or -1 (loss 0).  Targets out of range count as -1 and are
-    reported by :meth:`DeviceContext.check_policy`."""
-    c = _ctx(ctx)
-    return _loss("bf_policy_loss", c, *_head(c, features, logit_kernel, targets), ())
-
-
-@torch.library.custom_op("batchfirst::policy_loss_grad", mutates_args=())
-def policy_loss_grad(ctx: int, features: torch.Tensor, logit_kernel: torch.Tensor, targets: torch.Tensor,
-                     board_weights: torch.Tensor, features_grad: bool = True,
-                     kernel_grad: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(loss[N], gradients of sum(board_weights * loss)) in one pass; board_weights float32[N] or [1].  A gradient that
-    is not asked for comes back empty."""
-    c = _ctx(ctx)
-    return _loss_grad("bf_policy_loss", c, *_head(c, features, logit_kernel, targets), (), board_weights, features_grad, kernel_grad)
-
-
-@torch.library.custom_op("batchfirst::policy_move_loss", mutates_args=())
-def policy_move_loss(ctx: int, features: torch.Tensor, logit_kernel: torch.Tensor, from_squares: torch.Tensor,
-                     move_filters: torch.Tensor, moves_per_board: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-    """The same over each board's own moves, as :func:`policy_scores` takes them; a target is a place in the board's
-    list, or -1 (a board without moves has no other).  Lists that do not add up, squares, filters or targets out of
-    range are reported by :meth:`DeviceContext.check_policy`; the call itself never waits for the device."""
-    c = _ctx(ctx)
-    x, w, t = _head(c, features, logit_kernel, targets)
-    frm, flt, per = _move_lists(c, from_squares, move_filters, moves_per_board, x.shape[0])
-    return _loss("bf_policy_move_loss", c, x, w, t, (frm.data_ptr(), flt.data_ptr(), per.data_ptr(), frm.numel()))
-
-
-@torch.library.custom_op("batchfirst::policy_move_loss_grad", mutates_args=())
-def policy_move_loss_grad(ctx: int, features: torch.Tensor, logit_kernel: torch.Tensor, from_squares: torch.Tensor,
-                          move_filters: torch.Tensor, moves_per_board: torch.Tensor, targets: torch.Tensor,
-                          board_weights: torch.Tensor, features_grad: bool = True,
-                          kernel_grad: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    c = _ctx(ctx)
-    x, w, t = _head(c, features, logit_kernel, targets)
-    frm, flt, per = _move_lists(c, from_squares, move_filters, moves_per_board, x.shape[0])
-    return _loss_grad("bf_policy_move_loss", c, x, w, t, (frm.data_ptr(), flt.data_ptr(), per.data_ptr(), frm.numel()), board_weights,
-                      features_grad, kernel_grad)
-
-
-def _save_inputs(ctx, inputs, output):
-    ctx.handle = inputs[0]
-    ctx.save_for_backward(*inputs[1:])
-
-
-def _backward_of(grad_op, lists):
-    def backward(ctx, g):
-        # the registered op, so that differentiating a second time is refused instead of silently wrong
-        _, dx, dw = grad_op(ctx.handle, *ctx.saved_tensors, g, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
-        return (None, dx if ctx.needs_input_grad[1] else None, dw if ctx.needs_input_grad[2] else None) + (None,) * (lists + 1)
-    return backward
-
-
-policy_loss.register_autograd(_backward_of(policy_loss_grad, 0), setup_context=_save_inputs)
-policy_move_loss.register_autograd(_backward_of(policy_move_loss_grad, 3), setup_context=_save_inputs)
-
-
-def _dense(t):
-    return t.is_contiguous() or torch._prims_common.is_non_overlapping_and_dense(t)
-
-
-def _span(t):
-    last = sum((k - 1) * s for k, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-
-def _norm_tables(c, tensors):
-    """Flat tensors and the host tables of their pointers, element counts and types.  The elements' order does not
-    matter, so a dense tensor is taken as it lies; one with gaps or repeats is copied."""
-    try:
-        types = np.array([_TYPES[t.dtype] for t in tensors], np.int32)
-    except KeyError:
-        raise ValueError("tensors must be float32, bfloat16 or float16") from None
-    index, flat = c.device.index, tensors
-    if not all([t.get_device() == index and t.is_contiguous() for t in tensors]):
-        flat = [t if t.get_device() == index and _dense(t) else _dev(t, t.dtype, "tensors", c) for t in tensors]
-    ptrs = np.array([t.data_ptr() for t in flat], np.uint64)
-    counts = np.array([t.numel() for t in flat], np.uint64)
-    n = len(flat)
-    work = torch.empty(c._lib.bf_grad_norm_workspace(n), dtype=torch.uint8, device=c.device)
-    return flat, (ptrs, counts, types), (ptrs.ctypes.data, counts.ctypes.data, types.ctypes.data, n), work
-
-
-def _check_gapped(tensors):
-    """The library refuses dense tensors that overlap; tensors with gaps reach it as copies and are checked here."""
-    if all([t.is_contiguous() for t in tensors]):
-        return
-    for i, t in enumerate(tensors):
-        if t.numel() == 0 or _dense(t):
-            continue
-        if any(s == 0 and k > 1 for s, k in zip(t.stride(), t.shape)):
-            raise ValueError("a tensor to clip must not be expanded")
-        lo, hi = _span(t)
-        for j, o in enumerate(tensors):
-            if j != i and o.numel() and _span(o)[0] < hi and lo < _span(o)[1]:
-                raise ValueError("two of the tensors to clip overlap or interleave")
-
-
-# Registered by hand: custom_op's wrappers visit every tensor of a list in Python several times over, 118 us for 307
-# tensors where these take 20.
-_lists = torch.library.Library("batchfirst", "FRAGMENT")
-_lists.define("global_norm(int ctx, Tensor[] tensors) -> Tensor")
-_lists.define("clip_grad_norm_(int ctx, Tensor(a!)[] tensors, float max_norm) -> Tensor")
-
-
-@torch.library.impl(_lists, "global_norm", "CompositeExplicitAutograd")
-def global_norm(ctx, tensors):
-    """The 2-norm over all elements of all tensors, a float32 scalar on the device; not differentiable."""
-    c = _ctx(ctx)
-    flat, _keep, tables, work = _norm_tables(c, tensors)
-    norm = torch.empty((), dtype=torch.float32, device=c.device)
-    _lib.check(c._lib.bf_global_norm(c._ctx, *tables, norm.data_ptr(), work.data_ptr(), work.numel(), _stream(c.device)))
-    return norm
-
-
-@torch.library.impl(_lists, "clip_grad_norm_", "CompositeExplicitAutograd")
-def clip_grad_norm_(ctx, tensors, max_norm):
-    """Scale all tensors in place by min(1, max_norm / (norm + 1e-6)); returns the norm before."""
-    c = _ctx(ctx)
-    if any([t.requires_grad for t in tensors]):
-        raise ValueError("tensors to clip are gradients: they must not require grad themselves")
-    _check_gapped(tensors)
-    flat, _keep, tables, work = _norm_tables(c, tensors)
-    norm = torch.empty((), dtype=torch.float32, device=c.device)
-    _lib.check(c._lib.bf_clip_grad_norm(c._ctx, *tables, max_norm, norm.data_ptr(), work.data_ptr(), work.numel(), _stream(c.device)))
-    torch.autograd.graph.increment_version(tensors)
-    if flat is not tensors:
-        for t, f in zip(tensors, flat):
-            if f is not t:
-                t.copy_(f)
-    return norm
+# The training operators are registered by libbatchfirst_torch.so (csrc/torch_ops.cpp), in C++ because their calls are as
+# short as a Python body's own time.
+policy_loss = torch.ops.batchfirst.policy_loss
+policy_loss_grad = torch.ops.batchfirst.policy_loss_grad
+policy_move_loss = torch.ops.batchfirst.policy_move_loss
+policy_move_loss_grad = torch.ops.batchfirst.policy_move_loss_grad
+global_norm = torch.ops.batchfirst.global_norm
+clip_grad_norm_ = torch.ops.batchfirst.clip_grad_norm_
 
 
 def eval_mailbox_debug(ctx, mailbox):

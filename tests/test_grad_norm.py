@@ -66,17 +66,21 @@ def test_refusals_of_the_c_entry_points():
 
 
 def test_gapped_tensors_that_overlap_are_refused():
+    """The check comes before the one that the tensors are on the context's device."""
     from batch_first_amd import ops
-    t = torch.zeros(8, 8)
-    ops._check_gapped([t, torch.zeros(4)])
-    ops._check_gapped([t[:, :4], torch.zeros(4)])
-    ops._check_gapped([t[:4, :4], t[4:, :4]])
-    for bad in ([t[:, :4], t], [t[:, :4], t[:, :4]], [t[::2], t[1::2]]):
-        with pytest.raises(ValueError, match="overlap"):
-            ops._check_gapped(bad)
-    with pytest.raises(ValueError, match="expanded"):
-        ops._check_gapped([torch.zeros(4, 1).expand(4, 4)])
-    ops._check_gapped([t[:0, :4], t])
+    clip, t = torch.ops.batchfirst.clip_grad_norm_, torch.zeros(8, 8)
+    ops._torch.bf_torch_context(1, 0)
+    try:
+        for good in ([t, torch.zeros(4)], [t[:, :4], torch.zeros(4)], [t[:4, :4], t[4:, :4]], [t[:0, :4], t]):
+            with pytest.raises(ValueError, match="device tensor"):
+                clip(1, good, 1.0)
+        for bad in ([t[:, :4], t], [t[:, :4], t[:, :4]], [t[::2], t[1::2]]):
+            with pytest.raises(ValueError, match="overlap"):
+                clip(1, bad, 1.0)
+        with pytest.raises(ValueError, match="expanded"):
+            clip(1, [torch.zeros(4, 1).expand(4, 4)], 1.0)
+    finally:
+        ops._torch.bf_torch_context(1, -1)
 
 
 # ---- on the GPU ------------------------------------------------------------------------------------------------------

@@ -157,13 +157,22 @@ def test_refusals_of_the_c_entry_points():
 
 def test_ops_refuse_host_tensors_and_unknown_contexts():
     from batch_first_amd import ops
+    o = torch.ops.batchfirst
     x, k, t = torch.zeros(2, 32, 8, 8), torch.zeros(32, 73), torch.zeros(2, dtype=torch.int64)
     with pytest.raises(ValueError, match="unknown batchfirst context"):
-        torch.ops.batchfirst.policy_loss(1, x, k, t)
-    with pytest.raises(ValueError, match="device tensor"):
-        ops._head(None, x, k, t)
-    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
-        ops._head(None, x.double(), k, t)
+        o.policy_loss(1, x, k, t)
+    ops._torch.bf_torch_context(1, 0)
+    try:
+        with pytest.raises(ValueError, match="device tensor"):
+            o.policy_loss(1, x, k, t)
+        with pytest.raises(ValueError, match="device tensor"):
+            o.policy_loss(1, x.requires_grad_(), k, t)
+        with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+            o.policy_loss_grad(1, x.double(), k, t, torch.ones(1))
+    finally:
+        ops._torch.bf_torch_context(1, -1)
+    with pytest.raises(ValueError, match="unknown batchfirst context"):
+        o.policy_loss(1, x, k, t)
 
 
 # ---- on the GPU ------------------------------------------------------------------------------------------------------
