@@ -58,11 +58,13 @@ struct Arith {                                   // float32 and float16 features
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
     }
-    // (a, b) = terms hi + lo, each packed with a in the low half; rounded towards zero, so lo has hi's sign
+    // (a, b) = terms hi + lo, each packed with a in the low half.  Rounded to nearest: towards zero (which packs in one
+    // instruction as well) both terms and the product that is left out err to one side, 8e-7 of a gradient in place of 1e-7.
     static __device__ __forceinline__ void split(float a, float b, unsigned& hi, unsigned& lo) {
-        const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-        hi = __builtin_bit_cast(unsigned, h);
-        lo = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+        hi = __builtin_bit_cast(unsigned, half2v{(_Float16)a, (_Float16)b});
+        asm("" : "+v"(hi));                      // one rounding for both uses: a product a may be contracted into either
+        const half2v h = __builtin_bit_cast(half2v, hi);
+        lo = __builtin_bit_cast(unsigned, half2v{(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])});
     }
 };
 template <>
@@ -74,6 +76,7 @@ struct Arith<__bf16> {
     }
     static __device__ __forceinline__ void split(float a, float b, unsigned& hi, unsigned& lo) {
         hi = __builtin_bit_cast(unsigned, bf2{(__bf16)a, (__bf16)b});
+        asm("" : "+v"(hi));
         lo = __builtin_bit_cast(unsigned, bf2{(__bf16)(a - __uint_as_float(hi << 16)), (__bf16)(b - __uint_as_float(hi & 0xffff0000u))});
     }
 };
