@@ -909,9 +909,12 @@ hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
     float* part = static_cast<float*>(a.workspace);
     // At least four waves a workgroup, which share the work on the kernel.  (Spreading a small call's boards over all
     // compute units, one or two a workgroup, leaves more parts to add up: 17.6 in place of 16.4 us for 512 boards.)
-    // Without gradients more workgroups fit a compute unit.
+    // Without gradients more workgroups fit a compute unit, and as many are launched: of float32 three (registers) over the
+    // vocabulary and two (LDS) over moves, else four.  One more that has to wait costs more than it brings: 40 000 boards
+    // of float32 over moves in 62 us with two, 77 with three; 5 000 over the vocabulary in 14.2 us with three, 17.5 with four.
     const unsigned waves = WANT && a.n > 4 * kGroups ? 8 : 4, step = a.n_weights > 1 ? 1u : 0u;
-    const unsigned grid = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, WANT ? kGroups : 4 * kGroups);
+    const unsigned most = WANT ? kGroups : (sizeof(T) == 2 ? 4 : a.per_board ? 2 : 3) * kGroups;
+    const unsigned grid = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, most);
     if (grid && a.per_board)
         hipLaunchKernelGGL((k_policy_move_loss<T, WANT>), dim3(grid), dim3(waves * 64),
                            sizeof(MoveHeadLds<T>) + std::max<unsigned>(waves * move_wave_bytes<T>(WANT), kStageBytes), s, x, w, a.n, a.from, a.filter, a.per_board,
