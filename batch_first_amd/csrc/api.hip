@@ -303,12 +303,27 @@ int read_err_flag(Lane* c, hipStream_t s) {
     if (flag) {
         BF_HIP(hipMemsetAsync(c->d_err, 0, sizeof(int), s));
         BF_HIP(hipStreamSynchronize(s));
-        if (flag & 8) return bf::fail(BF_E_FORMAT, "loss input: a target or the move lists are out of range");
         if (flag & 4) return bf::fail(BF_E_FORMAT, "move input: board index, from-square or move filter out of range");
         if (flag & 2) return bf::fail(BF_E_FORMAT, "wire input holds code 15, which is not a piece code");
         return bf::fail(BF_E_FORMAT, "wire input: piece_filters length does not match the popcounts of occupied_bbs");
     }
     return BF_OK;
+}
+
+// The losses' own flag, in the block that d_err points to, so that only bf_policy_check reports it (a prediction's finish
+// call reads the lane's flag).
+int* loss_flag(const bf_ctx* c) { return c->policy.d_err + 32; }
+
+// Call with the policy lane's mutex held.
+int read_loss_flag(bf_ctx* c, hipStream_t s) {
+    Lane* L = &c->policy;
+    *L->h_flag = 0;
+    BF_HIP(hipMemcpyAsync(L->h_flag, loss_flag(c), sizeof(int), hipMemcpyDeviceToHost, s));
+    BF_HIP(hipStreamSynchronize(s));
+    if (!*L->h_flag) return BF_OK;
+    BF_HIP(hipMemsetAsync(loss_flag(c), 0, sizeof(int), s));
+    BF_HIP(hipStreamSynchronize(s));
+    return bf::fail(BF_E_FORMAT, "loss input: a target or the move lists are out of range");
 }
 
 constexpr size_t kMaxBoards = (size_t)1 << 26;
@@ -952,7 +967,8 @@ extern "C" int bf_policy_check(bf_ctx* c, void* stream) {
     if (!c) return bf::fail(BF_E_ARG, "bf_policy_check: null context");
     DeviceGuard guard(c->device);
     std::lock_guard<std::mutex> lock(c->policy.mu);
-    return read_err_flag(&c->policy, (hipStream_t)stream);
+    if (int r = read_err_flag(&c->policy, (hipStream_t)stream)) return r;
+    return read_loss_flag(c, (hipStream_t)stream);
 }
 
 // ---- losses of the move-scoring head, gradient clipping ------------------------------------------
@@ -981,7 +997,7 @@ int check_loss(bf_ctx* c, bf::PolicyLossArgs* a, bool grad, size_t workspace_byt
     const size_t need = a->d_kernel ? bf::policy_loss_workspace(a->n) : 0;
     if (workspace_bytes < need || (need && !a->workspace))
         return bf::fail(BF_E_ARG, "%s: the workspace has %zu bytes, %zu are needed", who, a->workspace ? workspace_bytes : 0, need);
-    a->err = c->policy.d_err;
+    a->err = loss_flag(c);
     return BF_OK;
 }
 

@@ -24,7 +24,7 @@ struct PolicyLossArgs {
     void* d_features;
     void* d_kernel;
     void* workspace;              // with d_kernel: policy_loss_workspace bytes, 16-byte aligned
-    int* err;                     // sticky flag, bit 8: target or move list out of range
+    int* err;                     // sticky flag: a target or a move list is out of range
 };
 size_t policy_loss_workspace(size_t n);
 hipError_t launch_policy_loss(const PolicyLossArgs& args, hipStream_t stream);

@@ -372,7 +372,7 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
         const bool in = base + lane * step < n, valid = t64 >= 0 && t64 < kVocab;
         const int my_target = (int)t64;
         if (in && !valid) {                      // no part in anything, whatever the features hold
-            if (t64 != -1) atomicOr(err, 8);
+            if (t64 != -1) atomicOr(err, 1);
             if (loss) loss[base + lane * step] = 0.0f;
         }
         if (WANT & kFeaturesGrad)
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
         const bool valid = t64 >= 0 && t64 < my_count;
         const int my_target = (int)t64;
         if (in && !valid) {                      // no part in anything, whatever the features hold
-            if (t64 != -1) atomicOr(err, 8);
+            if (t64 != -1) atomicOr(err, 1);
             if (loss) loss[base + lane] = 0.0f;
         }
         for (uint64_t left = __ballot(in && !valid); left; left &= left - 1) {
@@ -689,7 +689,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
             const uint64_t first = (uint64_t)(unsigned)__builtin_amdgcn_readlane((unsigned)my_first, who) |
                                    (uint64_t)(unsigned)__builtin_amdgcn_readlane((unsigned)(my_first >> 32), who) << 32;
             for (int m = lane; m < __builtin_amdgcn_readlane(my_count, who); m += 64)
-                if (from[first + m] >= kS || filter[first + m] >= kF) atomicOr(err, 8);
+                if (from[first + m] >= kS || filter[first + m] >= kF) atomicOr(err, 1);
         }
         uint64_t left = __ballot(valid);
         if (!left) continue;
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                 square = from[first + min(64 * p + lane, count - 1)];
                 filt = filter[first + min(64 * p + lane, count - 1)];
             }
-            if (square >= kS || filt >= kF) atomicOr(err, 8);
+            if (square >= kS || filt >= kF) atomicOr(err, 1);
             square = min(square, kS - 1u);
             list.square[64 * p + lane] = (unsigned char)(16 * (square & 3) + (square >> 2));
             list.filter[64 * p + lane] = (unsigned char)min(filt, kF - 1u);
@@ -872,7 +872,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
         if (!left) break;
       }
     }
-    if (lo < hi && hi == n && lane == 0 && start != n_moves) atomicOr(err, 8);
+    if (lo < hi && hi == n && lane == 0 && start != n_moves) atomicOr(err, 1);
     if (WANT & kKernelGrad) {
         __syncthreads();
         store_part(dw, first_wave, move_wave_bytes<T>(WANT), wave, waves, col, q, dw_part + (size_t)blockIdx.x * kXW,

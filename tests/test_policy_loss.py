@@ -271,7 +271,13 @@ def test_lists_of_every_length(ctx, dtype):
 @pytest.mark.parametrize("n", [1023, 1024, 1025, 4095, 4096, 4097, 9000])
 def test_list_starts(ctx, n):
     """Boards at the borders of whatever the prefix sum of the list lengths is cut into."""
-    check_all(ctx, make(n, torch.float32, seed=n, moves=True, longest=3))
+    case = make(n, torch.float32, seed=n, moves=True, longest=3)
+    want = check_all(ctx, case)
+    d = on_gpu(case)
+    odd = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
+    odd[5:5 + n] = d["lists"][2]
+    d["lists"] = d["lists"][:2] + (odd[5:5 + n],)
+    assert all(torch.equal(a, b) for a, b in zip(call(ctx, d), want))
 
 
 @gpu
@@ -334,6 +340,10 @@ def test_layouts_and_weights(ctx, moves):
     room = torch.empty(d["x"].numel() + 3, dtype=torch.bfloat16, device="cuda")
     room[3:] = d["x"].flatten()
     other["x"], other["k"] = room[3:].view_as(d["x"]), d["k"].t().contiguous().t()
+    for i, a in enumerate(d["lists"]):           # bytes that start anywhere
+        odd = torch.empty(a.numel() + 16, dtype=torch.uint8, device="cuda")
+        odd[3 + 2 * i:][:a.numel()] = a
+        other["lists"] = other["lists"][:i] + (odd[3 + 2 * i:][:a.numel()],) + other["lists"][i + 1:]
     assert all(torch.equal(a, b) for a, b in zip(call(ctx, other), want))
     d["w"] = torch.tensor([0.25], device="cuda")
     want = call(ctx, d)
@@ -438,6 +448,30 @@ def test_out_of_range_inputs_are_reported_once(ctx):
 
 
 @gpu
+def test_a_loss_flag_does_not_reach_a_prediction(ctx):
+    """Out-of-range inputs of a loss are bf_policy_check's to report, not the next move prediction's on the context."""
+    from batch_first_amd import chestimator, ops, positions, weights
+    pred, start, closer = chestimator.get_inference_functions(weights.make_weights(seed=7), policy_weights=weights.make_policy_weights(seed=1))
+    try:
+        from batch_first_amd.encoder import struct_array_to_ann_inputs
+        structs = positions.test_set(4, seed=1)
+        nib, occ = struct_array_to_ann_inputs(structs, structs[:0], np.ones(4, bool), np.zeros(0, bool), 4)
+        moves = [np.array([1, 2, 3, 4], np.uint8), np.array([5, 6, 7, 8], np.uint8), np.ones(4, np.uint8)]
+        want = start(nib, occ)(moves)
+        handle = pred._handle()
+        ops._torch.bf_torch_context(handle, 0)
+        d = on_gpu(make(2, torch.float32))
+        torch.ops.batchfirst.policy_loss(handle.value, d["x"], d["k"], torch.tensor([9999, 0], device="cuda"))
+        torch.cuda.synchronize()
+        assert np.array_equal(start(nib, occ)(moves), want)
+        assert _lib.load().bf_policy_check(handle, None) == _lib.BF_E_FORMAT and b"loss input" in _lib.load().bf_last_error()
+        assert _lib.load().bf_policy_check(handle, None) == 0
+        ops._torch.bf_torch_context(handle, -1)
+    finally:
+        closer()
+
+
+@gpu
 def test_ops_refuse(ctx):
     o = torch.ops.batchfirst
     x, k, t = torch.zeros(2, 32, 8, 8, device="cuda"), torch.zeros(32, 73, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
@@ -504,6 +538,72 @@ def test_streams_of_their_own(ctx):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@gpu
+def test_unlisted_squares_may_hold_anything(ctx):
+    """NaN and infinities in squares from which no move is listed change nothing but their own gradient's place: zero."""
+    for dtype in TYPES:
+        case = make(6, dtype, seed=13, moves=True, longest=20)
+        sq, fl, per = case["moves"]
+        sq[:] = sq % 32                          # squares 32 ... 63 of every board
+        case["t"] = torch.from_numpy(np.where(per > 0, 0, -1).astype(np.int64))
+        case["x"].view(6, 32, 64)[:, :, 32:] = 0
+        clean = check_all(ctx, case)
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            case["x"].view(6, 32, 64)[:, 5:9, 40:50] = bad
+            d = on_gpu(case)
+            got = call(ctx, d)
+            assert all(torch.equal(a, b) for a, b in zip(got, clean)), (dtype, bad)
+            assert torch.equal(forward(ctx, d), clean[0])
+
+
+@gpu
+def test_features_of_every_magnitude(ctx):
+    """float32 features whose scale differs from board to board by 2^200, which no float16 term could hold unscaled."""
+    rng = np.random.default_rng(1)
+    case = make(40, torch.float32, seed=21)
+    scale = torch.from_numpy(2.0 ** rng.integers(-100, 3, 40)).float()
+    case["x"] = case["x"] * scale[:, None, None, None]
+    case["t"] = torch.from_numpy(rng.integers(0, 4672, 40))
+    check_all(ctx, case)
+    # and of a kernel that makes up for it
+    case = make(20, torch.float32, seed=22, moves=True)
+    case["x"], case["k"] = case["x"] * 2.0 ** 60, case["k"] * 2.0 ** -60
+    check_all(ctx, case)
+    case["x"], case["k"] = case["x"] * 2.0 ** -120, case["k"] * 2.0 ** 120
+    check_all(ctx, case)
+
+
+@gpu
+def test_a_board_that_is_almost_certain(ctx):
+    """The target's probability within 1e-5 of one: the others' gradients keep their precision."""
+    for moves in (False, True):
+        for dtype in TYPES:
+            case = make(8, dtype, seed=31, moves=moves)
+            if moves:
+                case["t"] = torch.zeros(8, dtype=torch.int64)
+                sq, fl, per = case["moves"]
+                per[:] = np.maximum(per, 2)
+                m = int(per.sum())
+                rng = np.random.default_rng(5)
+                sq, fl = rng.integers(0, 64, m).astype(np.uint8), rng.integers(1, 73, m).astype(np.uint8)
+                first = np.cumsum(per.astype(int)) - per
+                sq[first], fl[first] = np.arange(8), 0
+                case["moves"] = sq, fl, per
+                at = [(b, b, 0) for b in range(8)]
+            else:
+                case["t"] = torch.tensor([64 * 0 + 3 * b for b in range(8)])
+                at = [(b, 3 * b, 0) for b in range(8)]
+            x, k = case["x"].view(8, 32, 64).float(), case["k"].float()
+            k[0], k[0, 0] = 0.0, 4.0
+            x[:, 0] = 0.0
+            for b, s, f in at:
+                x[b, 0, s] = 7.0                 # + 28 for the target's logit alone (filter 0, its square)
+            case["x"], case["k"] = x.view(8, 32, 8, 8).to(dtype), k.to(dtype)
+            ref = reference(case)
+            assert ref["loss"].max() < 1e-5
+            check_all(ctx, case)
 
 
 @gpu
