@@ -21,7 +21,9 @@ constexpr int kThreads = 256;
 constexpr int kInFlight = 4;                                        // 16-byte accesses a thread and chunk
 constexpr size_t kChunkBytes = (size_t)kThreads * kInFlight * 16;
 constexpr int kTable = 160;        // tensors a launch: their table travels in the kernel's arguments, of which there are 4 KB
-constexpr unsigned kGroups = 2048; // workgroups a launch: eight a compute unit
+// Workgroups a launch, four a compute unit: eight leave every workgroup of the scaling pass more partial sums to add up
+// (150 M float32 elements clipped in 348 in place of 334 us), two keep fewer loads in flight.
+constexpr unsigned kGroups = 1024;
 constexpr int kTypeShift = 56;
 
 struct Table {
@@ -110,6 +112,7 @@ __device__ __forceinline__ double block_sum(double v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
+    static_assert(kThreads == 256, "four waves");
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
