@@ -6,7 +6,8 @@
 // Bound by reading (and, to scale, reading again and writing): a workgroup walks a run of 16 KB chunks, through however
 // many tensors it spans, with 16-byte accesses and four of them in flight a thread, and leaves one partial sum; every
 // workgroup of the scaling pass adds the partial sums up by itself, in the same fixed order, which spares a launch between the two.
-// The scaling pass walks its run backwards, so that it begins with what the first pass has left in the caches.
+// The scaling pass walks its run backwards, so that it begins with what the first pass has left in the caches (100 M float32
+// elements clipped in 208 us; forwards 253).  A few chunks, as a head's own gradient, take one workgroup and one launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -56,14 +57,14 @@ __device__ __forceinline__ double square(T v) {
     return d * d;
 }
 
-// Pieces [at, at + kThreads * kInFlight) of a tensor: whole(i, piece) for those inside it, part(element) for the
-// elements of those that its ends cut.
+// One chunk of a tensor by kThreads threads: whole(where, piece) for the pieces inside it, part(element) for the elements
+// of those that its ends cut.
 template <typename T, typename Whole, typename Part>
 __device__ __forceinline__ void chunk_of(char* p, unsigned long long count, unsigned chunk, Whole&& whole, Part&& part) {
     typedef T piece_t __attribute__((ext_vector_type(16 / sizeof(T))));
     constexpr int kPer = Pieces<T>::kPer;
     const Pieces<T> t(p, count);
-    const long long at = (long long)chunk * (kThreads * kInFlight) + threadIdx.x;
+    const long long at = (long long)chunk * (kThreads * kInFlight) + threadIdx.x % kThreads;
     piece_t v[kInFlight];
     bool in[kInFlight];
 #pragma unroll
@@ -105,15 +106,40 @@ __device__ __forceinline__ void scale(char* p, unsigned long long count, unsigne
                 [&](T* e) { *e = (T)((float)*e * f); });
 }
 
-// The workgroup's sum, the same in every thread.
+// Chunk c of the table, which belongs to tensor k.
+__device__ __forceinline__ double squares_of(const Table& t, int k, unsigned c) {
+    const unsigned long long count = t.count[k] & ((1ull << kTypeShift) - 1);
+    const int type = (int)(t.count[k] >> kTypeShift);
+    if (type == BF_TYPE_F32) return squares<float>(t.ptr[k], count, c - t.first[k]);
+    if (type == BF_TYPE_BF16) return squares<__bf16>(t.ptr[k], count, c - t.first[k]);
+    return squares<_Float16>(t.ptr[k], count, c - t.first[k]);
+}
+__device__ __forceinline__ void scale_of(const Table& t, int k, unsigned c, float f) {
+    const unsigned long long count = t.count[k] & ((1ull << kTypeShift) - 1);
+    const int type = (int)(t.count[k] >> kTypeShift);
+    if (type == BF_TYPE_F32) scale<float>(t.ptr[k], count, c - t.first[k], f);
+    else if (type == BF_TYPE_BF16) scale<__bf16>(t.ptr[k], count, c - t.first[k], f);
+    else scale<_Float16>(t.ptr[k], count, c - t.first[k], f);
+}
+
+// The sum over the workgroup's WAVES waves, the same in every thread.
+template <int WAVES>
 __device__ __forceinline__ double block_sum(double v) {
-    __shared__ double red[kThreads / 64];
+    __shared__ double red[WAVES];
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    static_assert(kThreads == 256, "four waves");
-    return (red[0] + red[1]) + (red[2] + red[3]);
+    double a = red[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) a += red[i];
+    return a;
+}
+
+// min(1, limit / (norm + 1e-6)): a norm of NaN gives a factor of NaN, one of infinity a factor of 0, as the formula has it
+__device__ __forceinline__ float factor(float norm, float limit) {
+    const float f = limit / (norm + 1e-6f);
+    return f >= 1.0f ? 1.0f : f;
 }
 
 // The tensor that a chunk belongs to.
@@ -139,20 +165,16 @@ __global__ __launch_bounds__(kThreads) void k_squares(Table t, double* __restric
     int k = find(t, lo);
     for (unsigned c = lo; c < hi; ++c) {
         while (c >= t.first[k + 1]) ++k;
-        const unsigned long long count = t.count[k] & ((1ull << kTypeShift) - 1);
-        const int type = (int)(t.count[k] >> kTypeShift);
-        if (type == BF_TYPE_F32) a += squares<float>(t.ptr[k], count, c - t.first[k]);
-        else if (type == BF_TYPE_BF16) a += squares<__bf16>(t.ptr[k], count, c - t.first[k]);
-        else a += squares<_Float16>(t.ptr[k], count, c - t.first[k]);
+        a += squares_of(t, k, c);
     }
-    a = block_sum(a);
+    a = block_sum<kThreads / 64>(a);
     if (threadIdx.x == 0) part[blockIdx.x] = a;
 }
 
 __device__ __forceinline__ float norm_of(const double* __restrict__ part, unsigned parts) {
     double a = 0.0;
     for (unsigned i = threadIdx.x; i < parts; i += kThreads) a += part[i];
-    return (float)sqrt(block_sum(a));
+    return (float)sqrt(block_sum<kThreads / 64>(a));
 }
 
 __global__ __launch_bounds__(kThreads) void k_norm(const double* __restrict__ part, unsigned parts, float* __restrict__ norm) {
@@ -164,21 +186,32 @@ __global__ __launch_bounds__(kThreads) void k_scale(Table t, const double* __res
                                                     float* __restrict__ norm) {
     const float v = norm_of(part, parts);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
-    // a norm of NaN gives a factor of NaN, one of infinity a factor of 0, as the formula has it
-    const float f = limit / (v + 1e-6f);
-    if (f >= 1.0f) return;   // within the limit: every product would be the value itself
+    const float f = factor(v, limit);
+    if (f == 1.0f) return;   // within the limit: every product would be the value itself
     unsigned lo, hi;
     run_of(t, lo, hi);
     if (lo == hi) return;
     int k = find(t, hi - 1);
     for (unsigned c = hi; c-- > lo;) {
         while (c < t.first[k]) --k;
-        const unsigned long long count = t.count[k] & ((1ull << kTypeShift) - 1);
-        const int type = (int)(t.count[k] >> kTypeShift);
-        if (type == BF_TYPE_F32) scale<float>(t.ptr[k], count, c - t.first[k], f);
-        else if (type == BF_TYPE_BF16) scale<__bf16>(t.ptr[k], count, c - t.first[k], f);
-        else scale<_Float16>(t.ptr[k], count, c - t.first[k], f);
+        scale_of(t, k, c, f);
     }
+}
+
+// Both passes over a few chunks by one workgroup, four chunks at a time: 2.9 us on the GPU and 6.7 a call where the two
+// launches take 4.1 and 10.8, as long on the GPU (4.9 us) at twelve chunks, longer from there on.
+constexpr int kSmallThreads = 1024;
+constexpr unsigned kSmallChunks = 12;
+__global__ __launch_bounds__(kSmallThreads) void k_small(Table t, bool clip, float limit, float* __restrict__ norm) {
+    constexpr unsigned kAtOnce = kSmallThreads / kThreads;
+    const unsigned chunks = t.first[t.n], mine = threadIdx.x / kThreads;
+    double a = 0.0;
+    for (unsigned c = mine; c < chunks; c += kAtOnce) a += squares_of(t, find(t, c), c);
+    const float v = (float)sqrt(block_sum<kSmallThreads / 64>(a));
+    if (threadIdx.x == 0) *norm = v;
+    const float f = clip ? factor(v, limit) : 1.0f;
+    if (f == 1.0f) return;
+    for (unsigned c = mine; c < chunks; c += kAtOnce) scale_of(t, find(t, c), c, f);
 }
 
 size_t chunks_of(const void* ptr, size_t count, int type) {
@@ -214,6 +247,15 @@ size_t grad_norm_workspace(size_t n_tensors) { return std::max<size_t>((n_tensor
 
 hipError_t launch_grad_norm(void* const* ptrs, const size_t* counts, const int* types, size_t n_tensors, bool clip, float limit,
                             float* d_norm, void* workspace, hipStream_t s) {
+    size_t chunks = 0, filled = 0;
+    for (size_t i = 0; i < n_tensors; ++i)
+        if (counts[i]) chunks += chunks_of(ptrs[i], counts[i], types[i]), ++filled;
+    if (chunks <= kSmallChunks && filled) {      // no more tensors than chunks
+        static_assert(kSmallChunks <= kTable, "one table");
+        return tables(ptrs, counts, types, n_tensors, [&](const Table& t, unsigned) {
+            hipLaunchKernelGGL(k_small, dim3(1), dim3(kSmallThreads), 0, s, t, clip, limit, d_norm);
+        });
+    }
     double* part = static_cast<double*>(workspace);
     unsigned parts = 0;
     hipError_t e = tables(ptrs, counts, types, n_tensors, [&](const Table& t, unsigned groups) {

@@ -110,18 +110,25 @@ def clip_and_check(ctx, tensors, limit):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
-@pytest.mark.parametrize("n", [1, 2, 7, 8, 255, 2336, 4097, 65535, 65537, 200003, 1 << 20, 3000001])
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 255, 2336, 4097, 32768, 49151, 49152, 49153, 65535, 65537, 98305, 200003, 1 << 20, 3000001])
 def test_one_tensor(ctx, n, dtype):
     clip_and_check(ctx, [randn(n, dtype, n)], 0.3 * n ** 0.5)
 
 
 @gpu
-@pytest.mark.parametrize("count", [2, 27, 159, 160, 161, 321, 1000])
+@pytest.mark.parametrize("count", [2, 5, 11, 12, 13, 14, 27, 159, 160, 161, 321, 1000])
 def test_many_tensors_of_mixed_types_and_sizes(ctx, count):
     rng = np.random.default_rng(count)
     tensors = [randn(int(k), TYPES[i % 3], i, 0.1) for i, k in enumerate(np.exp(rng.uniform(0, 10, count)).astype(int))]
     tensors[1] = torch.empty(0, device="cuda")
     clip_and_check(ctx, tensors, 0.7)
+
+
+@gpu
+@pytest.mark.parametrize("count", [2, 3, 4, 11, 12, 13])
+def test_few_small_tensors(ctx, count):
+    """As many as one workgroup takes, and one more."""
+    clip_and_check(ctx, [randn(700 + 31 * i, TYPES[i % 3], i, 0.1) for i in range(count)], 0.7)
 
 
 @gpu
