@@ -120,7 +120,8 @@ __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0
 constexpr int kTiles = 5;                        // of 16 filters
 constexpr int kRow = 40;                         // 16-bit elements of a row of 32 in LDS: 16 rows start in 16 different bank groups
 constexpr int kTerm = kS * kRow;                 // elements of 64 rows
-constexpr int kPartBytes = 64 * 40 * 4;          // a wave's kernel gradient in LDS, when its boards are done
+constexpr int kPart = kC * 16 * kTiles;          // elements of a part of the kernel's gradient: [32][80], 73 of 80 in use
+constexpr int kPartBytes = kPart * 4;            // a wave's in LDS, when its boards are done
 constexpr int kStageBytes = kXW * 4;             // the kernel on its way to its operands
 
 // A board's features: a lane holds channels 8 q ... 8 q + 7 of squares 4 col ... 4 col + 3 and turns them into operands
@@ -212,7 +213,7 @@ __device__ __forceinline__ void store_features_grad(T* board, int col, int q, co
 }
 
 // The workgroup's part of the kernel's gradient: dw[a][t] of every wave, rows channel 16 a + 4 q + r, columns the filters
-// that filter_of(t, col) says; `mine` and `stride` bytes further on the other waves' LDS.
+// that filter_of(t, col) says; the waves' LDS lies `stride` bytes apart.
 template <typename F>
 __device__ __forceinline__ void store_part(const f32x4 (&dw)[2][kTiles], unsigned char* first, int stride, int wave, int waves, int col, int q,
                                            float* __restrict__ part, F&& filter_of) {
@@ -223,10 +224,11 @@ __device__ __forceinline__ void store_part(const f32x4 (&dw)[2][kTiles], unsigne
         mine[(16 * a + 4 * q + r) * (16 * kTiles) + filter_of(t, col)] = dw[a][t][r];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kXW; i += blockDim.x) {
-        float a = 0.0f;
-        for (int k = 0; k < waves; ++k) a += reinterpret_cast<const float*>(first + k * stride)[i / kF * (16 * kTiles) + i % kF];
-        part[i] = a;
+    for (int i = threadIdx.x; i < kPart / 4; i += blockDim.x) {
+        f32x4 a = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int k = 0; k < waves; ++k) a += reinterpret_cast<const f32x4*>(first + k * stride)[i];
+        reinterpret_cast<f32x4*>(part)[i] = a;
     }
 }
 
@@ -293,8 +295,8 @@ enum { kFeaturesGrad = 1, kKernelGrad = 2 };
 
 template <typename T>
 struct HeadLds {                                 // the kernel as operands, 16 bytes a lane
-    u32x4 logit[kTiles][Arith<T>::kTerms][64];   // rows filter, k channel
-    u32x4 back[3][2][Arith<T>::kTerms][64];      // rows channel, k filter as the logits' results hold them
+    // five for the logits: rows filter, k channel; 2 u + a: rows channel, k filter as the logits' results hold them
+    u32x4 operand[kTiles + 6][Arith<T>::kTerms][64];
     float red[8];
 };
 constexpr int kWaveLds = 2 * kTerm * 2;          // bytes a wave: the crossing
@@ -336,29 +338,28 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
         float w_scale;
         float* stage = reinterpret_cast<float*>(smem + sizeof(HeadLds<T>));
         stage_head<T>(w, stage, lds.red, w_scale, w_back);
-        for (int i = threadIdx.x; i < kTiles * 64; i += blockDim.x) {
-            const int f = (i >> 6) * 16 + (i & 15);
-            float v[8];
+        // an operand a wave at a time: five for the logits, six for the way back; all of a wave's are read at once
+        constexpr int kOperands = kTiles + (WANT & kFeaturesGrad ? 6 : 0), kRounds = (kOperands + 3) / 4;
+        float v[kRounds][8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = f < kF ? stage[(8 * (i >> 4 & 3) + k) * kF + f] : 0.0f;
-            u32x4 out[NT];
-            operand<T>(v, w_scale, out);
+        for (int r = 0; r < kRounds; ++r) {
+            const int i = wave + r * waves, j = i - kTiles;
 #pragma unroll
-            for (int k = 0; k < NT; ++k) lds.logit[i >> 6][k][i & 63] = out[k];
-        }
-        if (WANT & kFeaturesGrad)
-            for (int i = threadIdx.x; i < 6 * 64; i += blockDim.x) {
-                float v[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int f = 32 * (i >> 7) + 16 * (k >> 2) + 4 * (i >> 4 & 3) + (k & 3);
-                    v[k] = f < kF ? stage[(16 * (i >> 6 & 1) + (i & 15)) * kF + f] : 0.0f;
-                }
-                u32x4 out[NT];
-                operand<T>(v, w_scale, out);
-#pragma unroll
-                for (int k = 0; k < NT; ++k) lds.back[i >> 7][i >> 6 & 1][k][i & 63] = out[k];
+            for (int k = 0; k < 8; ++k) {
+                const int c = i < kTiles ? 8 * q + k : 16 * (j & 1) + col;
+                const int f = i < kTiles ? 16 * i + col : 32 * (j >> 1) + 16 * (k >> 2) + 4 * q + (k & 3);
+                v[r][k] = i < kOperands && f < kF ? stage[c * kF + f] : 0.0f;
             }
+        }
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const int i = wave + r * waves;
+            u32x4 out[NT];
+            operand<T>(v[r], w_scale, out);
+            if (i < kOperands)
+#pragma unroll
+                for (int k = 0; k < NT; ++k) lds.operand[i][k][lane] = out[k];
+        }
         __syncthreads();
     }
 
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
         for (int t = 0; t < kTiles; ++t) {
             u32x4 a[NT];
 #pragma unroll
-            for (int k = 0; k < NT; ++k) a[k] = lds.logit[t][k][lane];
+            for (int k = 0; k < NT; ++k) a[k] = lds.operand[t][k][lane];
             f32x4 l[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
             products<T, NT, NT>(l, [&](int, int k) { return a[k]; }, [&](int j, int k) { return xc[j][k]; });
 #pragma unroll
@@ -506,7 +507,7 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
             if (WANT & kFeaturesGrad) {
                 u32x4 wk[2][NT];
 #pragma unroll
-                for (int i = 0; i < 2 * NT; ++i) wk[i / NT][i % NT] = lds.back[u][i / NT][i % NT][lane];
+                for (int i = 0; i < 2 * NT; ++i) wk[i / NT][i % NT] = lds.operand[kTiles + 2 * u + i / NT][i % NT][lane];
                 products<T, NT, 2>(g, [&](int i, int k) { return wk[i >> 2][k]; }, [&](int i, int k) { return d[i & 3][k]; });
             }
             if (WANT & kKernelGrad) {
@@ -538,7 +539,7 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
       }
     }
     if (WANT & kKernelGrad)
-        store_part(dw, smem + sizeof(HeadLds<T>), kWaveLds, wave, waves, col, q, dw_part + (size_t)blockIdx.x * kXW, [](int t, int col) {
+        store_part(dw, smem + sizeof(HeadLds<T>), kWaveLds, wave, waves, col, q, dw_part + (size_t)blockIdx.x * kPart, [](int t, int col) {
             // column c of a pair of tiles is filter 16 (c >> 2 & 1) + 4 (c >> 3) + (c & 3) of the pair's 32
             const int c = 16 * (t & 1) + col;
             return t == 4 ? 64 + col : 32 * (t >> 1) + 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
@@ -875,7 +876,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
     if (lo < hi && hi == n && lane == 0 && start != n_moves) atomicOr(err, 1);
     if (WANT & kKernelGrad) {
         __syncthreads();
-        store_part(dw, first_wave, move_wave_bytes<T>(WANT), wave, waves, col, q, dw_part + (size_t)blockIdx.x * kXW,
+        store_part(dw, first_wave, move_wave_bytes<T>(WANT), wave, waves, col, q, dw_part + (size_t)blockIdx.x * kPart,
                    [](int t, int col) { return 16 * t + col; });
     }
 }
@@ -891,16 +892,17 @@ __global__ __launch_bounds__(1024) void k_sum_parts(const float* __restrict__ pa
 #pragma unroll
     for (unsigned k = 0; k < kGroups / 32; ++k) {
         const unsigned p = j + 32 * k;
-        a += p < parts ? part[(size_t)p * kXW + blockIdx.x * 32 + i] : 0.0f;
+        a += p < parts ? part[(size_t)p * kPart + blockIdx.x * 32 + i] : 0.0f;
     }
     sums[i][j] = a;
     __syncthreads();
     a = sums[j][i];
 #pragma unroll
     for (int o = 16; o; o >>= 1) a += __shfl_xor(a, o);
-    if (i == 0) dw[blockIdx.x * 32 + j] = (T)(float)a;
+    const int e = blockIdx.x * 32 + j, c = e / (16 * kTiles), f = e % (16 * kTiles);
+    if (i == 0 && f < kF) dw[c * kF + f] = (T)(float)a;
 }
-static_assert(kXW % 32 == 0, "k_sum_parts needs no bounds check");
+static_assert(kPart % 32 == 0, "k_sum_parts needs no bounds check");
 
 template <typename T, int WANT>
 hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
@@ -924,7 +926,7 @@ hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
                            sizeof(HeadLds<T>) + std::max(WANT & kKernelGrad ? waves * kWaveLds : 0u, (unsigned)kStageBytes), s, x, w,
                            a.n, a.targets, a.weights, step, a.loss, dx, part, a.err);
     if (hipError_t e = hipGetLastError()) return e;
-    if (WANT & kKernelGrad) hipLaunchKernelGGL(k_sum_parts<T>, dim3(kXW / 32), dim3(1024), 0, s, part, grid, static_cast<T*>(a.d_kernel));
+    if (WANT & kKernelGrad) hipLaunchKernelGGL(k_sum_parts<T>, dim3(kPart / 32), dim3(1024), 0, s, part, grid, static_cast<T*>(a.d_kernel));
     return hipGetLastError();
 }
 
@@ -936,7 +938,7 @@ hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
 
 }  // namespace
 
-size_t policy_loss_workspace(size_t n) { return std::min<size_t>(n, kGroups) * kXW * sizeof(float); }
+size_t policy_loss_workspace(size_t n) { return std::min<size_t>(n, kGroups) * kPartBytes; }
 
 hipError_t launch_policy_loss(const PolicyLossArgs& a, hipStream_t stream) {
     if (a.type == BF_TYPE_F32) return launch<float>(a, stream);
