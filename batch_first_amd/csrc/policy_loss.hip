@@ -343,12 +343,13 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
         float v[kRounds][8];
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
-            const int i = wave + r * waves, j = i - kTiles;
+            const int i = min(wave + r * waves, kOperands - 1), j = i - kTiles;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const int c = i < kTiles ? 8 * q + k : 16 * (j & 1) + col;
                 const int f = i < kTiles ? 16 * i + col : 32 * (j >> 1) + 16 * (k >> 2) + 4 * q + (k & 3);
-                v[r][k] = i < kOperands && f < kF ? stage[c * kF + f] : 0.0f;
+                const float e = stage[c * kF + min(f, kF - 1)];
+                v[r][k] = f < kF ? e : 0.0f;
             }
         }
 #pragma unroll
