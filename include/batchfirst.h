@@ -296,8 +296,8 @@ int bf_multi_policy_finish_host(bf_multi* m, const uint8_t* h_from_square, const
  * both of one type (BF_TYPE_*).  The logits of a board's move vocabulary (index = move_filter * 64 + from_square) are
  * l[filter][square] = sum over channels of kernel[channel][filter] * features[channel][square]; they are never written
  * out.  Logits, softmax sums and the sums of the gradients are float32 or wider; a gradient has its input's type.
- * All pointers but bf_global_norm's and bf_clip_grad_norm's tables are device pointers on the context's GPU.  Tensors
- * and workspaces need 16-byte alignment.  The calls allocate nothing, read nothing back, enqueue kernels only (so they
+ * All pointers but bf_global_norm's and bf_clip_grad_norm's tables are device pointers on the context's GPU.  Features,
+ * kernels, their gradients and workspaces need 16-byte alignment, the rest that of their elements; outputs overlap nothing.  The calls allocate nothing, read nothing back, enqueue kernels only (so they
  * can be captured into a graph) and give the same bits for the same inputs.  A workspace belongs to one call at a time:
  * calls that may overlap, or graphs whose replays may, need one each. */
 enum { BF_TYPE_F32 = 0, BF_TYPE_BF16 = 1, BF_TYPE_F16 = 2 };
