@@ -21,30 +21,17 @@ namespace bf {
 namespace {
 
 constexpr int kC = 32, kS = 64, kF = 73, kVocab = kF * kS, kXW = kC * kF;
-// ---- the whole vocabulary --------------------------------------------------------------------------------------------
+
+// ---- arithmetic, and what both losses share --------------------------------------------------------------------------
 //
-// One wave a board, everything between the features and the gradients in its registers, on 16x16x32 MFMAs with float32
-// sums.  Lane l = (n = l & 15, q = l >> 4) of an operand holds eight k (8 q ... 8 q + 7) of row or column n, of a result
-// the rows 4 q ... 4 q + 3 of column n.
-//
-//   logits   rows filter (five tiles of 16, 73 padded to 80), columns square, k channel.  Column n of tile j is square
-//            4 n + j, so that a lane's features are four neighbours in memory.
-//   dX       rows channel, columns square, k filter.  k is numbered so that a lane's eight are the filters whose logits
-//            it holds already: the probabilities become an operand where they are.
-//   dW       rows channel, columns filter, k square: features and probabilities are written to LDS a square's channels
-//            or filters at a time, as they lie in the lanes, and read transposed (32 filters at a time); the sums stay
-//            in registers over all the wave's boards.
+// 16x16x32 MFMAs with float32 sums.  Lane l = (col = l & 15, q = l >> 4) of an operand holds eight k (8 q ... 8 q + 7) of row or
+// column col, of a result the rows 4 q ... 4 q + 3 of column col.
 //
 // float32 operands travel as two float16 terms (22 bits), scaled by a power of two, the kernel's by its largest element
 // and the features' by the board's, so that the larger term stays normal down to 2^-27 of the largest; of the four
-// products of terms the least is left out (2^-22).  bfloat16 and float16 operands are exact as they are.  The logits' gradients d (before the
-// weight) travel as two terms: bfloat16 ones for bfloat16 features, else float16 ones, scaled like the features.  Their
-// largest is the target's, which is the negative sum of all the others.
-//
-// Loss and both gradients of 65 536 float32 boards: 267 to 280 us, 3.9 TB/s of features and gradients (a copy reaches
-// 4.75; float32 MFMAs alone would take 384); of 32 768 bfloat16 boards 95 us.  Bound by issue: of a board's 5 600 cycles a
-// SIMD the 765 (bfloat16; float32 880) vector instructions take 3 400 and the 108 (192) MFMAs 1 700 (3 100), with two
-// waves of 220 to 254 registers a SIMD to overlap them.  The loss alone reads 65 536 float32 boards in 119 us, 4.5 TB/s.
+// products of terms the least is left out (2^-22).  bfloat16 and float16 operands are exact as they are.  The logits'
+// gradients d (before the weight) travel as two terms: bfloat16 ones for bfloat16 features, else float16 ones, scaled like
+// the features.  Their largest is the target's, which is the negative sum of all the others.
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -70,7 +57,7 @@ struct Arith {                                   // float32 and float16 features
         asm("" : "+v"(hi));                      // one rounding for both uses: a product a may be contracted into either
         const half2v h = __builtin_bit_cast(half2v, hi);
         float ra = a - (float)h[0], rb = b - (float)h[1];
-        asm("" : "+v"(ra));                      // packed together: fused with the subtraction, their rounding takes 1 % of the call longer
+        asm("" : "+v"(ra));                      // packed together: rounded in the subtraction they cost 1 % of the call
         asm("" : "+v"(rb));
         lo = __builtin_bit_cast(unsigned, half2v{(_Float16)ra, (_Float16)rb});
     }
@@ -178,7 +165,8 @@ struct Features {
             for (int k = 0; k < kTerms; ++k)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    column[j][k][i] = __builtin_amdgcn_perm(rows[k][2 * i + 1][j >> 1], rows[k][2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+                    column[j][k][i] = __builtin_amdgcn_perm(rows[k][2 * i + 1][j >> 1], rows[k][2 * i][j >> 1],
+                                                            j & 1 ? 0x07060302u : 0x05040100u);
     }
 };
 
@@ -223,8 +211,8 @@ __device__ __forceinline__ void store_features_grad(T* board, int col, int q, co
 // The workgroup's part of the kernel's gradient: dw[a][t] of every wave, rows channel 16 a + 4 q + r, columns the filters
 // that filter_of(t, col) says; the waves' LDS lies `stride` bytes apart.
 template <typename F>
-__device__ __forceinline__ void store_part(const f32x4 (&dw)[2][kTiles], unsigned char* first, int stride, int wave, int waves, int col, int q,
-                                           float* __restrict__ part, F&& filter_of) {
+__device__ __forceinline__ void store_part(const f32x4 (&dw)[2][kTiles], unsigned char* first, int stride, int wave, int waves,
+                                           int col, int q, float* __restrict__ part, F&& filter_of) {
     float* mine = reinterpret_cast<float*>(first + wave * stride);
 #pragma unroll
     for (int i = 0; i < 8 * kTiles; ++i) {
@@ -300,6 +288,23 @@ __device__ __forceinline__ void products(f32x4 (&c)[N], A&& a, B&& b) {
 
 // What a call asks for beside the loss.
 enum { kFeaturesGrad = 1, kKernelGrad = 2 };
+
+// ---- the whole vocabulary --------------------------------------------------------------------------------------------
+//
+// One wave a board, everything between the features and the gradients in its registers.
+//
+//   logits   rows filter (five tiles of 16, 73 padded to 80), columns square, k channel.  Column col of tile j is square
+//            4 col + j, so that a lane's features are four neighbours in memory.
+//   dX       rows channel, columns square, k filter.  k is numbered so that a lane's eight are the filters whose logits
+//            it holds already: the probabilities become an operand where they are.
+//   dW       rows channel, columns filter, k square: features and probabilities are written to LDS a square's channels
+//            or filters at a time, as they lie in the lanes, and read transposed (32 filters at a time); the sums stay
+//            in registers over all the wave's boards.
+//
+// Loss and both gradients of 65 536 float32 boards: 267 to 280 us, 3.9 TB/s of features and gradients (a copy reaches
+// 4.75; float32 MFMAs alone would take 384); of 32 768 bfloat16 boards 95 us.  Bound by issue: of a board's 5 600 cycles a
+// SIMD the 765 (bfloat16; float32 880) vector instructions take 3 400 and the 108 (192) MFMAs 1 700 (3 100), with two
+// waves of 220 to 254 registers a SIMD to overlap them.  The loss alone reads 65 536 float32 boards in 119 us, 4.5 TB/s.
 
 template <typename T>
 struct HeadLds {                                 // the kernel as operands, 16 bytes a lane
@@ -390,162 +395,162 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
                 zero_features_grad(dx + (base + __builtin_ctzll(left) * step) * (kC * kS), lane);
         uint64_t left = __ballot(valid);
         if (left && !(loaded && (left & 1))) features.load(x + (base + __builtin_ctzll(left) * step) * (kC * kS), col, q);
-      while (left) {
-        const int who = __builtin_ctzll(left);
-        const size_t b = base + who * step;
-        left &= left - 1;
-        const T* next = x + (base + (left ? __builtin_ctzll(left) : 0) * step) * (kC * kS);   // read ahead; after the last, in vain
-        const int target = __builtin_amdgcn_readlane(my_target, who);
+        while (left) {
+            const int who = __builtin_ctzll(left);
+            const size_t b = base + who * step;
+            left &= left - 1;
+            const T* next = x + (base + (left ? __builtin_ctzll(left) : 0) * step) * (kC * kS);   // read ahead; after the last, in vain
+            const int target = __builtin_amdgcn_readlane(my_target, who);
 
-        features.convert();
-        const u32x4 (&xc)[4][NT] = features.column;
-        const float x_back = features.back;
-        if (WANT == 0) features.load(next, col, q);
-        u32x4 xr[2][2][NT];                      // and as rows (channel, k square) for dW
-        if (WANT & kKernelGrad) {
-            write_rows<NT>(mine, col, q, xc);
-            lds_fence();
+            features.convert();
+            const u32x4 (&xc)[4][NT] = features.column;
+            const float x_back = features.back;
+            if (WANT == 0) features.load(next, col, q);
+            u32x4 xr[2][2][NT];                      // and as rows (channel, k square) for dW
+            if (WANT & kKernelGrad) {
+                write_rows<NT>(mine, col, q, xc);
+                lds_fence();
 #pragma unroll
-            for (int i = 0; i < 4 * NT; ++i) xr[i / NT >> 1][i / NT & 1][i % NT] = crossed(i % NT, i / NT & 1, i / NT >> 1);
-            lds_fence();
-        }
-
-        // logits, in units of 2^-(scales)
-        f32x16 v[kTiles];                        // [tile of filters][4 * square + row]
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            u32x4 a[NT];
-#pragma unroll
-            for (int k = 0; k < NT; ++k) a[k] = lds.operand[t][k][lane];
-            f32x4 l[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
-            products<T, NT, NT>(l, [&](int, int k) { return a[k]; }, [&](int j, int k) { return xc[j][k]; });
-#pragma unroll
-            for (int k = 0; k < 16; ++k) v[t][k] = l[k >> 2][k & 3];
-        }
-        // the padding's filters 73 ... 79
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (64 + 4 * q + r >= kF) v[kTiles - 1][4 * j + r] = -INFINITY;
-
-        // the target's place: tile, register and lane are uniform
-        const int tf = target >> 6, ts = target & 63;
-        const int t_tile = tf >> 4, t_reg = (ts & 3) * 4 + (tf & 3), t_lane = (tf >> 2 & 3) * 16 + (ts >> 2);
-        auto at_target = [&](auto&& change) {    // returns what the target's lane then holds
-            float e = 0.0f;
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-                if (t == t_tile) {
-                    e = change(v[t][t_reg]);
-                    v[t][t_reg] = e;
-                    asm volatile("" : "+v"(e));  // keeps the branch
-                }
-            return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), t_lane));
-        };
-        const float l_target = at_target([&](float e) { return e; });
-
-        float top = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int k = 0; k < 16; k += 2) top = larger(top, larger(v[t][k], v[t][k + 1]));
-        top = lanes_reduce<true>(top);
-        // exp(l - top) = 2^(l unit - top unit); an error of the rounded second product is common to all of the board
-        const float unit = fminf(fmaxf(w_back * x_back, 1e-36f), 1e38f);
-        const float unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
-        float z4[4] = {};
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                v[t][k] = __builtin_amdgcn_exp2f(fmaf(v[t][k], unit2, top2));
-                z4[k & 3] += v[t][k];
+                for (int i = 0; i < 4 * NT; ++i) xr[i / NT >> 1][i / NT & 1][i % NT] = crossed(i % NT, i / NT & 1, i / NT >> 1);
+                lds_fence();
             }
-        const float z = lanes_reduce<false>((z4[0] + z4[1]) + (z4[2] + z4[3]));
-        if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
-        if (!WANT) continue;
 
-        // the logits' gradients times z: exponentials, less z at the target.  The target's is the largest but for
-        // rounding: z's own, up to 90 * 2^-24, can make the target's smaller than another by as much, which the least
-        // scale covers.
-        const float rz = __builtin_amdgcn_rcpf(z);
-        const float d_target = at_target([&](float e) { return e - (lane == t_lane ? z : 0.0f); }) * rz;
-        float inv = 1.0f, wb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
-        if constexpr (Arith<T>::kScaled) {
-            float d_scale, d_back;
-            scale_of(fabsf(d_target), -17, d_scale, d_back);
-            inv = d_scale * rz;
-            wb *= d_back;
-        } else {
-            wb *= rz;
-        }
-
-        f32x4 g[8];                              // [4 * half of channels + square of four]
+            // logits, in units of 2^-(scales)
+            f32x16 v[kTiles];                        // [tile of filters][4 * square + row]
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = f32x4{0, 0, 0, 0};
-        const float w_scale = wb * x_back;
+            for (int t = 0; t < kTiles; ++t) {
+                u32x4 a[NT];
 #pragma unroll
-        for (int u = 0; u < 3; ++u) {
-            const int tiles = u < 2 ? 2 : 1;
-            u32x4 d[4][2];                       // [square of four][term]: eight filters
+                for (int k = 0; k < NT; ++k) a[k] = lds.operand[t][k][lane];
+                f32x4 l[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+                products<T, NT, NT>(l, [&](int, int k) { return a[k]; }, [&](int j, int k) { return xc[j][k]; });
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[t][k] = l[k >> 2][k & 3];
+            }
+            // the padding's filters 73 ... 79
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    unsigned hi = 0, lo = 0;
-                    if (i < 2 * tiles) {
-                        const f32x16& p = v[2 * u + (i >> 1)];
-                        const int k = 4 * j + 2 * (i & 1);
-                        if constexpr (Arith<T>::kScaled) Arith<T>::split(p[k] * inv, p[k + 1] * inv, hi, lo);
-                        else Arith<T>::split(p[k], p[k + 1], hi, lo);
+                for (int r = 0; r < 4; ++r)
+                    if (64 + 4 * q + r >= kF) v[kTiles - 1][4 * j + r] = -INFINITY;
+
+            // the target's place: tile, register and lane are uniform
+            const int tf = target >> 6, ts = target & 63;
+            const int t_tile = tf >> 4, t_reg = (ts & 3) * 4 + (tf & 3), t_lane = (tf >> 2 & 3) * 16 + (ts >> 2);
+            auto at_target = [&](auto&& change) {    // returns what the target's lane then holds
+                float e = 0.0f;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+                    if (t == t_tile) {
+                        e = change(v[t][t_reg]);
+                        v[t][t_reg] = e;
+                        asm volatile("" : "+v"(e));  // keeps the branch
                     }
-                    d[j][0][i] = hi;
-                    d[j][1][i] = lo;
+                return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), t_lane));
+            };
+            const float l_target = at_target([&](float e) { return e; });
+
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) top = larger(top, larger(v[t][k], v[t][k + 1]));
+            top = lanes_reduce<true>(top);
+            // exp(l - top) = 2^(l unit - top unit); an error of the rounded second product is common to all of the board
+            const float unit = fminf(fmaxf(w_back * x_back, 1e-36f), 1e38f);
+            const float unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
+            float z4[4] = {};
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    v[t][k] = __builtin_amdgcn_exp2f(fmaf(v[t][k], unit2, top2));
+                    z4[k & 3] += v[t][k];
                 }
-            if (u == 0) features.load(next, col, q);   // the first two tiles' registers are free
-            if (WANT & kKernelGrad) {
-                if (tiles == 2) write_rows<2>(mine, col, q, d);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<u32x2*>(mine + (i & 1) * kTerm + (16 * (i >> 1) + col) * kRow + 4 * q) =
-                            u32x2{d[i >> 1][i & 1][0], d[i >> 1][i & 1][1]};
-                lds_fence();
+            const float z = lanes_reduce<false>((z4[0] + z4[1]) + (z4[2] + z4[3]));
+            if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
+            if (!WANT) continue;
+
+            // the logits' gradients times z: exponentials, less z at the target.  The target's is the largest but for
+            // rounding: z's own, up to 90 * 2^-24, can make the target's smaller than another by as much, which the least
+            // scale covers.
+            const float rz = __builtin_amdgcn_rcpf(z);
+            const float d_target = at_target([&](float e) { return e - (lane == t_lane ? z : 0.0f); }) * rz;
+            float inv = 1.0f, wb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
+            if constexpr (Arith<T>::kScaled) {
+                float d_scale, d_back;
+                scale_of(fabsf(d_target), -17, d_scale, d_back);
+                inv = d_scale * rz;
+                wb *= d_back;
+            } else {
+                wb *= rz;
             }
-            if (WANT & kFeaturesGrad) {
-                u32x4 wk[2][NT];
+
+            f32x4 g[8];                              // [4 * half of channels + square of four]
 #pragma unroll
-                for (int i = 0; i < 2 * NT; ++i) wk[i / NT][i % NT] = lds.operand[kTiles + 2 * u + i / NT][i % NT][lane];
-                products<T, NT, 2>(g, [&](int i, int k) { return wk[i >> 2][k]; }, [&](int i, int k) { return d[i & 3][k]; });
-            }
-            if (WANT & kKernelGrad) {
-                auto sums = [&](auto& s) {       // [2 * tile + half of channels]
+            for (int i = 0; i < 8; ++i) g[i] = f32x4{0, 0, 0, 0};
+            const float w_scale = wb * x_back;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        u32x4 dk[2][2];
+            for (int u = 0; u < 3; ++u) {
+                const int tiles = u < 2 ? 2 : 1;
+                u32x4 d[4][2];                       // [square of four][term]: eight filters
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        unsigned hi = 0, lo = 0;
+                        if (i < 2 * tiles) {
+                            const f32x16& p = v[2 * u + (i >> 1)];
+                            const int k = 4 * j + 2 * (i & 1);
+                            if constexpr (Arith<T>::kScaled) Arith<T>::split(p[k] * inv, p[k + 1] * inv, hi, lo);
+                            else Arith<T>::split(p[k], p[k + 1], hi, lo);
+                        }
+                        d[j][0][i] = hi;
+                        d[j][1][i] = lo;
+                    }
+                if (u == 0) features.load(next, col, q);   // the first two tiles' registers are free
+                if (WANT & kKernelGrad) {
+                    if (tiles == 2) write_rows<2>(mine, col, q, d);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<u32x2*>(mine + (i & 1) * kTerm + (16 * (i >> 1) + col) * kRow + 4 * q) =
+                                u32x2{d[i >> 1][i & 1][0], d[i >> 1][i & 1][1]};
+                    lds_fence();
+                }
+                if (WANT & kFeaturesGrad) {
+                    u32x4 wk[2][NT];
+#pragma unroll
+                    for (int i = 0; i < 2 * NT; ++i) wk[i / NT][i % NT] = lds.operand[kTiles + 2 * u + i / NT][i % NT][lane];
+                    products<T, NT, 2>(g, [&](int i, int k) { return wk[i >> 2][k]; }, [&](int i, int k) { return d[i & 3][k]; });
+                }
+                if (WANT & kKernelGrad) {
+                    auto sums = [&](auto& s) {       // [2 * tile + half of channels]
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            u32x4 dk[2][2];
+#pragma unroll
+                            for (int i = 0; i < 2 * tiles; ++i)
+                                dk[i >> 1][i & 1] = crossed(i & 1, h, i >> 1);
+                            products<T, NT, 2>(s, [&](int i, int k) { return xr[i & 1][h][k]; }, [&](int i, int k) { return dk[i >> 1][k]; });
+                        }
 #pragma unroll
                         for (int i = 0; i < 2 * tiles; ++i)
-                            dk[i >> 1][i & 1] = crossed(i & 1, h, i >> 1);
-                        products<T, NT, 2>(s, [&](int i, int k) { return xr[i & 1][h][k]; }, [&](int i, int k) { return dk[i >> 1][k]; });
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) dw[i & 1][2 * u + (i >> 1)][r] = fmaf(s[i][r], w_scale, dw[i & 1][2 * u + (i >> 1)][r]);
+                    };
+                    if (tiles == 2) {
+                        f32x4 s[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+                        sums(s);
+                    } else {
+                        f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                        sums(s);
                     }
-#pragma unroll
-                    for (int i = 0; i < 2 * tiles; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) dw[i & 1][2 * u + (i >> 1)][r] = fmaf(s[i][r], w_scale, dw[i & 1][2 * u + (i >> 1)][r]);
-                };
-                if (tiles == 2) {
-                    f32x4 s[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
-                    sums(s);
-                } else {
-                    f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-                    sums(s);
+                    lds_fence();
                 }
-                lds_fence();
             }
+            if (WANT & kFeaturesGrad) store_features_grad(dx + b * (kC * kS), col, q, g, wb * w_back);
         }
-        if (WANT & kFeaturesGrad) store_features_grad(dx + b * (kC * kS), col, q, g, wb * w_back);
-      }
     }
     if (WANT & kKernelGrad)
         store_part(dw, smem + sizeof(HeadLds<T>), kWaveLds, wave, waves, col, q, dw_part + (size_t)blockIdx.x * kPart, [](int t, int col) {
@@ -720,170 +725,172 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
         };
         int who = __builtin_ctzll(left);
         fetch(who, loaded && who == 0);
-      while (true) {
-        const size_t b = base + who;
-        const int target = __builtin_amdgcn_readlane(my_target, who), count = cnt;
-        const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
-        features.convert();
-        const float x_back = features.back;
-        write_rows<NT>(rows, col, q, features.column);
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            if (64 * p >= count) continue;
-            if (p) {
-                square = from[first + min(64 * p + lane, count - 1)];
-                filt = filter[first + min(64 * p + lane, count - 1)];
-            }
-            if (square >= kS || filt >= kF) atomicOr(err, 1);
-            square = min(square, kS - 1u);
-            list.square[64 * p + lane] = (unsigned char)(16 * (square & 3) + (square >> 2));
-            list.filter[64 * p + lane] = (unsigned char)min(filt, kF - 1u);
-        }
-        left &= left - 1;
-        if (left) {
-            who = __builtin_ctzll(left);
-            fetch(who, false);
-        }
-        lds_fence();
-
-        // logits, in units of 2^-(scales)
-        for (int m = 0; m < count; m += 32) {
-            u32x4 a[2][NT], f[2][NT];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int sq = list.square[m + 16 * i + col], fl = list.filter[m + 16 * i + col];
-#pragma unroll
-                for (int k = 0; k < NT; ++k) {
-                    a[i][k] = *reinterpret_cast<const u32x4*>(rows + k * kTerm + sq * kRow + 8 * q);
-                    f[i][k] = *reinterpret_cast<const u32x4*>(&head.rows[k][fl][8 * q]);
-                }
-            }
-            f32x4 l[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            products<T, NT, NT>(l, [&](int i, int k) { return a[i][k]; }, [&](int i, int k) { return f[i][k]; });
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float even = col & 2 ? l[i][2] : l[i][0], odd = col & 2 ? l[i][3] : l[i][1];
-                if (q == col >> 2) list.logit[m + 16 * i + col] = col & 1 ? odd : even;
-            }
-        }
-        lds_fence();
-        const float l_target = list.logit[target];
-        float v[4], top = -INFINITY;             // [pass of 64 moves]
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            v[p] = -INFINITY;
-            if (64 * p >= count) continue;
-            if (64 * p + lane < count) v[p] = list.logit[64 * p + lane];
-            top = larger(top, v[p]);
-        }
-        top = lanes_reduce<true>(top);
-        const float unit = fminf(fmaxf(w_back * x_back, 1e-36f), 1e38f), unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
-        float z = 0.0f;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            if (64 * p >= count) continue;
-            v[p] = __builtin_amdgcn_exp2f(fmaf(v[p], unit2, top2));
-            z += v[p];
-        }
-        z = lanes_reduce<false>(z);
-        if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
-
-        if (WANT) {
-            // the logits' gradients times z, as over the vocabulary
-            const float rz = __builtin_amdgcn_rcpf(z), e_target = __builtin_amdgcn_exp2f(fmaf(l_target, unit2, top2));
-            float inv = 1.0f, wb = weight;
-            if constexpr (Arith<T>::kScaled) {
-                float d_scale, d_back;
-                scale_of(fabsf(e_target - z) * rz, -17, d_scale, d_back);
-                inv = d_scale * rz;
-                wb *= d_back;
-            } else {
-                wb *= rz;
-            }
+        while (true) {
+            const size_t b = base + who;
+            const int target = __builtin_amdgcn_readlane(my_target, who), count = cnt;
+            const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
+            features.convert();
+            const float x_back = features.back;
+            write_rows<NT>(rows, col, q, features.column);
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 if (64 * p >= count) continue;
-                unsigned hi, lo;
-                Arith<T>::split((v[p] - (64 * p + lane == target ? z : 0.0f)) * inv, 0.0f, hi, lo);
-                list.hi[64 * p + lane] = (unsigned short)hi;
-                list.lo[64 * p + lane] = (unsigned short)lo;
+                if (p) {
+                    square = from[first + min(64 * p + lane, count - 1)];
+                    filt = filter[first + min(64 * p + lane, count - 1)];
+                }
+                if (square >= kS || filt >= kF) atomicOr(err, 1);
+                square = min(square, kS - 1u);
+                list.square[64 * p + lane] = (unsigned char)(16 * (square & 3) + (square >> 2));
+                list.filter[64 * p + lane] = (unsigned char)min(filt, kF - 1u);
             }
-            f32x4 g[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] = f32x4{0, 0, 0, 0};
+            left &= left - 1;
+            if (left) {
+                who = __builtin_ctzll(left);
+                fetch(who, false);
+            }
+            lds_fence();
+
+            // logits, in units of 2^-(scales)
             for (int m = 0; m < count; m += 32) {
-                {                                // pair `col`, tile q
-                    const unsigned s2 = *reinterpret_cast<const unsigned short*>(&list.square[m + 2 * col]);
-                    const unsigned f2 = *reinterpret_cast<const unsigned short*>(&list.filter[m + 2 * col]);
-                    list.square_tile[q][col] = halves((s2 >> 4 & 15) == (unsigned)q, s2 >> 12 == (unsigned)q);
-                    list.filter_tile[q][col] = halves((f2 >> 4 & 15) == (unsigned)q, f2 >> 12 == (unsigned)q);
-                    if (q == 0) list.filter_tile[4][col] = halves((f2 >> 4 & 15) == 4, f2 >> 12 == 4);
+                u32x4 a[2][NT], f[2][NT];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int sq = list.square[m + 16 * i + col], fl = list.filter[m + 16 * i + col];
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) {
+                        a[i][k] = *reinterpret_cast<const u32x4*>(rows + k * kTerm + sq * kRow + 8 * q);
+                        f[i][k] = *reinterpret_cast<const u32x4*>(&head.rows[k][fl][8 * q]);
+                    }
                 }
-                lds_fence();
-                // the lane's eight moves m + 8 q ...: the terms, kept where the move's square or filter is in the lane's column
-                u32x4 d[2];
-                d[0] = *reinterpret_cast<const u32x4*>(&list.hi[m + 8 * q]);
-                d[1] = *reinterpret_cast<const u32x4*>(&list.lo[m + 8 * q]);
-                const int row_lo = m + 8 * q + (col >> 2), row_hi = row_lo + 4;   // whose row the lane names in a transposed read
-                auto in_column = [&](const unsigned char* of, u32x4 (&out)[2]) {
-                    const u32x2 s8 = *reinterpret_cast<const u32x2*>(of + m + 8 * q);
+                f32x4 l[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                products<T, NT, NT>(l, [&](int i, int k) { return a[i][k]; }, [&](int i, int k) { return f[i][k]; });
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const unsigned pair = s8[i >> 1] >> 16 * (i & 1);
-                        const unsigned keep = halves((pair & 15) == (unsigned)col, (pair >> 8 & 15) == (unsigned)col);
-                        out[0][i] = d[0][i] & keep;
-                        out[1][i] = d[1][i] & keep;
-                    }
-                };
-                if (WANT & kFeaturesGrad) {
-                    u32x4 a[2][NT], mine[2], s[4][2];
-                    const short *w_lo = &head.rows[0][list.filter[row_lo]][4 * (col & 3)], *w_hi = &head.rows[0][list.filter[row_hi]][4 * (col & 3)];
-#pragma unroll
-                    for (int i = 0; i < 2 * NT; ++i) {
-                        const int at = (i % NT) * kF * kRow + 16 * (i / NT);
-                        a[i / NT][i % NT] = transposed(w_lo + at, w_hi + at);
-                    }
-                    in_column(list.square, mine);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.square_tile[j][4 * q]);
-                        s[j][0] = mine[0] & keep;
-                        s[j][1] = mine[1] & keep;
-                    }
-                    products<T, NT, 2>(g, [&](int i, int k) { return a[i >> 2][k]; }, [&](int i, int k) { return s[i & 3][k]; });
+                for (int i = 0; i < 2; ++i) {
+                    const float even = col & 2 ? l[i][2] : l[i][0], odd = col & 2 ? l[i][3] : l[i][1];
+                    if (q == col >> 2) list.logit[m + 16 * i + col] = col & 1 ? odd : even;
                 }
-                if (WANT & kKernelGrad) {
-                    u32x4 a[2][NT], mine[2];
-                    const short *x_lo = rows + list.square[row_lo] * kRow + 4 * (col & 3), *x_hi = rows + list.square[row_hi] * kRow + 4 * (col & 3);
-#pragma unroll
-                    for (int i = 0; i < 2 * NT; ++i) {
-                        const int at = (i % NT) * kTerm + 16 * (i / NT);
-                        a[i / NT][i % NT] = transposed(x_lo + at, x_hi + at);
-                    }
-                    in_column(list.filter, mine);
-                    const float w_scale = wb * x_back;
-                    f32x4 sum[2 * kTiles];
-                    u32x4 f[kTiles][2];
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t) {
-                        const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.filter_tile[t][4 * q]);
-                        f[t][0] = mine[0] & keep;
-                        f[t][1] = mine[1] & keep;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2 * kTiles; ++i) sum[i] = f32x4{0, 0, 0, 0};
-                    products<T, NT, 2>(sum, [&](int i, int k) { return a[i & 1][k]; }, [&](int i, int k) { return f[i >> 1][k]; });
-#pragma unroll
-                    for (int i = 0; i < 8 * kTiles; ++i)
-                        dw[i >> 2 & 1][i >> 3][i & 3] = fmaf(sum[i >> 2][i & 3], w_scale, dw[i >> 2 & 1][i >> 3][i & 3]);
-                }
-                lds_fence();
             }
-            if (WANT & kFeaturesGrad) store_features_grad(dx + b * (kC * kS), col, q, g, wb * w_back);
+            lds_fence();
+            const float l_target = list.logit[target];
+            float v[4], top = -INFINITY;             // [pass of 64 moves]
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                v[p] = -INFINITY;
+                if (64 * p >= count) continue;
+                if (64 * p + lane < count) v[p] = list.logit[64 * p + lane];
+                top = larger(top, v[p]);
+            }
+            top = lanes_reduce<true>(top);
+            const float unit = fminf(fmaxf(w_back * x_back, 1e-36f), 1e38f), unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
+            float z = 0.0f;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                if (64 * p >= count) continue;
+                v[p] = __builtin_amdgcn_exp2f(fmaf(v[p], unit2, top2));
+                z += v[p];
+            }
+            z = lanes_reduce<false>(z);
+            if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
+
+            if (WANT) {
+                // the logits' gradients times z, as over the vocabulary
+                const float rz = __builtin_amdgcn_rcpf(z), e_target = __builtin_amdgcn_exp2f(fmaf(l_target, unit2, top2));
+                float inv = 1.0f, wb = weight;
+                if constexpr (Arith<T>::kScaled) {
+                    float d_scale, d_back;
+                    scale_of(fabsf(e_target - z) * rz, -17, d_scale, d_back);
+                    inv = d_scale * rz;
+                    wb *= d_back;
+                } else {
+                    wb *= rz;
+                }
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    if (64 * p >= count) continue;
+                    unsigned hi, lo;
+                    Arith<T>::split((v[p] - (64 * p + lane == target ? z : 0.0f)) * inv, 0.0f, hi, lo);
+                    list.hi[64 * p + lane] = (unsigned short)hi;
+                    list.lo[64 * p + lane] = (unsigned short)lo;
+                }
+                f32x4 g[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] = f32x4{0, 0, 0, 0};
+                for (int m = 0; m < count; m += 32) {
+                    {                                // pair `col`, tile q
+                        const unsigned s2 = *reinterpret_cast<const unsigned short*>(&list.square[m + 2 * col]);
+                        const unsigned f2 = *reinterpret_cast<const unsigned short*>(&list.filter[m + 2 * col]);
+                        list.square_tile[q][col] = halves((s2 >> 4 & 15) == (unsigned)q, s2 >> 12 == (unsigned)q);
+                        list.filter_tile[q][col] = halves((f2 >> 4 & 15) == (unsigned)q, f2 >> 12 == (unsigned)q);
+                        if (q == 0) list.filter_tile[4][col] = halves((f2 >> 4 & 15) == 4, f2 >> 12 == 4);
+                    }
+                    lds_fence();
+                    // the lane's eight moves m + 8 q ...: the terms, kept where the move's square or filter is in the lane's column
+                    u32x4 d[2];
+                    d[0] = *reinterpret_cast<const u32x4*>(&list.hi[m + 8 * q]);
+                    d[1] = *reinterpret_cast<const u32x4*>(&list.lo[m + 8 * q]);
+                    const int row_lo = m + 8 * q + (col >> 2), row_hi = row_lo + 4;   // whose row the lane names in a transposed read
+                    auto in_column = [&](const unsigned char* of, u32x4 (&out)[2]) {
+                        const u32x2 s8 = *reinterpret_cast<const u32x2*>(of + m + 8 * q);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const unsigned pair = s8[i >> 1] >> 16 * (i & 1);
+                            const unsigned keep = halves((pair & 15) == (unsigned)col, (pair >> 8 & 15) == (unsigned)col);
+                            out[0][i] = d[0][i] & keep;
+                            out[1][i] = d[1][i] & keep;
+                        }
+                    };
+                    if (WANT & kFeaturesGrad) {
+                        u32x4 a[2][NT], mine[2], s[4][2];
+                        const short* w_lo = &head.rows[0][list.filter[row_lo]][4 * (col & 3)];
+                        const short* w_hi = &head.rows[0][list.filter[row_hi]][4 * (col & 3)];
+#pragma unroll
+                        for (int i = 0; i < 2 * NT; ++i) {
+                            const int at = (i % NT) * kF * kRow + 16 * (i / NT);
+                            a[i / NT][i % NT] = transposed(w_lo + at, w_hi + at);
+                        }
+                        in_column(list.square, mine);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.square_tile[j][4 * q]);
+                            s[j][0] = mine[0] & keep;
+                            s[j][1] = mine[1] & keep;
+                        }
+                        products<T, NT, 2>(g, [&](int i, int k) { return a[i >> 2][k]; }, [&](int i, int k) { return s[i & 3][k]; });
+                    }
+                    if (WANT & kKernelGrad) {
+                        u32x4 a[2][NT], mine[2];
+                        const short* x_lo = rows + list.square[row_lo] * kRow + 4 * (col & 3);
+                        const short* x_hi = rows + list.square[row_hi] * kRow + 4 * (col & 3);
+#pragma unroll
+                        for (int i = 0; i < 2 * NT; ++i) {
+                            const int at = (i % NT) * kTerm + 16 * (i / NT);
+                            a[i / NT][i % NT] = transposed(x_lo + at, x_hi + at);
+                        }
+                        in_column(list.filter, mine);
+                        const float w_scale = wb * x_back;
+                        f32x4 sum[2 * kTiles];
+                        u32x4 f[kTiles][2];
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) {
+                            const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.filter_tile[t][4 * q]);
+                            f[t][0] = mine[0] & keep;
+                            f[t][1] = mine[1] & keep;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2 * kTiles; ++i) sum[i] = f32x4{0, 0, 0, 0};
+                        products<T, NT, 2>(sum, [&](int i, int k) { return a[i & 1][k]; }, [&](int i, int k) { return f[i >> 1][k]; });
+#pragma unroll
+                        for (int i = 0; i < 8 * kTiles; ++i)
+                            dw[i >> 2 & 1][i >> 3][i & 3] = fmaf(sum[i >> 2][i & 3], w_scale, dw[i >> 2 & 1][i >> 3][i & 3]);
+                    }
+                    lds_fence();
+                }
+                if (WANT & kFeaturesGrad) store_features_grad(dx + b * (kC * kS), col, q, g, wb * w_back);
+            }
+            lds_fence();
+            if (!left) break;
         }
-        lds_fence();
-        if (!left) break;
-      }
     }
     if (lo < hi && hi == n && lane == 0 && start != n_moves) atomicOr(err, 1);
     if (WANT & kKernelGrad) {
@@ -931,8 +938,8 @@ hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, most);
     if (grid && a.per_board)
         hipLaunchKernelGGL((k_policy_move_loss<T, WANT>), dim3(grid), dim3(waves * 64),
-                           sizeof(MoveHeadLds<T>) + std::max<unsigned>(waves * move_wave_bytes<T>(WANT), kStageBytes), s, x, w, a.n, a.from, a.filter, a.per_board,
-                           a.n_moves, a.targets, a.weights, step, a.loss, dx, part, a.err);
+                           sizeof(MoveHeadLds<T>) + std::max<unsigned>(waves * move_wave_bytes<T>(WANT), kStageBytes), s, x, w, a.n,
+                           a.from, a.filter, a.per_board, a.n_moves, a.targets, a.weights, step, a.loss, dx, part, a.err);
     else if (grid)
         hipLaunchKernelGGL((k_policy_loss<T, WANT>), dim3(grid), dim3(waves * 64),
                            sizeof(HeadLds<T>) + std::max(WANT & kKernelGrad ? waves * kWaveLds : 0u, (unsigned)kStageBytes), s, x, w,

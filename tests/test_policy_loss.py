@@ -315,6 +315,10 @@ def test_no_boards(ctx, moves):
     d["w"] = torch.ones(1, device="cuda")
     loss, dx, dk = call(ctx, d)
     assert loss.shape == (0,) and dx.shape == (0, 32, 8, 8) and dk.shape == (32, 73) and not dk.any()
+    o = torch.ops.batchfirst
+    k = d["k"].clone().requires_grad_()
+    (o.policy_move_loss if moves else o.policy_loss)(ctx.handle, d["x"], k, *d["lists"], d["t"]).sum().backward()
+    assert not k.grad.any()
 
 
 @gpu
