@@ -117,7 +117,6 @@ constexpr int kRow = 40;                         // 16-bit elements of a row of 
 constexpr int kTerm = kS * kRow;                 // elements of 64 rows
 constexpr int kPart = kC * 16 * kTiles;          // elements of a part of the kernel's gradient: [32][80], 73 of 80 in use
 constexpr int kPartBytes = kPart * 4;            // a wave's in LDS, when its boards are done
-constexpr int kStageBytes = kXW * 4;             // the kernel on its way to its operands
 
 // A board's features: a lane holds channels 8 q ... 8 q + 7 of squares 4 col ... 4 col + 3 and turns them into operands
 // of columns square (4 col + j), k channel.  The scale goes by the largest finite one, so that squares that a list of
@@ -228,31 +227,20 @@ __device__ __forceinline__ void store_part(const f32x4 (&dw)[2][kTiles], unsigne
     }
 }
 
-// The kernel as float32 in `stage`, and its scale, which is by the largest finite element.
+// The kernel's scale, by its largest finite element.  Every wave looks at all of it (9 KB out of the cache, loads that are
+// in flight beside those of its operands), which spares a pass through LDS and a barrier.
 template <typename T>
-__device__ __forceinline__ void stage_head(const T* __restrict__ w, float* stage, float* red, float& scale, float& back) {
-    typedef T piece_t __attribute__((ext_vector_type(16 / sizeof(T))));
-    constexpr int kPer = 16 / sizeof(T);
-    static_assert(kXW % kPer == 0, "whole pieces");
-    float largest = 0.0f;
-#pragma unroll 3
-    for (int i = threadIdx.x; i < kXW / kPer; i += blockDim.x) {
-        const piece_t v = reinterpret_cast<const piece_t*>(w)[i];
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            stage[i * kPer + k] = (float)v[k];
-            if (finite((float)v[k])) largest = fmaxf(largest, fabsf((float)v[k]));
-        }
-    }
+__device__ __forceinline__ void head_scale(const T* __restrict__ w, int lane, float& scale, float& back) {
     scale = back = 1.0f;
     if constexpr (Arith<T>::kTerms == 2) {
-        largest = lanes_reduce<true>(largest);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = largest;
-        __syncthreads();
-        for (int i = 0; i < (int)blockDim.x >> 6; ++i) largest = fmaxf(largest, red[i]);
-        scale_of(largest, -100, scale, back);
-    } else {
-        __syncthreads();
+        constexpr int kPieces = kXW / 4, kLoads = (kPieces + 63) / 64;
+        f32x4 v[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) v[i] = reinterpret_cast<const f32x4*>(w)[min(i * 64 + lane, kPieces - 1)];
+        float largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4 * kLoads; ++i) largest = larger(largest, finite(v[i >> 2][i & 3]) ? fabsf(v[i >> 2][i & 3]) : 0.0f);
+        scale_of(lanes_reduce<true>(largest), -100, scale, back);
     }
 }
 
@@ -310,7 +298,6 @@ template <typename T>
 struct HeadLds {                                 // the kernel as operands, 16 bytes a lane
     // five for the logits: rows filter, k channel; 2 u + a: rows channel, k filter as the logits' results hold them
     u32x4 operand[kTiles + 6][Arith<T>::kTerms][64];
-    float red[8];
 };
 constexpr int kWaveLds = 2 * kTerm * 2;          // bytes a wave: the crossing
 static_assert(kWaveLds >= kPartBytes, "at the end it takes the wave's kernel gradient");
@@ -348,12 +335,9 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
 
     float w_back;
     {
-        float w_scale;
-        float* stage = reinterpret_cast<float*>(smem + sizeof(HeadLds<T>));
-        stage_head<T>(w, stage, lds.red, w_scale, w_back);
         // an operand a wave at a time: five for the logits, six for the way back; all of a wave's are read at once
         constexpr int kOperands = kTiles + (WANT & kFeaturesGrad ? 6 : 0), kRounds = (kOperands + 3) / 4;
-        float v[kRounds][8];
+        T v[kRounds][8];
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
             const int i = min(wave + r * waves, kOperands - 1), j = i - kTiles;
@@ -361,15 +345,20 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
             for (int k = 0; k < 8; ++k) {
                 const int c = i < kTiles ? 8 * q + k : 16 * (j & 1) + col;
                 const int f = i < kTiles ? 16 * i + col : 32 * (j >> 1) + 16 * (k >> 2) + 4 * q + (k & 3);
-                const float e = stage[c * kF + min(f, kF - 1)];
-                v[r][k] = f < kF ? e : 0.0f;
+                v[r][k] = w[c * kF + min(f, kF - 1)];
             }
         }
+        float w_scale;
+        head_scale<T>(w, lane, w_scale, w_back);
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
-            const int i = wave + r * waves;
+            const int i = wave + r * waves, j = i - kTiles;
+            float e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)          // the padding's filters are zero
+                e[k] = (i < kTiles ? 16 * i + col : 32 * (j >> 1) + 16 * (k >> 2) + 4 * q + (k & 3)) < kF ? (float)v[r][k] : 0.0f;
             u32x4 out[NT];
-            operand<T>(v[r], w_scale, out);
+            operand<T>(e, w_scale, out);
             if (i < kOperands)
 #pragma unroll
                 for (int k = 0; k < NT; ++k) lds.operand[i][k][lane] = out[k];
@@ -582,7 +571,6 @@ template <typename T>
 struct MoveHeadLds {
     short rows[Arith<T>::kTerms][kF][kRow];      // [filter][channel]
     uint64_t sum[8];
-    float red[8];
 };
 static_assert(sizeof(MoveHeadLds<float>) % 16 == 0 && sizeof(MoveHeadLds<__bf16>) % 16 == 0, "the waves' parts are aligned");
 struct __attribute__((aligned(16))) MoveList {   // a board's moves, up to a multiple of 32; beyond its last, that again
@@ -644,18 +632,29 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
 
     float w_back;
     {
-        float w_scale;
-        float* stage = reinterpret_cast<float*>(first_wave);
-        stage_head<T>(w, stage, head.red, w_scale, w_back);
-        for (int i = tid; i < kF * 4; i += blockDim.x) {
-            float v[8];
+        constexpr int kRounds = 2;               // (filter, eight channels) a thread; at least 256 threads
+        T v[kRounds][8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = stage[(8 * (i & 3) + k) * kF + (i >> 2)];
-            u32x4 out[NT];
-            operand<T>(v, w_scale, out);
+        for (int r = 0; r < kRounds; ++r) {
+            const int i = min(tid + r * (int)blockDim.x, kF * 4 - 1);
 #pragma unroll
-            for (int k = 0; k < NT; ++k) *reinterpret_cast<u32x4*>(&head.rows[k][i >> 2][8 * (i & 3)]) = out[k];
+            for (int k = 0; k < 8; ++k) v[r][k] = w[(8 * (i & 3) + k) * kF + (i >> 2)];
         }
+        float w_scale;
+        head_scale<T>(w, lane, w_scale, w_back);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const int i = tid + r * (int)blockDim.x;
+            float e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = (float)v[r][k];
+            u32x4 out[NT];
+            operand<T>(e, w_scale, out);
+            if (i < kF * 4)
+#pragma unroll
+                for (int k = 0; k < NT; ++k) *reinterpret_cast<u32x4*>(&head.rows[k][i >> 2][8 * (i & 3)]) = out[k];
+        }
+        static_assert(kF * 4 <= kRounds * 256, "every element");
     }
 
     // where their lists begin
@@ -928,7 +927,7 @@ hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
     const T *x = static_cast<const T*>(a.features), *w = static_cast<const T*>(a.kernel);
     T* dx = static_cast<T*>(a.d_features);
     float* part = static_cast<float*>(a.workspace);
-    // At least four waves a workgroup, which share the work on the kernel.  (Spreading a small call's boards over all
+    // At least four waves a workgroup, which share the work on the kernel's operands.  (Spreading a small call's boards over all
     // compute units, one or two a workgroup, leaves more parts to add up: 17.6 in place of 16.4 us for 512 boards.)
     // Without gradients more workgroups fit a compute unit, and as many are launched: of float32 three (registers) over the
     // vocabulary and two (LDS) over moves, else four.  One more that has to wait costs more than it brings: 40 000 boards
@@ -938,11 +937,11 @@ hipError_t launch(const PolicyLossArgs& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min<size_t>((a.n + waves - 1) / waves, most);
     if (grid && a.per_board)
         hipLaunchKernelGGL((k_policy_move_loss<T, WANT>), dim3(grid), dim3(waves * 64),
-                           sizeof(MoveHeadLds<T>) + std::max<unsigned>(waves * move_wave_bytes<T>(WANT), kStageBytes), s, x, w, a.n,
+                           sizeof(MoveHeadLds<T>) + waves * move_wave_bytes<T>(WANT), s, x, w, a.n,
                            a.from, a.filter, a.per_board, a.n_moves, a.targets, a.weights, step, a.loss, dx, part, a.err);
     else if (grid)
         hipLaunchKernelGGL((k_policy_loss<T, WANT>), dim3(grid), dim3(waves * 64),
-                           sizeof(HeadLds<T>) + std::max(WANT & kKernelGrad ? waves * kWaveLds : 0u, (unsigned)kStageBytes), s, x, w,
+                           sizeof(HeadLds<T>) + (WANT & kKernelGrad ? waves * kWaveLds : 0), s, x, w,
                            a.n, a.targets, a.weights, step, a.loss, dx, part, a.err);
     if (hipError_t e = hipGetLastError()) return e;
     if (WANT & kKernelGrad) hipLaunchKernelGGL(k_sum_parts<T>, dim3(kPart / 32), dim3(1024), 0, s, part, grid, static_cast<T*>(a.d_kernel));
