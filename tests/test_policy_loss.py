@@ -528,6 +528,72 @@ def test_captured_and_replayed(ctx, moves):
 
 
 @gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_captured_backward(ctx, moves):
+    """Loss and backward pass of leaves of their own in one graph, replayed with other features."""
+    cases = [make(70, torch.float32, seed=s, moves=moves) for s in (3, 4)]
+    if moves:
+        cases[1]["moves"] = cases[0]["moves"]
+    cases[1]["t"] = cases[0]["t"]
+    d = on_gpu(cases[0])
+    x, k = d["x"].clone().requires_grad_(), d["k"].clone().requires_grad_()
+    o = torch.ops.batchfirst
+    op = o.policy_move_loss if moves else o.policy_loss
+
+    def step():
+        x.grad, k.grad = None, None
+        op(ctx.handle, x, k, *d["lists"], d["t"]).backward(d["w"])
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        x.grad, k.grad = None, None
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            step()
+    torch.cuda.synchronize()
+    for turn in range(4):
+        other = on_gpu(cases[turn % 2])
+        want = call(ctx, other)
+        with torch.no_grad():
+            x.copy_(other["x"])
+            k.copy_(other["k"])
+            d["w"].copy_(other["w"])
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x.grad, want[1]) and torch.equal(k.grad, want[2]), turn
+
+
+@gpu
+def test_two_threads(ctx):
+    """Calls of one context from two threads, each on a stream of its own."""
+    import threading
+    cases = [on_gpu(make(400, torch.bfloat16, seed=s, moves=bool(s), longest=30)) for s in range(2)]
+    want = [call(ctx, d) for d in cases]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i] = call(ctx, cases[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:      # noqa: BLE001  reported by the test
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@gpu
 def test_streams_of_their_own(ctx):
     """Calls on two streams at once, each with its own workspace, give what they give alone."""
     cases = [on_gpu(make(700, torch.float32, seed=s, moves=s % 2 == 1, longest=30)) for s in range(4)]
