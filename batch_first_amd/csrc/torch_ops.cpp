@@ -179,6 +179,34 @@ at::Tensor once(at::Tensor g) {
     return (*refuse)({g})[0];
 }
 
+// The capture a stream belongs to, 0 if none.  The default stream never belongs to one and must not be asked during one.
+unsigned long long capture_of(hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (!s || hipStreamGetCaptureInfo(s, &status, &id) != hipSuccess) return 0;
+    return status == hipStreamCaptureStatusActive ? id : 0;
+}
+// Called in a backward pass.  While it is captured, its gradients can go to nodes of the same capture only.  A leaf's
+// accumulator stays on its first stream as long as any graph over the leaf lives: with an eager graph still there the
+// engine would make the eager stream wait for the captured one, and the process ends in the engine's threads.
+void check_receivers(torch::autograd::AutogradContext* ac, const Context& c) {
+    const auto here = c10::hip::getCurrentHIPStream(c.device.index());
+    const unsigned long long capture = capture_of(here.stream());
+    const auto node = capture ? torch::autograd::get_current_node() : nullptr;
+    if (!node) return;
+    for (size_t i = 0; i < 2; ++i) {
+        const auto& edge = node->next_edge(i);
+        if (!ac->needs_input_grad(i) || !edge.is_valid()) continue;
+        const auto there = edge.function->stream();
+        if (!there) continue;
+        // torch names a GPU's streams after CUDA's devices, the HIP stream class wants its own name
+        const auto receiver = c10::hip::HIPStream::unpack3(there->id(), there->device_index(), c10::kHIP);
+        TORCH_CHECK(receiver == here || capture_of(receiver.stream()) == capture,
+                    "a captured backward pass would hand its gradient to another stream outside the capture: drop the eager graphs "
+                    "of the same leaves first, or run them on the captured stream");
+    }
+}
+
 using Lists = std::optional<at::Tensor>;         // from-squares, move filters, moves per board: all three or none
 struct Loss : torch::autograd::Function<Loss> {
     static at::Tensor forward(torch::autograd::AutogradContext* ac, int64_t ctx, const at::Tensor& features, const at::Tensor& kernel,
@@ -199,6 +227,7 @@ struct Loss : torch::autograd::Function<Loss> {
         if (grads[0].defined()) {
             at::AutoDispatchBelowADInplaceOrView below;
             const int64_t ctx = ac->saved_data["ctx"].toInt();
+            check_receivers(ac, context(ctx));
             out = saved.size() > 3 ? policy_move_loss_grad(ctx, saved[0], saved[1], saved[3], saved[4], saved[5], saved[2], grads[0], fg, kg)
                                      : policy_loss_grad(ctx, saved[0], saved[1], saved[2], grads[0], fg, kg);
         }

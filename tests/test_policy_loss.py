@@ -566,6 +566,34 @@ def test_captured_backward(ctx, moves):
 
 
 @gpu
+def test_captured_backward_beside_an_eager_graph(ctx):
+    """Refused while an eager graph of another stream keeps a leaf's accumulator; once that is gone it is captured."""
+    d = on_gpu(make(70, torch.float32, seed=5))
+    x, k = d["x"].clone().requires_grad_(), d["k"].clone().requires_grad_()
+    op = torch.ops.batchfirst.policy_loss
+    want = call(ctx, d)
+    eager = op(ctx.handle, x, k, d["t"])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="outside the capture"):
+            op(ctx.handle, x, k, d["t"]).backward(d["w"])
+    assert x.grad is None and k.grad is None
+    eager.backward(d["w"])                      # the eager one goes on as before
+    assert torch.equal(x.grad, want[1]) and torch.equal(k.grad, want[2])
+    del eager
+    x.grad, k.grad = None, None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        op(ctx.handle, x, k, d["t"]).backward(d["w"])
+    for _ in range(3):
+        x.grad.zero_()
+        k.grad.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x.grad, want[1]) and torch.equal(k.grad, want[2])
+
+
+@gpu
 def test_two_threads(ctx):
     """Calls of one context from two threads, each on a stream of its own."""
     import threading
