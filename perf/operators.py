@@ -9,7 +9,6 @@ of that layer; the logit kernel is [32][73].
     moves        the same over the board's own list of legal moves (ops.policy_move_loss, ops.policy_move_loss_grad)
     norm         the norm over many gradients (ops.global_norm), and clipping them to a limit (ops.clip_grad_norm_)
 """
-import functools
 import math
 import random
 
@@ -138,15 +137,9 @@ def prepare(case, seed):
             lists = _moves(n, np.random.default_rng(seed))
             state["squares"], state["filters"], state["per"], state["targets"] = (torch.from_numpy(a).to(dev) for a in lists)
     if own:
-        state["ctx"] = _context()
+        from batch_first_amd import ops, weights
+        state["ctx"] = ops.DeviceContext(weights.make_weights())
     return state
-
-
-@functools.lru_cache(maxsize=None)
-def _context():
-    """The one context that a program keeps for as long as it runs."""
-    from batch_first_amd import ops, weights
-    return ops.DeviceContext(weights.make_weights())
 
 
 # ---- one pass -------------------------------------------------------------------------------------------------------
