@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/batchfirst.h"
 #include "bf_train.h"
@@ -27,9 +28,9 @@ constexpr int kC = 32, kS = 64, kF = 73, kVocab = kF * kS, kXW = kC * kF;
 // 16x16x32 MFMAs with float32 sums.  Lane l = (col = l & 15, q = l >> 4) of an operand holds eight k (8 q ... 8 q + 7) of row or
 // column col, of a result the rows 4 q ... 4 q + 3 of column col.
 //
-// float32 operands travel as two float16 terms (22 bits), scaled by a power of two, the kernel's by its largest element
-// and the features' by the board's, so that the larger term stays normal down to 2^-27 of the largest; of the four
-// products of terms the least is left out (2^-22).  bfloat16 and float16 operands are exact as they are.  The logits'
+// float32 operands travel as two float16 terms (22 bits), scaled by a power of two so that the larger term stays normal
+// down to 2^-27 of the largest: over the vocabulary the kernel's by its largest element and the features' by the board's,
+// over moves by the filter's and by the square's; of the four products of terms the least is left out (2^-22).  bfloat16 and float16 operands are exact as they are.  The logits'
 // gradients d (before the weight) travel as two terms: bfloat16 ones for bfloat16 features, else float16 ones, scaled like
 // the features.  Their largest is the target's, which is the negative sum of all the others.
 
@@ -104,6 +105,13 @@ __device__ __forceinline__ float lanes_reduce(float v) {
     return step(step(at(0), at(16)), step(at(32), at(48)));
 }
 
+// The largest over the four lanes of a column, NaN if one is, the same in all four.
+__device__ __forceinline__ float rows_max(float v) {
+    auto step = [](auto pair) { return larger(__uint_as_float(pair[0]), __uint_as_float(pair[1])); };
+    v = step(__builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return step(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+}
+
 // 2^(13 - e) for a largest magnitude in [2^e, 2^(e+1)), and its reciprocal; magnitudes below 2^least count as that.
 __device__ __forceinline__ void scale_of(float largest, int least, float& scale, float& back) {
     const int e = max((int)(__float_as_uint(largest) >> 23 & 255u) - 127, least);
@@ -119,22 +127,22 @@ constexpr int kPart = kC * 16 * kTiles;          // elements of a part of the ke
 constexpr int kPartBytes = kPart * 4;            // a wave's in LDS, when its boards are done
 
 // A board's features: a lane holds channels 8 q ... 8 q + 7 of squares 4 col ... 4 col + 3 and turns them into operands
-// of columns square (4 col + j), k channel.  The scale goes by the largest finite one, so that squares that a list of
-// moves leaves out may hold anything.
+// of columns square (4 col + j), k channel.
 template <typename T>
 struct Features {
     static constexpr int kTerms = Arith<T>::kTerms;
     typename Raw<T>::type raw[8];
     u32x4 column[4][kTerms];
-    float scale, back;
+    float back;
 
     __device__ __forceinline__ void load(const T* board, int col, int q) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const typename Raw<T>::type*>(board + (8 * q + i) * kS + 4 * col);
     }
+    // One scale for the board.
     __device__ __forceinline__ void convert() {
-        u32x2 rows[kTerms][8];                   // pairs of squares
-        scale = back = 1.0f;
+        back = 1.0f;
+        float scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};
         if constexpr (kTerms == 2) {
             float largest = 0.0f;
 #pragma unroll
@@ -146,11 +154,35 @@ struct Features {
                 for (int i = 0; i < 32; ++i) largest = larger(largest, finite(raw[i >> 2][i & 3]) ? fabsf(raw[i >> 2][i & 3]) : 0.0f);
                 largest = lanes_reduce<true>(largest);
             }
-            scale_of(largest, -100, scale, back);
+            scale_of(largest, -100, scale[0], back);
+            scale[1] = scale[2] = scale[3] = scale[0];
+        }
+        terms(scale);
+    }
+    // One for each square, by its own largest: squares that a list of moves leaves out may hold anything, and one whose
+    // moves are out of the question costs the others nothing.
+    __device__ __forceinline__ void convert_squares(f32x4& squares_back) {
+        float scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+        if constexpr (kTerms == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float largest = fabsf(raw[0][j]), b;
+#pragma unroll
+                for (int i = 1; i < 8; ++i) largest = larger(largest, fabsf(raw[i][j]));
+                scale_of(rows_max(largest), -100, scale[j], b);
+                squares_back[j] = b;
+            }
+        }
+        terms(scale);
+    }
+    __device__ __forceinline__ void terms(const float (&scale)[4]) {
+        u32x2 rows[kTerms][8];                   // pairs of squares
+        if constexpr (kTerms == 2) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
+                const int j = 2 * (i & 1);
                 unsigned hi, lo;
-                Arith<T>::split(raw[i >> 1][2 * (i & 1)] * scale, raw[i >> 1][2 * (i & 1) + 1] * scale, hi, lo);
+                Arith<T>::split(raw[i >> 1][j] * scale[j], raw[i >> 1][j + 1] * scale[j + 1], hi, lo);
                 rows[0][i >> 1][i & 1] = hi;
                 rows[1][i >> 1][i & 1] = lo;
             }
@@ -560,8 +592,13 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
 //            each in the column of its move's square, zero in the others
 //   dW       rows channel, columns filter, k move: the squares' rows, the gradients in the columns of their filters
 //
-// What bounds it is reading the features and writing their gradient: 65 536 float32 boards with lists of 32 moves in 240 us,
-// 4.5 TB/s (a copy reaches 4.75), 8 191 bfloat16 boards in 30 us, the loss alone of 65 536 float32 boards in 109 us.  (One
+// float32: every filter and every square has a scale of its own, so that what the list leaves out, or what the softmax
+// does, takes no bits from the rest.  The logits' gradients then carry the filters' units into dX and the squares' into dW,
+// as two pairs of terms, each scaled by its own largest (one scale a board and kernel: 239 in place of 245 us, and wrong
+// where an unlisted square was 1e5 times larger).
+//
+// What bounds it is reading the features and writing their gradient: 65 536 float32 boards with lists of 32 moves in 245 us,
+// 4.4 TB/s (a copy reaches 4.75), 8 191 bfloat16 boards in 30 us, the loss alone of 65 536 float32 boards in 109 us.  (One
 // float32 sum a move, with the gradients added up in LDS, took 342 us: its chains of reads and writes left the memory
 // idle; LDS's own float adds take 200 cycles each and 880 us.)  A wave's boards are neighbours: it finds where its
 // lists begin by adding up the counts of all boards before its own, a byte a board beside the 8 to 16 KB that each
@@ -570,19 +607,24 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
 template <typename T>
 struct MoveHeadLds {
     short rows[Arith<T>::kTerms][kF][kRow];      // [filter][channel]
+    float back[Arith<T>::kTerms == 2 ? (kF + 3) / 4 * 4 : 4];   // float32: one over the filter's scale
     uint64_t sum[8];
 };
 static_assert(sizeof(MoveHeadLds<float>) % 16 == 0 && sizeof(MoveHeadLds<__bf16>) % 16 == 0, "the waves' parts are aligned");
+template <typename T>
 struct __attribute__((aligned(16))) MoveList {   // a board's moves, up to a multiple of 32; beyond its last, that again
+    static constexpr int kGradients = Arith<T>::kTerms;
     float logit[256];
-    unsigned short hi[256], lo[256];             // terms of the logit's gradient
+    // terms of the logits' gradients; float32: times one over the scale of the move's filter, for dX, and of its square, for dW
+    unsigned short hi[kGradients][256], lo[kGradients][256];
+    float back[Arith<T>::kTerms == 2 ? kS : 4];  // float32: one over the square's scale
     unsigned char square[256], filter[256];      // square: its row of features
     unsigned square_tile[4][16];                 // for 32 moves, a pair a word: which of the pair is in the tile of columns
     unsigned filter_tile[kTiles][16];
 };
 template <typename T>
 constexpr unsigned move_wave_bytes(int want) {
-    const unsigned rows = Arith<T>::kTerms * kTerm * 2, most = rows + sizeof(MoveList);
+    const unsigned rows = Arith<T>::kTerms * kTerm * 2, most = rows + sizeof(MoveList<T>);
     return (want & kKernelGrad) && most < (unsigned)kPartBytes ? kPartBytes : most;
 }
 
@@ -610,7 +652,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
     const int col = lane & 15, q = lane >> 4;
     unsigned char* const first_wave = smem + sizeof(MoveHeadLds<T>);
     short* rows = reinterpret_cast<short*>(first_wave + wave * move_wave_bytes<T>(WANT));
-    MoveList& list = *reinterpret_cast<MoveList*>(rows + NT * kTerm);
+    MoveList<T>& list = *reinterpret_cast<MoveList<T>*>(rows + NT * kTerm);
 
     // the wave's boards [lo, hi)
     const size_t all = (size_t)gridDim.x * waves, me = (size_t)blockIdx.x * waves + wave;
@@ -630,7 +672,6 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
     look_up();
     if (base < hi) features.load(x + base * (kC * kS), col, q);
 
-    float w_back;
     {
         constexpr int kRounds = 2;               // (filter, eight channels) a thread; at least 256 threads
         T v[kRounds][8];
@@ -640,19 +681,27 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[r][k] = w[(8 * (i & 3) + k) * kF + (i >> 2)];
         }
-        float w_scale;
-        head_scale<T>(w, lane, w_scale, w_back);
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
             const int i = tid + r * (int)blockDim.x;
-            float e[8];
+            float e[8], w_scale = 1.0f, w_back = 1.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) e[k] = (float)v[r][k];
+            if constexpr (NT == 2) {             // the filter's scale, by its four threads
+                float largest = fabsf(e[0]);
+#pragma unroll
+                for (int k = 1; k < 8; ++k) largest = larger(largest, fabsf(e[k]));
+                largest = larger(largest, __shfl_xor(largest, 1));
+                largest = larger(largest, __shfl_xor(largest, 2));
+                scale_of(largest, -100, w_scale, w_back);
+            }
             u32x4 out[NT];
             operand<T>(e, w_scale, out);
-            if (i < kF * 4)
+            if (i < kF * 4) {
 #pragma unroll
                 for (int k = 0; k < NT; ++k) *reinterpret_cast<u32x4*>(&head.rows[k][i >> 2][8 * (i & 3)]) = out[k];
+                if (NT == 2 && (i & 3) == 0) head.back[i >> 2] = w_back;
+            }
         }
         static_assert(kF * 4 <= kRounds * 256, "every element");
     }
@@ -728,9 +777,12 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
             const size_t b = base + who;
             const int target = __builtin_amdgcn_readlane(my_target, who), count = cnt;
             const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
-            features.convert();
-            const float x_back = features.back;
+            f32x4 x_back;
+            features.convert_squares(x_back);
             write_rows<NT>(rows, col, q, features.column);
+            if (NT == 2 && q == 0) *reinterpret_cast<f32x4*>(&list.back[4 * col]) = x_back;
+            const T* const board = x + b * (kC * kS);
+            unsigned move[4];                        // [pass of 64 moves]: square, filter
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 if (64 * p >= count) continue;
@@ -740,8 +792,10 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                 }
                 if (square >= kS || filt >= kF) atomicOr(err, 1);
                 square = min(square, kS - 1u);
+                filt = min(filt, kF - 1u);
                 list.square[64 * p + lane] = (unsigned char)(16 * (square & 3) + (square >> 2));
-                list.filter[64 * p + lane] = (unsigned char)min(filt, kF - 1u);
+                list.filter[64 * p + lane] = (unsigned char)filt;
+                move[p] = square | filt << 8;
             }
             left &= left - 1;
             if (left) {
@@ -750,7 +804,9 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
             }
             lds_fence();
 
-            // logits, in units of 2^-(scales)
+            auto square_back = [&](int p) { return list.back[move[p] & 255u]; };
+            auto filter_back = [&](int p) { return head.back[move[p] >> 8]; };
+            // logits, float32 ones in units of their squares' and filters'
             for (int m = 0; m < count; m += 32) {
                 u32x4 a[2][NT], f[2][NT];
 #pragma unroll
@@ -771,47 +827,77 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                 }
             }
             lds_fence();
-            const float l_target = list.logit[target];
             float v[4], top = -INFINITY;             // [pass of 64 moves]
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 v[p] = -INFINITY;
                 if (64 * p >= count) continue;
-                if (64 * p + lane < count) v[p] = list.logit[64 * p + lane];
+                if (64 * p + lane < count) {
+                    v[p] = list.logit[64 * p + lane];
+                    if constexpr (NT == 2) {
+                        v[p] *= square_back(p) * filter_back(p);
+                        if (v[p] != v[p]) {          // an infinity has no second term, and units may pass float32's range
+                            v[p] = 0.0f;
+                            for (int c = 0; c < kC; ++c)
+                                v[p] = fmaf((float)board[c * kS + (move[p] & 255u)], (float)w[c * kF + (move[p] >> 8)], v[p]);
+                        }
+                    }
+                }
                 top = larger(top, v[p]);
             }
             top = lanes_reduce<true>(top);
-            const float unit = fminf(fmaxf(w_back * x_back, 1e-36f), 1e38f), unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
-            float z = 0.0f;
+            float l_target = 0.0f, z = 0.0f;
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 if (64 * p >= count) continue;
-                v[p] = __builtin_amdgcn_exp2f(fmaf(v[p], unit2, top2));
+                if (p == target >> 6) l_target = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v[p]), target & 63));
+                v[p] = __builtin_amdgcn_exp2f((v[p] - top) * 1.44269504088896341f);
                 z += v[p];
             }
             z = lanes_reduce<false>(z);
-            if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
+            if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, top - l_target);
 
             if (WANT) {
                 // the logits' gradients times z, as over the vocabulary
-                const float rz = __builtin_amdgcn_rcpf(z), e_target = __builtin_amdgcn_exp2f(fmaf(l_target, unit2, top2));
+                const float rz = __builtin_amdgcn_rcpf(z);
                 float inv = 1.0f, wb = weight;
-                if constexpr (Arith<T>::kScaled) {
-                    float d_scale, d_back;
-                    scale_of(fabsf(e_target - z) * rz, -17, d_scale, d_back);
-                    inv = d_scale * rz;
-                    wb *= d_back;
-                } else {
-                    wb *= rz;
+                if constexpr (NT == 1) {
+                    if constexpr (Arith<T>::kScaled) {
+                        const float e_target = __builtin_amdgcn_exp2f((l_target - top) * 1.44269504088896341f);
+                        float d_scale, d_back;
+                        scale_of(fabsf(e_target - z) * rz, -17, d_scale, d_back);
+                        inv = d_scale * rz;
+                        wb *= d_back;
+                    } else {
+                        wb *= rz;
+                    }
                 }
+                float wb_x = wb, wb_w = wb;          // what dX and dW are multiplied by
+                // float32: each takes them in the units of its factor, scaled by the largest
+                auto gradients = [&](int of, auto&& unit, float& back) {
+                    float largest = 0.0f, scale = 1.0f, scale_back;
+                    if constexpr (NT == 2) {
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    if (64 * p >= count) continue;
-                    unsigned hi, lo;
-                    Arith<T>::split((v[p] - (64 * p + lane == target ? z : 0.0f)) * inv, 0.0f, hi, lo);
-                    list.hi[64 * p + lane] = (unsigned short)hi;
-                    list.lo[64 * p + lane] = (unsigned short)lo;
-                }
+                        for (int p = 0; p < 4; ++p)
+                            if (64 * p < count) largest = larger(largest, fabsf((v[p] - (64 * p + lane == target ? z : 0.0f)) * rz * unit(p)));
+                        scale_of(lanes_reduce<true>(largest), -113, scale, scale_back);
+                        back *= scale_back;
+                    }
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        if (64 * p >= count) continue;
+                        float d = v[p] - (64 * p + lane == target ? z : 0.0f);
+                        if constexpr (NT == 2) d = d * rz * unit(p) * scale;
+                        else d *= inv;
+                        unsigned hi, lo;
+                        Arith<T>::split(d, 0.0f, hi, lo);
+                        list.hi[of][64 * p + lane] = (unsigned short)hi;
+                        list.lo[of][64 * p + lane] = (unsigned short)lo;
+                    }
+                };
+                constexpr int kOfX = 0, kOfW = NT - 1;
+                if ((WANT & kFeaturesGrad) || NT == 1) gradients(kOfX, filter_back, wb_x);
+                if ((WANT & kKernelGrad) && NT == 2) gradients(kOfW, square_back, wb_w);
                 f32x4 g[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) g[i] = f32x4{0, 0, 0, 0};
@@ -825,11 +911,10 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                     }
                     lds_fence();
                     // the lane's eight moves m + 8 q ...: the terms, kept where the move's square or filter is in the lane's column
-                    u32x4 d[2];
-                    d[0] = *reinterpret_cast<const u32x4*>(&list.hi[m + 8 * q]);
-                    d[1] = *reinterpret_cast<const u32x4*>(&list.lo[m + 8 * q]);
                     const int row_lo = m + 8 * q + (col >> 2), row_hi = row_lo + 4;   // whose row the lane names in a transposed read
-                    auto in_column = [&](const unsigned char* of, u32x4 (&out)[2]) {
+                    auto in_column = [&](int term, const unsigned char* of, u32x4 (&out)[2]) {
+                        const u32x4 d[2] = {*reinterpret_cast<const u32x4*>(&list.hi[term][m + 8 * q]),
+                                            *reinterpret_cast<const u32x4*>(&list.lo[term][m + 8 * q])};
                         const u32x2 s8 = *reinterpret_cast<const u32x2*>(of + m + 8 * q);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -848,7 +933,7 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                             const int at = (i % NT) * kF * kRow + 16 * (i / NT);
                             a[i / NT][i % NT] = transposed(w_lo + at, w_hi + at);
                         }
-                        in_column(list.square, mine);
+                        in_column(kOfX, list.square, mine);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.square_tile[j][4 * q]);
@@ -866,26 +951,32 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                             const int at = (i % NT) * kTerm + 16 * (i / NT);
                             a[i / NT][i % NT] = transposed(x_lo + at, x_hi + at);
                         }
-                        in_column(list.filter, mine);
-                        const float w_scale = wb * x_back;
-                        f32x4 sum[2 * kTiles];
-                        u32x4 f[kTiles][2];
+                        in_column(kOfW, list.filter, mine);
+                        // float32's in two turns: all five tiles' operands and sums beside a[2][2] pass the registers
+                        auto tiles = [&](auto first, auto end) {
+                            constexpr int t0 = decltype(first)::value, N = decltype(end)::value - t0;
+                            f32x4 sum[2 * N];
+                            u32x4 f[N][2];
 #pragma unroll
-                        for (int t = 0; t < kTiles; ++t) {
-                            const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.filter_tile[t][4 * q]);
-                            f[t][0] = mine[0] & keep;
-                            f[t][1] = mine[1] & keep;
-                        }
+                            for (int t = 0; t < N; ++t) {
+                                const u32x4 keep = *reinterpret_cast<const u32x4*>(&list.filter_tile[t0 + t][4 * q]);
+                                f[t][0] = mine[0] & keep;
+                                f[t][1] = mine[1] & keep;
+                            }
 #pragma unroll
-                        for (int i = 0; i < 2 * kTiles; ++i) sum[i] = f32x4{0, 0, 0, 0};
-                        products<T, NT, 2>(sum, [&](int i, int k) { return a[i & 1][k]; }, [&](int i, int k) { return f[i >> 1][k]; });
+                            for (int i = 0; i < 2 * N; ++i) sum[i] = f32x4{0, 0, 0, 0};
+                            products<T, NT, 2>(sum, [&](int i, int k) { return a[i & 1][k]; }, [&](int i, int k) { return f[i >> 1][k]; });
 #pragma unroll
-                        for (int i = 0; i < 8 * kTiles; ++i)
-                            dw[i >> 2 & 1][i >> 3][i & 3] = fmaf(sum[i >> 2][i & 3], w_scale, dw[i >> 2 & 1][i >> 3][i & 3]);
+                            for (int i = 0; i < 8 * N; ++i)
+                                dw[i >> 2 & 1][t0 + (i >> 3)][i & 3] = fmaf(sum[i >> 2][i & 3], wb_w, dw[i >> 2 & 1][t0 + (i >> 3)][i & 3]);
+                        };
+                        constexpr int kTurn = NT == 2 ? 3 : kTiles;
+                        tiles(std::integral_constant<int, 0>{}, std::integral_constant<int, kTurn>{});
+                        if constexpr (kTurn < kTiles) tiles(std::integral_constant<int, kTurn>{}, std::integral_constant<int, kTiles>{});
                     }
                     lds_fence();
                 }
-                if (WANT & kFeaturesGrad) store_features_grad(dx + b * (kC * kS), col, q, g, wb * w_back);
+                if (WANT & kFeaturesGrad) store_features_grad(dx + b * (kC * kS), col, q, g, wb_x);
             }
             lds_fence();
             if (!left) break;

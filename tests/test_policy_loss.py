@@ -727,3 +727,165 @@ def test_features_beyond_four_gib(ctx):
     want = torch.ops.batchfirst.policy_move_loss_grad(ctx.handle, x[-16:].clone(), d["k"], *last, one, kernel_grad=False)
     assert torch.equal(loss[-16:], want[0]) and torch.equal(dx[-16:], want[1])
     ctx.check_policy()
+
+
+def whole_lists(case, shortest):
+    """New lists of `shortest` moves a board at least."""
+    rng = np.random.default_rng(1)
+    per = np.maximum(case["moves"][2], shortest).astype(np.uint8)
+    m = int(per.sum())
+    case["moves"] = rng.integers(0, 64, m).astype(np.uint8), rng.integers(0, 73, m).astype(np.uint8), per
+    return case["moves"]
+
+
+@gpu
+@pytest.mark.parametrize("value", [1e4, 1e8, 1e12, 1e20, 3e38])
+def test_unlisted_squares_and_filters_of_any_size(ctx, value):
+    """Finite values in squares and in columns of the kernel that no listed move uses change no bit, however large."""
+    case = make(7, torch.float32, seed=17, moves=True, longest=40)
+    sq, fl, per = whole_lists(case, 1)
+    sq[:], fl[:] = sq % 32, fl % 60              # squares 32 ... 63 and filters 60 ... 72 of every board
+    case["t"] = torch.zeros(7, dtype=torch.int64)
+    case["x"].view(7, 32, 64)[:, :, 32:] = 0
+    case["k"][:, 60:] = 0
+    clean = check_all(ctx, case)
+    for kind in ("square", "filter", "both"):
+        big = dict(case, x=case["x"].clone(), k=case["k"].clone())
+        if kind != "filter":
+            big["x"].view(7, 32, 64)[:, 5:9, 40:50] = value
+            big["x"].view(7, 32, 64)[:, 20, 33] = -value
+        if kind != "square":
+            big["k"][3:5, 61:70] = -value
+            big["k"][17, 72] = value
+        d = on_gpu(big)
+        assert torch.equal(forward(ctx, d), clean[0]), kind
+        # what the unlisted columns and squares hold takes no part in either gradient
+        assert all(torch.equal(a, b) for a, b in zip(call(ctx, d), clean)), kind
+
+
+def without(case, masked):
+    """`case` with lists of the moves that `masked` (filter, square) leaves, for the oracle alone: targets as before."""
+    n = len(case["t"])
+    if case["moves"] is None:
+        f, s = np.divmod(np.arange(4672), 64)
+        boards = [(s, f)] * n
+    else:
+        ends = np.cumsum(case["moves"][2].astype(int))
+        boards = [(case["moves"][0][a:b].astype(int), case["moves"][1][a:b].astype(int)) for a, b in zip(ends - case["moves"][2], ends)]
+    out, sq, fl, per, targets = dict(case), [], [], [], []
+    for (s, f), t in zip(boards, case["t"].tolist()):
+        keep = ~masked(f, s)
+        assert keep[t]
+        sq.append(s[keep]), fl.append(f[keep]), per.append(int(keep.sum())), targets.append(int(keep[:t].sum()))
+    out["moves"], out["t"] = (np.concatenate(sq), np.concatenate(fl), np.array(per)), torch.tensor(targets)
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("value", [1e5, 1e9, 1e20, 1e36])
+@pytest.mark.parametrize("what", ["filter", "square"])
+@pytest.mark.parametrize("moves", [True], ids=["moves"])
+def test_logits_far_below_the_others(ctx, moves, what, value):
+    """Filters or squares whose logits a large negative value takes out of the softmax: the others keep their precision.
+
+    The oracle sees them taken out of the lists: at -1e4 and below, exp is zero in 64 bits too."""
+    case = make(9, torch.float32, seed=23, moves=moves)
+    case["x"] += 0.25                            # every channel of every square counts
+    x, k = case["x"].view(9, 32, 64), case["k"]
+    if what == "filter":
+        k[:, 7], k[:, 64] = -value, -value / 3
+        masked = lambda f, s: (f == 7) | (f == 64)
+    else:
+        k[11] = -(k[11].abs() + 0.125)
+        x[:, 11, 5], x[:, 11, 63] = value, value / 3
+        masked = lambda f, s: (s == 5) | (s == 63)
+    if moves:                                    # a target that is left, and one masked move at least
+        sq, fl, per = whole_lists(case, 3)
+        first = np.cumsum(per.astype(int)) - per
+        sq[first], fl[first], sq[first + 1], fl[first + 1] = 5, 7, 9, 11
+        case["t"] = torch.ones(9, dtype=torch.int64)
+    else:
+        case["t"] = torch.arange(9) * 65 + 66    # filters 1 ... 9, squares 2 ... 10
+        case["t"][case["t"] // 64 == 7] = 66
+        case["t"][case["t"] % 64 == 5] = 66
+    left = without(case, masked)
+    small = dict(left, x=case["x"].clone(), k=case["k"].clone())      # for the tolerances: values that take part
+    if what == "filter":
+        small["k"][:, 7] = small["k"][:, 64] = 0
+    else:
+        small["x"].view(9, 32, 64)[:, 11, 5] = small["x"].view(9, 32, 64)[:, 11, 63] = 0
+    ref = reference(small)
+    tol = limits(ref, small)
+    d = on_gpu(case)
+    loss = forward(ctx, d)
+    close(loss, ref["loss"], tol[0], "loss")
+    got = call(ctx, d)
+    assert torch.equal(got[0], loss)
+    close(got[1], ref["d_features"], tol[1], "d_features")
+    close(got[2], ref["d_kernel"], tol[2], "d_kernel")
+    only = call(ctx, d, kernel_grad=False), call(ctx, d, features_grad=False)
+    assert torch.equal(only[0][1], got[1]) and torch.equal(only[1][2], got[2])
+    ctx.check_policy()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("moves", [True], ids=["moves"])
+def test_logits_of_minus_infinity(ctx, moves, dtype):
+    """An infinity that makes a square's logits -inf takes them out of the softmax; only its channel's row of the kernel's
+    gradient, 0 times infinity, is NaN, as by the formula.  One that makes a logit +inf makes its board's loss NaN."""
+    case = make(5, dtype, seed=29, moves=moves)
+    case["k"][11] = -(case["k"][11].float().abs() + 0.125).to(dtype)
+    if moves:
+        sq, fl, per = whole_lists(case, 3)
+        first = np.cumsum(per.astype(int)) - per
+        sq[first], fl[first], sq[first + 1], fl[first + 1] = 5, 7, 9, 11
+        case["t"] = torch.ones(5, dtype=torch.int64)
+    else:
+        case["t"] = torch.arange(5) * 65 + 70     # squares 6 ... 10
+    left = without(case, lambda f, s: s == 5)
+    ref = reference(left)
+    tol = limits(ref, left)
+    case["x"].view(5, 32, 64)[:, 11, 5] = float("inf")
+    d = on_gpu(case)
+    close(forward(ctx, d), ref["loss"], tol[0], "loss")
+    got = call(ctx, d)
+    close(got[0], ref["loss"], tol[0], "loss")
+    close(got[1], ref["d_features"], tol[1], "d_features")
+    rest = torch.arange(32) != 11
+    close(got[2][rest.cuda()], ref["d_kernel"][rest.numpy()], tol[2][rest.numpy()], "d_kernel")
+    assert got[2][11].isnan().all()
+    case["x"].view(5, 32, 64)[2, 11, 5] = -float("inf")
+    got = call(ctx, on_gpu(case))[0].cpu()
+    assert got[2].isnan() and not got[[0, 1, 3, 4]].isnan().any()
+
+
+@gpu
+@pytest.mark.parametrize("moves", [True], ids=["moves"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+def test_logits_at_the_end_of_the_range(ctx, dtype, moves):
+    """Logits near float32's largest, of either sign: their differences are what counts.  One channel makes the logits
+    up: features 2^63 times powers of two, the kernel 2^62 ... 2^64; one place stands out and is the target or is not."""
+    for sign in (1, -1):
+        case = make(4, dtype, seed=3, moves=moves)
+        case["x"].zero_(), case["k"].zero_()
+        x, k = case["x"].view(4, 32, 64), case["k"]
+        x[:, 6] = 2.0 ** 63
+        k[6] = sign * 2.0 ** 64
+        k[6, 3] = sign * (2.0 ** 64 + (2.0 ** 63 if sign > 0 else -(2.0 ** 63)))     # sign > 0: the largest, 1.5 * 2^127
+        k[6, 4] = sign * 2.0 ** 62                                                  # sign < 0: the largest, -2^125
+        best = 3 if sign > 0 else 4
+        if moves:
+            case["moves"] = (np.array([9, 8, 7] * 4, np.uint8), np.array([best, 5, 6] * 4, np.uint8), np.full(4, 3, np.uint8))
+            case["t"] = torch.tensor([0, 1, 0, 2])
+        else:
+            x[:, 6, :] = 2.0 ** 62
+            x[:, 6, 10] = 2.0 ** 63 if sign > 0 else 2.0 ** 61
+            case["t"] = torch.tensor([64 * best + 10, 1, 64 * best + 10, 700])
+        want = np.asarray(reference(case)["loss"])
+        got = forward(ctx, on_gpu(case)).double().cpu().numpy()
+        # exact products and one place that holds all of the probability: its loss is 0, the others' a difference
+        # of two numbers of float32, rounded once
+        with np.errstate(over="ignore"):
+            assert np.array_equal(got, want.astype(np.float32).astype(np.float64)), (got, want)
+        assert got[0] == 0 and got[1] > 1e30
