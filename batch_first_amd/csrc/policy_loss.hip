@@ -112,13 +112,13 @@ __device__ __forceinline__ float rows_max(float v) {
     return step(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
 }
 
-// 2^(13 - e) for a largest magnitude in [2^e, 2^(e+1)), and its reciprocal; magnitudes below 2^least count as that.
+// 2^(13 - e) for a largest magnitude in [2^e, 2^(e+1)), and its reciprocal; magnitudes below 2^least count as that, infinity
+// and NaN as 2^128.
 __device__ __forceinline__ void scale_of(float largest, int least, float& scale, float& back) {
     const int e = max((int)(__float_as_uint(largest) >> 23 & 255u) - 127, least);
     scale = __uint_as_float((unsigned)(127 + 13 - e) << 23);
     back = __uint_as_float((unsigned)(127 - 13 + e) << 23);
 }
-__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
 constexpr int kTiles = 5;                        // of 16 filters
 constexpr int kRow = 40;                         // 16-bit elements of a row of 32 in LDS: 16 rows start in 16 different bank groups
@@ -139,7 +139,7 @@ struct Features {
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const typename Raw<T>::type*>(board + (8 * q + i) * kS + 4 * col);
     }
-    // One scale for the board.
+    // One scale for the board; float32: not finite where a feature is not.
     __device__ __forceinline__ void convert() {
         back = 1.0f;
         float scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};
@@ -148,12 +148,6 @@ struct Features {
 #pragma unroll
             for (int i = 0; i < 32; ++i) largest = larger(largest, fabsf(raw[i >> 2][i & 3]));
             largest = lanes_reduce<true>(largest);
-            if (!finite(largest)) {
-                largest = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) largest = larger(largest, finite(raw[i >> 2][i & 3]) ? fabsf(raw[i >> 2][i & 3]) : 0.0f);
-                largest = lanes_reduce<true>(largest);
-            }
             scale_of(largest, -100, scale[0], back);
             scale[1] = scale[2] = scale[3] = scale[0];
         }
@@ -259,7 +253,7 @@ __device__ __forceinline__ void store_part(const f32x4 (&dw)[2][kTiles], unsigne
     }
 }
 
-// The kernel's scale, by its largest finite element.  Every wave looks at all of it (9 KB out of the cache, loads that are
+// The kernel's scale, by its largest element.  Every wave looks at all of it (9 KB out of the cache, loads that are
 // in flight beside those of its operands), which spares a pass through LDS and a barrier.
 template <typename T>
 __device__ __forceinline__ void head_scale(const T* __restrict__ w, int lane, float& scale, float& back) {
@@ -271,7 +265,7 @@ __device__ __forceinline__ void head_scale(const T* __restrict__ w, int lane, fl
         for (int i = 0; i < kLoads; ++i) v[i] = reinterpret_cast<const f32x4*>(w)[min(i * 64 + lane, kPieces - 1)];
         float largest = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4 * kLoads; ++i) largest = larger(largest, finite(v[i >> 2][i & 3]) ? fabsf(v[i >> 2][i & 3]) : 0.0f);
+        for (int i = 0; i < 4 * kLoads; ++i) largest = larger(largest, fabsf(v[i >> 2][i & 3]));
         scale_of(lanes_reduce<true>(largest), -100, scale, back);
     }
 }
@@ -334,8 +328,105 @@ struct HeadLds {                                 // the kernel as operands, 16 b
 constexpr int kWaveLds = 2 * kTerm * 2;          // bytes a wave: the crossing
 static_assert(kWaveLds >= kPartBytes, "at the end it takes the wave's kernel gradient");
 
+// A float32 board whose largest feature and the kernel's largest element make 2^12 or more, or are not finite.  What two
+// float16 terms lose, 2^-38 of the largest, would begin to show in logits that the largest take no part in (a filter that a
+// column of -1e30 takes out of the softmax, say), so such a board goes by float32 MFMAs, which take a few times as long.
+constexpr float kWide = 0x1p-16f;                // 2^(12 - 2) by the scales' reciprocals, 2^-13 each
+
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// v as the main path has it, in units of 1: rows filter, columns square, k channel 8 q + i in step i
+template <typename T>
+__device__ __forceinline__ void wide_logits(const T* __restrict__ board, const T* __restrict__ w, int col, int q, f32x16 (&v)[kTiles]) {
+    Features<T> f;
+    f.load(board, col, q);
+    asm volatile("" : "+v"(col), "+v"(q));       // addresses worked out here, not kept through the main path
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        f32x4 l[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+        const T* filter = w + 8 * q * kF + min(16 * t + col, kF - 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = (float)filter[i * kF];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[j] = mfma_f32(a, (float)f.raw[i][j], l[j]);
+            __builtin_amdgcn_sched_barrier(0);       // no loads ahead: the registers are the main path's
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[t][k] = l[k >> 2][k & 3];
+    }
+}
+
+// The filter of column `col` of tile t of the kernel's gradient: c of a pair of tiles is 16 (c >> 2 & 1) + 4 (c >> 3) + (c & 3)
+// of the pair's 32.
+__device__ __forceinline__ int filter_of(int t, int col) {
+    const int c = 16 * (t & 1) + col;
+    return t == kTiles - 1 ? 64 + col : 32 * (t >> 1) + 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
+}
+
+// Both gradients from v = the logits' gradients times z.
+template <int WANT, typename T>
+__device__ __forceinline__ void wide_gradients(const T* __restrict__ board, const T* __restrict__ w, float* crossing, int lane, float rz,
+                                               float weight, f32x16 (&v)[kTiles], T* __restrict__ dx, f32x4 (&dw)[2][kTiles]) {
+    asm volatile("" : "+v"(lane));
+    const int col = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[t][k] *= rz;
+    if (WANT & kFeaturesGrad) {                  // k filter: a step takes row r of the four lanes' results where it is
+        f32x4 g[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int f = 16 * t + 4 * q + r;
+                const T* channel = w + col * kF + min(f, kF - 1);
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const float e = (float)channel[16 * a * kF], k = f < kF ? e : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) g[4 * a + j] = mfma_f32(k, v[t][4 * j + r], g[4 * a + j]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        store_features_grad(dx, col, q, g, weight);
+    }
+    if (WANT & kKernelGrad) {                    // k square: a pair of tiles crosses the lanes by LDS, a square's 32 filters a row
+        constexpr int kPitch = 36;
+        static_assert(kS * kPitch * 4 <= kWaveLds, "a pair of tiles");
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+            const int tiles = u < 2 ? 2 : 1;
+#pragma unroll
+            for (int i = 0; i < 4 * tiles; ++i) {
+                const f32x16& p = v[2 * u + (i >> 2)];
+                const int j = i & 3;
+                *reinterpret_cast<f32x4*>(crossing + (4 * col + j) * kPitch + 16 * (i >> 2) + 4 * q) =
+                    f32x4{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]};
+            }
+            lds_fence();
+            f32x4 s[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll 1
+            for (int k = q; k < kS; k += 4) {
+                const float a[2] = {(float)board[col * kS + k], (float)board[(16 + col) * kS + k]};
+#pragma unroll
+                for (int i = 0; i < 2 * tiles; ++i)
+                    s[i] = mfma_f32(a[i & 1], crossing[k * kPitch + (filter_of(2 * u + (i >> 1), col) - 32 * u)], s[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * tiles; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dw[i & 1][2 * u + (i >> 1)][r] = fmaf(s[i][r], weight, dw[i & 1][2 * u + (i >> 1)][r]);
+            lds_fence();
+        }
+    }
+}
+
 template <typename T, int WANT>
-__global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
+__global__ __launch_bounds__(512, WANT ? 2 : 3) void k_policy_loss(const T* __restrict__ x, const T* __restrict__ w, size_t n,
                                                      const int64_t* __restrict__ targets, const float* __restrict__ weights,
                                                      unsigned weight_step, float* __restrict__ loss, T* __restrict__ dx,
                                                      float* __restrict__ dw_part, int* __restrict__ err) {
@@ -356,13 +447,13 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
     size_t base = (size_t)wave * gridDim.x + blockIdx.x; // lane i looks after board base + i step
     int64_t t64;
     float my_weight;
-    auto look_up = [&] {
+    auto look_up = [&](int lane) {
         const size_t b = base + lane * step;
         t64 = b < n ? targets[b] : -1;
         my_weight = WANT && b < n ? weights[b * weight_step] : 0.0f;
     };
     // the first board's loads are under way while the kernel is prepared
-    look_up();
+    look_up(lane);
     if (base < n) features.load(x + base * (kC * kS), col, q);
 
     float w_back;
@@ -404,12 +495,14 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
         for (int i = 0; i < 2 * kTiles; ++i) dw[i / kTiles][i % kTiles] = f32x4{0, 0, 0, 0};
 
     for (bool loaded = true; base < n; base += 64 * step, loaded = false) {
-        if (!loaded) look_up();
-        const bool in = base + lane * step < n, valid = t64 >= 0 && t64 < kVocab;
+        int mine_at = lane;
+        asm volatile("" : "+v"(mine_at));        // worked out here, not kept in registers through the loop
+        if (!loaded) look_up(mine_at);
+        const bool in = base + mine_at * step < n, valid = t64 >= 0 && t64 < kVocab;
         const int my_target = (int)t64;
         if (in && !valid) {                      // no part in anything, whatever the features hold
             if (t64 != -1) atomicOr(err, 1);
-            if (loss) loss[base + lane * step] = 0.0f;
+            if (loss) loss[base + mine_at * step] = 0.0f;
         }
         if (WANT & kFeaturesGrad)
             for (uint64_t left = __ballot(in && !valid); left; left &= left - 1)
@@ -426,6 +519,77 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
             features.convert();
             const u32x4 (&xc)[4][NT] = features.column;
             const float x_back = features.back;
+            // From logits in units of `unit` to the loss and v = the logits' gradients times z; the others' come from
+            // the target's, d_target.
+            auto solve = [&](f32x16 (&v)[kTiles], float unit, float& rz, float& d_target) __attribute__((always_inline)) {
+                // the padding's filters 73 ... 79
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (64 + 4 * q + r >= kF) v[kTiles - 1][4 * j + r] = -INFINITY;
+
+                // the target's place: tile, register and lane are uniform
+                const int tf = target >> 6, ts = target & 63;
+                const int t_tile = tf >> 4, t_reg = (ts & 3) * 4 + (tf & 3), t_lane = (tf >> 2 & 3) * 16 + (ts >> 2);
+                auto at_target = [&](auto&& change) {    // returns what the target's lane then holds
+                    float e = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t)
+                        if (t == t_tile) {
+                            e = change(v[t][t_reg]);
+                            v[t][t_reg] = e;
+                            asm volatile("" : "+v"(e));  // keeps the branch
+                        }
+                    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), t_lane));
+                };
+                float l_target = at_target([&](float e) { return e; });
+
+                float top = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) top = larger(top, larger(v[t][k], v[t][k + 1]));
+                top = lanes_reduce<true>(top);
+                // exp(l - top) = 2^(l unit - top unit); an error of the rounded second product is common to all of the board.
+                // Where the products pass float32's range, or their rounding shows, the largest is subtracted first.
+                if (fabsf(top) * unit > 4096.0f) {
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[t][k] -= top;
+                    l_target -= top;
+                    top = 0.0f;
+                }
+                const float unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
+                float z4[4] = {};
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        v[t][k] = __builtin_amdgcn_exp2f(fmaf(v[t][k], unit2, top2));
+                        z4[k & 3] += v[t][k];
+                    }
+                const float z = lanes_reduce<false>((z4[0] + z4[1]) + (z4[2] + z4[3]));
+                if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
+                if (!WANT) return;
+                // the logits' gradients times z: exponentials, less z at the target.  The target's is the largest but for
+                // rounding: z's own, up to 90 * 2^-24, can make the target's smaller than another by as much, which the least
+                // scale covers.
+                rz = __builtin_amdgcn_rcpf(z);
+                d_target = at_target([&](float e) { return e - (lane == t_lane ? z : 0.0f); }) * rz;
+            };
+            if (NT == 2 && __builtin_expect(!(w_back * x_back <= kWide), 0)) {
+                const T* board = x + b * (kC * kS);
+                f32x16 v[kTiles];
+                wide_logits(board, w, col, q, v);
+                float rz, d_target;
+                solve(v, 1.0f, rz, d_target);
+                const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
+                if (WANT) wide_gradients<WANT>(board, w, reinterpret_cast<float*>(mine), lane, rz, weight, v, dx + b * (kC * kS), dw);
+                features.load(next, col, q);
+                continue;
+            }
             if (WANT == 0) features.load(next, col, q);
             u32x4 xr[2][2][NT];                      // and as rows (channel, k square) for dW
             if (WANT & kKernelGrad) {
@@ -448,55 +612,9 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
 #pragma unroll
                 for (int k = 0; k < 16; ++k) v[t][k] = l[k >> 2][k & 3];
             }
-            // the padding's filters 73 ... 79
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (64 + 4 * q + r >= kF) v[kTiles - 1][4 * j + r] = -INFINITY;
-
-            // the target's place: tile, register and lane are uniform
-            const int tf = target >> 6, ts = target & 63;
-            const int t_tile = tf >> 4, t_reg = (ts & 3) * 4 + (tf & 3), t_lane = (tf >> 2 & 3) * 16 + (ts >> 2);
-            auto at_target = [&](auto&& change) {    // returns what the target's lane then holds
-                float e = 0.0f;
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t)
-                    if (t == t_tile) {
-                        e = change(v[t][t_reg]);
-                        v[t][t_reg] = e;
-                        asm volatile("" : "+v"(e));  // keeps the branch
-                    }
-                return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), t_lane));
-            };
-            const float l_target = at_target([&](float e) { return e; });
-
-            float top = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                for (int k = 0; k < 16; k += 2) top = larger(top, larger(v[t][k], v[t][k + 1]));
-            top = lanes_reduce<true>(top);
-            // exp(l - top) = 2^(l unit - top unit); an error of the rounded second product is common to all of the board
-            const float unit = fminf(fmaxf(w_back * x_back, 1e-36f), 1e38f);
-            const float unit2 = unit * 1.44269504088896341f, top2 = -(top * unit2);
-            float z4[4] = {};
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    v[t][k] = __builtin_amdgcn_exp2f(fmaf(v[t][k], unit2, top2));
-                    z4[k & 3] += v[t][k];
-                }
-            const float z = lanes_reduce<false>((z4[0] + z4[1]) + (z4[2] + z4[3]));
-            if (loss && lane == 0) loss[b] = fmaf(__builtin_amdgcn_logf(z), 0.693147180559945309f, (top - l_target) * unit);
+            float rz, d_target;
+            solve(v, fmaxf(w_back * x_back, 1e-36f), rz, d_target);
             if (!WANT) continue;
-
-            // the logits' gradients times z: exponentials, less z at the target.  The target's is the largest but for
-            // rounding: z's own, up to 90 * 2^-24, can make the target's smaller than another by as much, which the least
-            // scale covers.
-            const float rz = __builtin_amdgcn_rcpf(z);
-            const float d_target = at_target([&](float e) { return e - (lane == t_lane ? z : 0.0f); }) * rz;
             float inv = 1.0f, wb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), who));
             if constexpr (Arith<T>::kScaled) {
                 float d_scale, d_back;
@@ -574,11 +692,7 @@ __global__ __launch_bounds__(512) void k_policy_loss(const T* __restrict__ x, co
         }
     }
     if (WANT & kKernelGrad)
-        store_part(dw, smem + sizeof(HeadLds<T>), kWaveLds, wave, waves, col, q, dw_part + (size_t)blockIdx.x * kPart, [](int t, int col) {
-            // column c of a pair of tiles is filter 16 (c >> 2 & 1) + 4 (c >> 3) + (c & 3) of the pair's 32
-            const int c = 16 * (t & 1) + col;
-            return t == 4 ? 64 + col : 32 * (t >> 1) + 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
-        });
+        store_part(dw, smem + sizeof(HeadLds<T>), kWaveLds, wave, waves, col, q, dw_part + (size_t)blockIdx.x * kPart, filter_of);
 }
 
 // ---- the boards' own moves -------------------------------------------------------------------------------------------

@@ -784,7 +784,7 @@ def without(case, masked):
 @gpu
 @pytest.mark.parametrize("value", [1e5, 1e9, 1e20, 1e36])
 @pytest.mark.parametrize("what", ["filter", "square"])
-@pytest.mark.parametrize("moves", [True], ids=["moves"])
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
 def test_logits_far_below_the_others(ctx, moves, what, value):
     """Filters or squares whose logits a large negative value takes out of the softmax: the others keep their precision.
 
@@ -830,7 +830,7 @@ def test_logits_far_below_the_others(ctx, moves, what, value):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
-@pytest.mark.parametrize("moves", [True], ids=["moves"])
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
 def test_logits_of_minus_infinity(ctx, moves, dtype):
     """An infinity that makes a square's logits -inf takes them out of the softmax; only its channel's row of the kernel's
     gradient, 0 times infinity, is NaN, as by the formula.  One that makes a logit +inf makes its board's loss NaN."""
@@ -861,7 +861,7 @@ def test_logits_of_minus_infinity(ctx, moves, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("moves", [True], ids=["moves"])
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
 def test_logits_at_the_end_of_the_range(ctx, dtype, moves):
     """Logits near float32's largest, of either sign: their differences are what counts.  One channel makes the logits
