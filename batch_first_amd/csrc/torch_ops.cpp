@@ -207,6 +207,12 @@ void check_receivers(torch::autograd::AutogradContext* ac, const Context& c) {
     }
 }
 
+// Forward-mode derivatives are not implemented: a result without a tangent would read as a derivative of zero.
+void no_tangents(at::ArrayRef<at::Tensor> inputs, const char* what) {
+    for (const at::Tensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "forward-mode derivatives of ", what, " are not implemented");
+}
+
 using Lists = std::optional<at::Tensor>;         // from-squares, move filters, moves per board: all three or none
 struct Loss : torch::autograd::Function<Loss> {
     static at::Tensor forward(torch::autograd::AutogradContext* ac, int64_t ctx, const at::Tensor& features, const at::Tensor& kernel,
@@ -225,6 +231,7 @@ struct Loss : torch::autograd::Function<Loss> {
         const bool fg = ac->needs_input_grad(0), kg = ac->needs_input_grad(1);   // counts tensors only
         std::tuple<at::Tensor, at::Tensor, at::Tensor> out;
         if (grads[0].defined()) {
+            no_tangents(grads[0], "a batchfirst loss's gradient");
             at::AutoDispatchBelowADInplaceOrView below;
             const int64_t ctx = ac->saved_data["ctx"].toInt();
             check_receivers(ac, context(ctx));
@@ -239,15 +246,34 @@ struct Loss : torch::autograd::Function<Loss> {
 bool differentiable(const at::Tensor& a, const at::Tensor& b) { return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad()); }
 
 at::Tensor policy_loss_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel, const at::Tensor& targets) {
+    no_tangents({features, kernel}, "policy_loss");
     if (differentiable(features, kernel)) return Loss::apply(ctx, features, kernel, targets, Lists(), Lists(), Lists());
     at::AutoDispatchBelowADInplaceOrView below;
     return policy_loss(ctx, features, kernel, targets);
 }
 at::Tensor policy_move_loss_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel, const at::Tensor& from_squares,
                                      const at::Tensor& move_filters, const at::Tensor& moves_per_board, const at::Tensor& targets) {
+    no_tangents({features, kernel}, "policy_move_loss");
     if (differentiable(features, kernel)) return Loss::apply(ctx, features, kernel, targets, Lists(from_squares), Lists(move_filters), Lists(moves_per_board));
     at::AutoDispatchBelowADInplaceOrView below;
     return policy_move_loss(ctx, features, kernel, from_squares, move_filters, moves_per_board, targets);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> policy_loss_grad_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel,
+                                                                         const at::Tensor& targets, const at::Tensor& board_weights,
+                                                                         bool features_grad, bool kernel_grad) {
+    no_tangents({features, kernel, board_weights}, "policy_loss_grad");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return policy_loss_grad(ctx, features, kernel, targets, board_weights, features_grad, kernel_grad);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> policy_move_loss_grad_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel,
+                                                                              const at::Tensor& from_squares, const at::Tensor& move_filters,
+                                                                              const at::Tensor& moves_per_board, const at::Tensor& targets,
+                                                                              const at::Tensor& board_weights, bool features_grad,
+                                                                              bool kernel_grad) {
+    no_tangents({features, kernel, board_weights}, "policy_move_loss_grad");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return policy_move_loss_grad(ctx, features, kernel, from_squares, move_filters, moves_per_board, targets, board_weights, features_grad,
+                                 kernel_grad);
 }
 
 // ---- norms ---------------------------------------------------------------------------------------------------------
@@ -324,6 +350,17 @@ at::Tensor clip_grad_norm_(int64_t ctx, at::TensorList tensors, double max_norm)
     return t.norm;
 }
 
+at::Tensor global_norm_autograd(int64_t ctx, at::TensorList tensors) {
+    no_tangents(tensors, "global_norm");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return global_norm(ctx, tensors);
+}
+at::Tensor clip_grad_norm_autograd(int64_t ctx, at::TensorList tensors, double max_norm) {
+    no_tangents(tensors, "clip_grad_norm_");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return clip_grad_norm_(ctx, tensors, max_norm);
+}
+
 }  // namespace
 
 extern "C" {
@@ -362,6 +399,8 @@ TORCH_LIBRARY_IMPL(batchfirst, Autograd, m) {
     m.impl("policy_loss", policy_loss_autograd);
     m.impl("policy_move_loss", policy_move_loss_autograd);
     // not differentiable: what they return does not require grad
-    for (const char* name : {"policy_loss_grad", "policy_move_loss_grad", "global_norm", "clip_grad_norm_"})
-        m.impl(name, torch::CppFunction::makeFallthrough());
+    m.impl("policy_loss_grad", policy_loss_grad_autograd);
+    m.impl("policy_move_loss_grad", policy_move_loss_grad_autograd);
+    m.impl("global_norm", global_norm_autograd);
+    m.impl("clip_grad_norm_", clip_grad_norm_autograd);
 }

@@ -332,3 +332,27 @@ def _scores(x, kernel, lists):
     for b, p in enumerate(per):
         yield np.einsum("cm,cm->m", xs[b][:, sq[at:at + p]], k[:, fl[at:at + p]])
         at += p
+
+
+def refuses_tangents(handle, device):
+    import torch.autograd.forward_ad as fwad
+    o, t = torch.ops.batchfirst, torch.ones(5, device=device)
+    with fwad.dual_level():
+        dual = fwad.make_dual(t, torch.ones_like(t))
+        with pytest.raises(NotImplementedError, match="forward-mode derivatives of global_norm "):
+            o.global_norm(handle, [t, dual])
+        with pytest.raises(NotImplementedError, match="forward-mode derivatives of clip_grad_norm_ "):
+            o.clip_grad_norm_(handle, [dual, t], 1.0)
+    with pytest.raises(NotImplementedError, match="forward-mode derivatives of global_norm "):
+        torch.func.jvp(lambda a: o.global_norm(handle, [a]), (t,), (torch.ones_like(t),))
+    assert torch.equal(t, torch.ones_like(t))
+
+
+def test_forward_mode_is_refused():
+    from batch_first_amd import ops                # noqa: F401  registers the operators
+    refuses_tangents(1, "cpu")
+
+
+@gpu
+def test_forward_mode_is_refused_on_the_gpu(ctx):
+    refuses_tangents(ctx.handle, "cuda")

@@ -175,6 +175,36 @@ def test_ops_refuse_host_tensors_and_unknown_contexts():
         o.policy_loss(1, x, k, t)
 
 
+def refuses_tangents(handle, device):
+    """Every form, given a tensor with a tangent, in place of a result without one (a derivative of zero)."""
+    import torch.autograd.forward_ad as fwad
+    o = torch.ops.batchfirst
+    x, k, t = torch.zeros(2, 32, 8, 8, device=device), torch.zeros(32, 73, device=device), torch.zeros(2, dtype=torch.int64, device=device)
+    u8 = torch.ones(2, dtype=torch.uint8, device=device)
+    w = torch.ones(2, device=device)
+    calls = {"policy_loss": lambda x, k, w: o.policy_loss(handle, x, k, t),
+             "policy_move_loss": lambda x, k, w: o.policy_move_loss(handle, x, k, u8, u8, u8, t),
+             "policy_loss_grad": lambda x, k, w: o.policy_loss_grad(handle, x, k, t, w),
+             "policy_move_loss_grad": lambda x, k, w: o.policy_move_loss_grad(handle, x, k, u8, u8, u8, t, w)}
+    for name, call_ in calls.items():
+        for i in range(3 if name.endswith("grad") else 2):
+            for leaf in (False, True):
+                args = [a.clone().requires_grad_(leaf) for a in (x, k, w)]
+                with fwad.dual_level():
+                    args[i] = fwad.make_dual(args[i], torch.ones_like(args[i]))
+                    with pytest.raises(NotImplementedError, match="forward-mode derivatives of %s " % name):
+                        call_(*args)
+                    with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode derivatives"):
+                        call_(*args)
+        with pytest.raises(NotImplementedError, match="forward-mode derivatives of %s " % name):
+            torch.func.jvp(lambda k: call_(x, k, w), (k,), (torch.ones_like(k),))
+
+
+def test_forward_mode_is_refused():
+    from batch_first_amd import ops                # noqa: F401  registers the operators
+    refuses_tangents(1, "cpu")
+
+
 # ---- on the GPU ------------------------------------------------------------------------------------------------------
 
 @pytest.fixture(scope="module")
@@ -889,3 +919,16 @@ def test_logits_at_the_end_of_the_range(ctx, dtype, moves):
         with np.errstate(over="ignore"):
             assert np.array_equal(got, want.astype(np.float32).astype(np.float64)), (got, want)
         assert got[0] == 0 and got[1] > 1e30
+
+
+@gpu
+def test_forward_mode_is_refused_on_the_gpu(ctx):
+    refuses_tangents(ctx.handle, "cuda")
+    # nor in the backward pass, whose incoming gradient may have a tangent
+    import torch.autograd.forward_ad as fwad
+    d = on_gpu(make(3, torch.float32))
+    k = d["k"].clone().requires_grad_()
+    loss = forward(ctx, dict(d, k=k))
+    with fwad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode derivatives"):
+        loss.backward(fwad.make_dual(d["w"], torch.ones_like(d["w"])))
+    assert k.grad is None
