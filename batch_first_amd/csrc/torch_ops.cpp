@@ -171,12 +171,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> policy_move_loss_grad(int64_t ctx
 
 // ---- autograd ------------------------------------------------------------------------------------------------------
 
-// A gradient that refuses to be differentiated once more.
-at::Tensor once(at::Tensor g) {
-    if (!at::GradMode::is_enabled() || !g.defined()) return g;
-    g = g.detach().set_requires_grad(true);
-    auto refuse = std::make_shared<torch::autograd::DelayedError>("the gradient of a batchfirst loss cannot be differentiated", 1);
-    return (*refuse)({g})[0];
+// A result that refuses to be differentiated.
+at::Tensor refusing(at::Tensor t, const char* why) {
+    if (!at::GradMode::is_enabled() || !t.defined()) return t;
+    t = t.detach().set_requires_grad(true);
+    auto refuse = std::make_shared<torch::autograd::DelayedError>(why, 1);
+    return (*refuse)({t})[0];
+}
+at::Tensor once(at::Tensor g) { return refusing(g, "the gradient of a batchfirst loss cannot be differentiated"); }
+bool any_requires_grad(at::ArrayRef<at::Tensor> inputs) {
+    return at::GradMode::is_enabled() && std::any_of(inputs.begin(), inputs.end(), [](const at::Tensor& t) { return t.requires_grad(); });
 }
 
 // The capture a stream belongs to, 0 if none.  The default stream never belongs to one and must not be asked during one.
@@ -243,37 +247,48 @@ struct Loss : torch::autograd::Function<Loss> {
     }
 };
 
-bool differentiable(const at::Tensor& a, const at::Tensor& b) { return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad()); }
-
 at::Tensor policy_loss_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel, const at::Tensor& targets) {
     no_tangents({features, kernel}, "policy_loss");
-    if (differentiable(features, kernel)) return Loss::apply(ctx, features, kernel, targets, Lists(), Lists(), Lists());
+    if (any_requires_grad({features, kernel})) return Loss::apply(ctx, features, kernel, targets, Lists(), Lists(), Lists());
     at::AutoDispatchBelowADInplaceOrView below;
     return policy_loss(ctx, features, kernel, targets);
 }
 at::Tensor policy_move_loss_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel, const at::Tensor& from_squares,
                                      const at::Tensor& move_filters, const at::Tensor& moves_per_board, const at::Tensor& targets) {
     no_tangents({features, kernel}, "policy_move_loss");
-    if (differentiable(features, kernel)) return Loss::apply(ctx, features, kernel, targets, Lists(from_squares), Lists(move_filters), Lists(moves_per_board));
+    if (any_requires_grad({features, kernel})) return Loss::apply(ctx, features, kernel, targets, Lists(from_squares), Lists(move_filters), Lists(moves_per_board));
     at::AutoDispatchBelowADInplaceOrView below;
     return policy_move_loss(ctx, features, kernel, from_squares, move_filters, moves_per_board, targets);
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor> policy_loss_grad_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel,
-                                                                         const at::Tensor& targets, const at::Tensor& board_weights,
-                                                                         bool features_grad, bool kernel_grad) {
-    no_tangents({features, kernel, board_weights}, "policy_loss_grad");
-    at::AutoDispatchBelowADInplaceOrView below;
-    return policy_loss_grad(ctx, features, kernel, targets, board_weights, features_grad, kernel_grad);
+// The one-pass forms: their gradients come without a graph, as those that a backward pass leaves; their losses would end one
+// without a word, and refuse instead.
+using Grads = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+Grads refusing_loss(Grads out, at::ArrayRef<at::Tensor> inputs) {
+    if (any_requires_grad(inputs))
+        std::get<0>(out) = refusing(std::get<0>(out), "the loss of a batchfirst _grad form cannot be differentiated: its gradients are beside it");
+    return out;
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor> policy_move_loss_grad_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel,
-                                                                              const at::Tensor& from_squares, const at::Tensor& move_filters,
-                                                                              const at::Tensor& moves_per_board, const at::Tensor& targets,
-                                                                              const at::Tensor& board_weights, bool features_grad,
-                                                                              bool kernel_grad) {
+Grads policy_loss_grad_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel, const at::Tensor& targets,
+                                const at::Tensor& board_weights, bool features_grad, bool kernel_grad) {
+    no_tangents({features, kernel, board_weights}, "policy_loss_grad");
+    Grads out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        out = policy_loss_grad(ctx, features, kernel, targets, board_weights, features_grad, kernel_grad);
+    }
+    return refusing_loss(std::move(out), {features, kernel, board_weights});
+}
+Grads policy_move_loss_grad_autograd(int64_t ctx, const at::Tensor& features, const at::Tensor& kernel, const at::Tensor& from_squares,
+                                     const at::Tensor& move_filters, const at::Tensor& moves_per_board, const at::Tensor& targets,
+                                     const at::Tensor& board_weights, bool features_grad, bool kernel_grad) {
     no_tangents({features, kernel, board_weights}, "policy_move_loss_grad");
-    at::AutoDispatchBelowADInplaceOrView below;
-    return policy_move_loss_grad(ctx, features, kernel, from_squares, move_filters, moves_per_board, targets, board_weights, features_grad,
-                                 kernel_grad);
+    Grads out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        out = policy_move_loss_grad(ctx, features, kernel, from_squares, move_filters, moves_per_board, targets, board_weights,
+                                    features_grad, kernel_grad);
+    }
+    return refusing_loss(std::move(out), {features, kernel, board_weights});
 }
 
 // ---- norms ---------------------------------------------------------------------------------------------------------
@@ -352,8 +367,12 @@ at::Tensor clip_grad_norm_(int64_t ctx, at::TensorList tensors, double max_norm)
 
 at::Tensor global_norm_autograd(int64_t ctx, at::TensorList tensors) {
     no_tangents(tensors, "global_norm");
-    at::AutoDispatchBelowADInplaceOrView below;
-    return global_norm(ctx, tensors);
+    at::Tensor norm;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        norm = global_norm(ctx, tensors);
+    }
+    return any_requires_grad(tensors) ? refusing(norm, "global_norm cannot be differentiated") : norm;
 }
 at::Tensor clip_grad_norm_autograd(int64_t ctx, at::TensorList tensors, double max_norm) {
     no_tangents(tensors, "clip_grad_norm_");
@@ -398,7 +417,7 @@ TORCH_LIBRARY_IMPL(batchfirst, CompositeExplicitAutograd, m) {
 TORCH_LIBRARY_IMPL(batchfirst, Autograd, m) {
     m.impl("policy_loss", policy_loss_autograd);
     m.impl("policy_move_loss", policy_move_loss_autograd);
-    // not differentiable: what they return does not require grad
+    // not differentiable
     m.impl("policy_loss_grad", policy_loss_grad_autograd);
     m.impl("policy_move_loss_grad", policy_move_loss_grad_autograd);
     m.impl("global_norm", global_norm_autograd);

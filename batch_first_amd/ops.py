@@ -28,8 +28,11 @@ board's own moves, as ``policy_scores`` takes them; a target is a place in the b
 differentiable in the features and the kernel; the ``_grad`` forms give the losses and the gradients of
 sum(board_weights * loss) in one pass where the boards' weights (f32[N] or [1]) are known beforehand, and an empty tensor
 for a gradient that is not asked for.  No call waits for the device: targets, squares and filters out of range, and lists
-that do not add up, are reported by :meth:`DeviceContext.check_policy` afterwards (a target then counts as -1).  Gradients
-are not differentiated once more, and a tensor with a forward-mode tangent is refused (NotImplementedError) by all six.
+that do not add up, are reported by :meth:`DeviceContext.check_policy` afterwards (a target then counts as -1).
+
+Gradients are not differentiated once more; ``global_norm`` and the losses of the ``_grad`` forms are not differentiable
+either: of inputs that require grad they raise in a backward pass (RuntimeError), while the ``_grad`` forms' gradients carry
+no graph.  A tensor with a forward-mode tangent is refused (NotImplementedError) by all six.
 ``clip_grad_norm_`` scales by min(1, max_norm / (norm + 1e-6)) and returns the norm before.
 
 ``ctx`` is the integer handle of a :class:`DeviceContext`.  occupied_bbs travels as int64

@@ -356,3 +356,17 @@ def test_forward_mode_is_refused():
 @gpu
 def test_forward_mode_is_refused_on_the_gpu(ctx):
     refuses_tangents(ctx.handle, "cuda")
+
+
+@gpu
+def test_the_norm_refuses_to_be_differentiated(ctx):
+    """A norm without a graph in a sum of losses would train without its part."""
+    o = torch.ops.batchfirst
+    a, b = torch.randn(300, device="cuda"), torch.randn(20, 7, device="cuda", requires_grad=True)
+    want = o.global_norm(ctx.handle, [a, b.detach()])
+    norm = o.global_norm(ctx.handle, [a, b])
+    assert not want.requires_grad and norm.requires_grad and torch.equal(norm.detach(), want) and norm.item() == want.item()
+    with pytest.raises(RuntimeError, match="global_norm cannot be differentiated"):
+        (b.sum() + norm).backward()
+    with torch.no_grad():
+        assert not o.global_norm(ctx.handle, [a, b]).requires_grad

@@ -932,3 +932,21 @@ def test_forward_mode_is_refused_on_the_gpu(ctx):
     with fwad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode derivatives"):
         loss.backward(fwad.make_dual(d["w"], torch.ones_like(d["w"])))
     assert k.grad is None
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_the_loss_of_a_grad_form_refuses_to_be_differentiated(ctx, moves):
+    """It would end the graph without a word; the gradients beside it come without one, as a backward pass leaves them."""
+    d = on_gpu(make(5, torch.float32, seed=2, moves=moves))
+    want = call(ctx, d)
+    for name in ("x", "k", "w"):
+        loss, dx, dk = call(ctx, dict(d, **{name: d[name].clone().requires_grad_()}))
+        assert all(torch.equal(a, b) for a, b in zip((loss.detach(), dx, dk), want))
+        assert loss.requires_grad and not dx.requires_grad and not dk.requires_grad
+        with pytest.raises(RuntimeError, match="cannot be differentiated"):
+            loss.sum().backward()
+        torch.ops.batchfirst.clip_grad_norm_(ctx.handle, [dk.clone()], 1.0)
+        with torch.no_grad():
+            assert not call(ctx, dict(d, **{name: d[name].clone().requires_grad_()}))[0].requires_grad
+    assert not want[0].requires_grad
