@@ -8,6 +8,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -352,8 +353,11 @@ at::Tensor global_norm(int64_t ctx, at::TensorList tensors) {
 }
 
 at::Tensor clip_grad_norm_(int64_t ctx, at::TensorList tensors, double max_norm) {
-    for (const at::Tensor& t : tensors)
+    for (const at::Tensor& t : tensors) {
         TORCH_CHECK_VALUE(!t.requires_grad(), "tensors to clip are gradients: they must not require grad themselves");
+        // torch says so itself, but only where the new version is noted, with the tensors scaled already
+        TORCH_CHECK_VALUE(!t.is_inference() || c10::InferenceMode::is_enabled(), "an inference tensor cannot be clipped outside inference mode");
+    }
     check_gapped(tensors);
     const Tables t(ctx, tensors);
     check(lib.clip_grad_norm(t.c.ctx, t.ptrs.data(), t.counts.data(), t.types.data(), t.ptrs.size(), (float)max_norm,

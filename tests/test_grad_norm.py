@@ -370,3 +370,28 @@ def test_the_norm_refuses_to_be_differentiated(ctx):
         (b.sum() + norm).backward()
     with torch.no_grad():
         assert not o.global_norm(ctx.handle, [a, b]).requires_grad
+
+
+def clips_no_inference_tensors(handle, device):
+    """Outside inference mode they may not be changed in place; that is said before they are."""
+    o = torch.ops.batchfirst
+    with torch.inference_mode():
+        t = torch.ones(6, device=device)
+    for tensors in ([t], [torch.ones(3, device=device), t.view(2, 3).t()[:2]]):
+        with pytest.raises(ValueError, match="inference tensor"):
+            o.clip_grad_norm_(handle, tensors, 0.5)
+    assert torch.equal(t.clone(), torch.ones(6, device=device))
+    return t
+
+
+def test_inference_tensors_are_not_clipped():
+    from batch_first_amd import ops                # noqa: F401  registers the operators
+    clips_no_inference_tensors(1, "cpu")
+
+
+@gpu
+def test_inference_tensors_are_clipped_in_inference_mode(ctx):
+    t = clips_no_inference_tensors(ctx.handle, "cuda")
+    with torch.inference_mode():
+        norm = torch.ops.batchfirst.clip_grad_norm_(ctx.handle, [t], 0.5)
+        assert float(norm) == pytest.approx(6 ** 0.5) and float(t.norm()) == pytest.approx(0.5, rel=1e-5)
