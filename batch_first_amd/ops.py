@@ -48,7 +48,18 @@ from . import _lib
 from .chestimator import _as_blob, _as_policy_blob
 
 _contexts = {}
-_torch = _lib.load_torch()
+# Evaluation needs libbatchfirst_hip.so alone: where the training operators' library is missing, or does not fit this torch,
+# they say so when they are called.
+_torch, _torch_error = None, None
+try:
+    _torch = _lib.load_torch()
+except (ImportError, OSError) as e:
+    _torch_error = "the training operators are not available: %s" % e
+
+
+def _announce(ctx, device):
+    if _torch is not None:
+        _torch.bf_torch_context(ctx, device)
 
 
 class DeviceContext:
@@ -64,7 +75,7 @@ class DeviceContext:
         self.device = torch.device("cuda", int(device))
         self.handle = int(ctx.value)
         _contexts[self.handle] = self
-        _torch.bf_torch_context(ctx, int(device))
+        _announce(ctx, int(device))
 
     def set_policy(self, policy_weights):
         blob = _as_policy_blob(policy_weights)
@@ -80,7 +91,7 @@ class DeviceContext:
     def close(self):
         if self._ctx is not None:
             _contexts.pop(self.handle, None)
-            _torch.bf_torch_context(self._ctx, -1)
+            _announce(self._ctx, -1)
             self._lib.bf_ctx_destroy(self._ctx)
             self._ctx = None
 
@@ -233,12 +244,21 @@ def policy_scores(ctx: int, features: torch.Tensor, from_squares: torch.Tensor, 
 
 # The training operators are registered by libbatchfirst_torch.so (csrc/torch_ops.cpp), in C++ because their calls are as
 # short as a Python body's own time.
-policy_loss = torch.ops.batchfirst.policy_loss
-policy_loss_grad = torch.ops.batchfirst.policy_loss_grad
-policy_move_loss = torch.ops.batchfirst.policy_move_loss
-policy_move_loss_grad = torch.ops.batchfirst.policy_move_loss_grad
-global_norm = torch.ops.batchfirst.global_norm
-clip_grad_norm_ = torch.ops.batchfirst.clip_grad_norm_
+def _training(name):
+    if _torch is not None:
+        return getattr(torch.ops.batchfirst, name)
+
+    def unavailable(*args, **kwargs):
+        raise ImportError(_torch_error)
+    return unavailable
+
+
+policy_loss = _training("policy_loss")
+policy_loss_grad = _training("policy_loss_grad")
+policy_move_loss = _training("policy_move_loss")
+policy_move_loss_grad = _training("policy_move_loss_grad")
+global_norm = _training("global_norm")
+clip_grad_norm_ = _training("clip_grad_norm_")
 
 
 def eval_mailbox_debug(ctx, mailbox):

@@ -17,6 +17,7 @@ Tolerances, with u = 2^-24 (half a step of float32), eps(t) / 2 half a step of t
   times as there are terms: 73 or 64.
 """
 import ctypes
+import os
 
 import numpy as np
 import pytest
@@ -203,6 +204,37 @@ def refuses_tangents(handle, device):
 def test_forward_mode_is_refused():
     from batch_first_amd import ops                # noqa: F401  registers the operators
     refuses_tangents(1, "cpu")
+
+
+@pytest.mark.parametrize("library", ["missing", "unloadable"])
+def test_evaluation_ops_need_no_training_library(tmp_path, library):
+    """Without libbatchfirst_torch.so, or with one that does not load, the other ops are there and these say what is wrong."""
+    import subprocess
+    import sys
+    path = tmp_path / "libbatchfirst_torch.so"
+    if library == "unloadable":
+        path.write_bytes(b"not a library")
+    code = """
+import torch
+from batch_first_amd import _lib
+_lib.TORCH_PATH = %r
+from batch_first_amd import ops
+assert torch.ops.batchfirst.eval_structs is not None and callable(ops.policy_scores)
+try:
+    torch.ops.batchfirst.eval_structs(1, torch.zeros(1, 82, dtype=torch.uint8))
+except ValueError as e:
+    assert "unknown batchfirst context" in str(e)
+ops._announce(None, 0)
+for name in ("policy_loss", "policy_loss_grad", "policy_move_loss", "policy_move_loss_grad", "global_norm", "clip_grad_norm_"):
+    try:
+        getattr(ops, name)(1, [])
+        raise SystemExit(name)
+    except ImportError as e:
+        assert "training operators are not available" in str(e) and _lib.TORCH_PATH in str(e), e
+""" % str(path)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr[-2000:]
 
 
 # ---- on the GPU ------------------------------------------------------------------------------------------------------
