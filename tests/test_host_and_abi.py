@@ -143,3 +143,48 @@ def test_t16_image_drives_kernel_model_to_bf16_oracle(golden):
     assert np.max(np.abs(scores - ref)) <= 1e-6
     assert mfmas == 2468    # 39 488 matrix-pipe cycles a board: DESIGN.md 3.2
     assert lib.bf_pack_weights_t16(blob.ctypes.data, blob.size, image.ctypes.data, image.size - 1) == _lib.BF_E_ARG
+
+
+def _script(path, text):
+    path.write_text("#!/bin/sh\n" + text)
+    path.chmod(0o755)
+    return str(path)
+
+
+def test_makefile_follows_torch(tmp_path):
+    """The torch registration is built again for another torch, and left out where there is none."""
+    import shutil
+    import subprocess
+    csrc = tmp_path / "pkg" / "csrc"
+    csrc.mkdir(parents=True)
+    (tmp_path / "include").mkdir()
+    (tmp_path / "include" / "batchfirst.h").touch()
+    here = os.path.join(ROOT, "batch_first_amd", "csrc")
+    shutil.copy(os.path.join(here, "Makefile"), csrc)
+    for name in os.listdir(here):
+        if name.endswith((".h", ".hip", ".cpp")):
+            (csrc / name).touch()
+    torch_dir = tmp_path / "torch"
+    torch_dir.mkdir()
+    log = tmp_path / "log"
+    # a compiler that writes down what it is asked for and touches it
+    compiler = _script(tmp_path / "cc", 'while [ $# -gt 0 ]; do [ "$1" = -o ] && { touch "$2"; echo "$2" >> %s; }; shift; done\n' % log)
+    python = _script(tmp_path / "python", 'echo "%s"\n' % torch_dir)
+
+    def make(target, python=python):
+        log.write_text("")
+        subprocess.run(["make", "-s", "-C", str(csrc), target, "CXX=" + compiler, "HIPCC=" + compiler, "ISA_CHECK=true",
+                        "PYTHON=" + python], check=True, capture_output=True, timeout=60)
+        return log.read_text().split()
+
+    (torch_dir / "version.py").write_text("__version__ = '1'\n")
+    assert make("torch") == ["../libbatchfirst_torch.so"]
+    assert make("torch") == []
+    (torch_dir / "version.py").write_text("__version__ = '2'\n")
+    os.utime(torch_dir / "version.py", (1, 1))      # an installer may keep the package's own time
+    assert make("torch") == ["../libbatchfirst_torch.so"]
+    assert make("torch") == []
+    (tmp_path / "pkg" / "libbatchfirst_torch.so").unlink()
+    built = make("all", _script(tmp_path / "no_torch", "exit 1\n"))
+    assert "../libbatchfirst_hip.so" in built and "../libbatchfirst_torch.so" not in built
+    assert "../libbatchfirst_torch.so" in make("all")
