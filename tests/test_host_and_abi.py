@@ -188,3 +188,27 @@ def test_makefile_follows_torch(tmp_path):
     built = make("all", _script(tmp_path / "no_torch", "exit 1\n"))
     assert "../libbatchfirst_hip.so" in built and "../libbatchfirst_torch.so" not in built
     assert "../libbatchfirst_torch.so" in make("all")
+
+
+def test_a_variant_of_the_library_has_all_of_it():
+    """tools/build_variant.sh builds one kernel file with other flags; the rest, and the flags, are the Makefile's."""
+    import shutil
+    import subprocess
+    import sys
+    name, csrc = "of_the_tests", os.path.join(ROOT, "batch_first_amd", "csrc")
+    objects = subprocess.run(["make", "-s", "-C", csrc, "objects"], check=True, capture_output=True, text=True).stdout.split()
+    if not all(os.path.exists(os.path.join(csrc, o)) for o in objects):
+        pytest.skip("the library's object files are not here")
+    subprocess.run([os.path.join(ROOT, "tools", "build_variant.sh"), name, "grad_norm", "-DNOT_USED"], check=True, capture_output=True, timeout=300)
+    variant = os.path.join(ROOT, "build", "variants", "libbf_%s.so" % name)
+    out = subprocess.run([sys.executable, "-c", "from batch_first_amd import _lib; print(_lib.load().bf_version(), _lib.LIB_PATH)"],
+                         cwd=ROOT, env=dict(os.environ, BATCHFIRST_LIB=variant), capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and variant in out.stdout, out.stderr[-2000:]
+    os.unlink(variant)
+    shutil.rmtree(os.path.join(ROOT, "build", "variants", "obj_" + name))
+
+    def flags(target):
+        return subprocess.run(["make", "-s", "-C", csrc, "flags-" + target], check=True, capture_output=True, text=True).stdout
+
+    for target in ("eval_f32.o", "eval_t16.o", "eval_t16s.o", "policy_loss.o"):
+        assert "-packed-fp32-ops" in flags(target) and ("-amdgpu-mfma-vgpr-form" in flags(target)) == ("t16" in target)
