@@ -982,3 +982,127 @@ def test_the_loss_of_a_grad_form_refuses_to_be_differentiated(ctx, moves):
         with torch.no_grad():
             assert not call(ctx, dict(d, **{name: d[name].clone().requires_grad_()}))[0].requires_grad
     assert not want[0].requires_grad
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("n", [1, 70, 2600])
+def test_one_gradient_alone(ctx, n, dtype, moves):
+    """Either gradient without the other, and without the losses, is what both together give."""
+    case = make(n, dtype, seed=40 + n, moves=moves, longest=80)
+    case["t"][0] = 0 if not moves or case["moves"][2][0] else -1
+    d = on_gpu(case)
+    loss, dx, dk = call(ctx, d)
+    one, other = call(ctx, d, kernel_grad=False), call(ctx, d, features_grad=False)
+    assert torch.equal(one[0], loss) and torch.equal(one[1], dx) and one[2].numel() == 0
+    assert torch.equal(other[0], loss) and other[1].numel() == 0 and torch.equal(other[2], dk)
+    o = torch.ops.batchfirst
+    op = o.policy_move_loss if moves else o.policy_loss
+    for name, want in (("x", dx), ("k", dk)):
+        leaf = d[name].clone().requires_grad_()
+        e = dict(d, **{name: leaf})
+        got, = torch.autograd.grad((op(ctx.handle, e["x"], e["k"], *d["lists"], d["t"]) * d["w"]).sum(), leaf)
+        assert torch.equal(got, want)
+    # the C entry may leave the losses out
+    lib, p = _lib.load(), lambda t: ctypes.c_void_p(t.data_ptr())
+    work = torch.empty(lib.bf_policy_loss_workspace(n), dtype=torch.uint8, device="cuda")
+    again = torch.empty_like(dx), torch.empty_like(dk)
+    type_ = TYPES.index(dtype)
+    tail = (p(d["t"]), p(d["w"]), n, None, p(again[0]), p(again[1]), p(work), work.numel(),
+            ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    if moves:
+        sq, fl, per = d["lists"]
+        rc = lib.bf_policy_move_loss_grad(ctypes.c_void_p(ctx.handle), p(d["x"]), type_, n, p(d["k"]), p(sq), p(fl), p(per), sq.numel(), *tail)
+    else:
+        rc = lib.bf_policy_loss_grad(ctypes.c_void_p(ctx.handle), p(d["x"]), type_, n, p(d["k"]), *tail)
+    assert rc == 0 and torch.equal(again[0], dx) and torch.equal(again[1], dk)
+    ctx.check_policy()
+
+
+def check_on_gpu(ctx, case):
+    """As check_all, with the definitions in float64 on the GPU: for many boards.
+
+    The kernel's gradient adds a board's 64 products and then the boards of a wave, of 2 048, one by one, and the waves of a
+    workgroup: 64 + n / 2048 + 8 roundings, which limits()' 600 covers up to a million boards."""
+    n, dtype = len(case["t"]), case["x"].dtype
+    assert n <= 1 << 20
+    d = on_gpu(case)
+    loss, dx, dk = call(ctx, d)
+    k = d["k"].double()
+    k_most = float(k.abs().max())
+    flush = 3 * 2.0 ** -126 * float(case["w"].max())
+    half, least = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    split = 0.0 if dtype == torch.float32 else 2.0 ** -17
+    want_dk, size_dk, p_most, x_most, lost_dk = torch.zeros_like(k), torch.zeros_like(k), 0.0, 0.0, 0.0
+    starts = torch.cumsum(d["lists"][2].long(), 0) - d["lists"][2].long() if d["lists"] else None
+    for lo in range(0, n, 4096):
+        x = d["x"][lo:lo + 4096].double().reshape(-1, 32, 64)
+        m = len(x)
+        t, w = d["t"][lo:lo + m], d["w"][lo:lo + m].double()
+        has = t >= 0
+        logits, size = (torch.matmul(a.t().contiguous(), b).flatten(1) for a, b in ((k, x), (k.abs(), x.abs())))
+        if starts is None:
+            listed, target = torch.ones_like(logits), t.clamp(min=0)
+        else:
+            sq, fl, per = (a.long() for a in d["lists"])
+            first, count = int(starts[lo]), int(per[lo:lo + m].sum())
+            places = fl[first:first + count] * 64 + sq[first:first + count]
+            board = torch.repeat_interleave(torch.arange(m, device="cuda"), per[lo:lo + m])
+            listed = torch.zeros_like(logits).index_put_((board, places), torch.ones_like(places, dtype=torch.float64), accumulate=True)
+            target = places[(starts[lo:lo + m] - first + t.clamp(min=0)).clamp(max=count - 1)]
+            listed[~has, 0] = 1
+        inside = listed > 0
+        top = logits.masked_fill(~inside, -float("inf")).amax(1)
+        spread = (top - logits.masked_fill(~inside, float("inf")).amin(1)) * has
+        e = torch.where(inside, listed * torch.exp(torch.clamp(logits - top[:, None], max=0.0)), 0.0)
+        z = e.sum(1, keepdim=True)
+        hot = torch.zeros_like(e).scatter_(1, target[:, None], 1.0)
+        want = torch.where(has, torch.log(z)[:, 0] + top - logits.gather(1, target[:, None])[:, 0], 0.0)
+        dl = 40 * U * size.masked_fill(~inside, 0.0).amax(1) * has
+        p = 2 * dl + U * (2 * spread + 100)
+        off = (loss[lo:lo + m].double() - want).abs() - (2 * dl + 16 * U * (1 + want + (top * has).abs()))
+        assert bool((off <= 0).all()), ("loss", float(off.max()))
+        w = (w * has)[:, None]
+        g, s = ((e / z - hot) * w).view(m, 73, 64), ((e / z + hot) * w.abs()).view(m, 73, 64)
+        lost = 2.0 ** -37 * d["w"][lo:lo + m].double() * torch.clamp(-torch.expm1(-want), min=2.0 ** -17)
+        want_dx = torch.matmul(k, g)
+        tol = (p[:, None, None] + U * 80 + split) * torch.matmul(k.abs(), s) + half * want_dx.abs() + least + flush * 73 * k_most
+        off = (dx[lo:lo + m].double().view(m, 32, 64) - want_dx).abs() - tol - (lost * 75 * k_most)[:, None, None]
+        assert bool((off <= 0).all()), ("d_features", float(off.max()))
+        want_dk += torch.matmul(x, g.transpose(1, 2).contiguous()).sum(0)
+        size_dk += torch.matmul(x.abs(), s.transpose(1, 2).contiguous()).sum(0)
+        most = x.abs().amax((1, 2))
+        p_most, x_most, lost_dk = max(p_most, float(p.max())), max(x_most, float(most.max())), lost_dk + float((lost * 66 * most).sum())
+    tol = (p_most + U * 600 + split) * size_dk + half * want_dk.abs() + least + flush * 64 * n * x_most + lost_dk
+    off = (dk.double() - want_dk).abs() - tol
+    assert bool((off <= 0).all()), ("d_kernel", float(off.max()))
+    only = call(ctx, d, features_grad=False)
+    assert torch.equal(only[0], loss) and torch.equal(only[2], dk)
+    ctx.check_policy()
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_kernel_gradient_of_many_boards(ctx, dtype, moves):
+    """Ten boards a wave, read ahead one by one."""
+    check_on_gpu(ctx, make(20011, dtype, seed=51, moves=moves, longest=40))
+
+
+@gpu
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_kernel_gradient_of_more_boards_than_a_round(ctx, moves):
+    """A wave looks targets and lists up for 64 of its boards at a time; 2 048 waves begin another round beyond 131 072."""
+    n = 131072 + 1027
+    case = make(4001, torch.float32, seed=52, moves=moves, longest=9)
+    again = -(-n // 4001)
+    case["x"] = case["x"].repeat(again, 1, 1, 1)[:n]
+    case["w"] = torch.from_numpy(np.random.default_rng(6).uniform(0.1, 1.0, n).astype(np.float32))
+    case["t"] = case["t"].repeat(again)[:n]
+    if moves:
+        sq, fl, per = case["moves"]
+        per = np.tile(per, again)[:n]
+        m = int(per.astype(np.int64).sum())
+        case["moves"] = np.tile(sq, again)[:m], np.tile(fl, again)[:m], per
+    check_on_gpu(ctx, case)
