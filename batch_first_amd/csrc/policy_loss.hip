@@ -949,8 +949,9 @@ __global__ __launch_bounds__(512) void k_policy_move_loss(const T* __restrict__ 
                 if (64 * p + lane < count) {
                     v[p] = list.logit[64 * p + lane];
                     if constexpr (NT == 2) {
-                        v[p] *= square_back(p) * filter_back(p);
-                        if (v[p] != v[p]) {          // an infinity has no second term, and units may pass float32's range
+                        const float unit = square_back(p) * filter_back(p);
+                        v[p] *= unit;
+                        if (!(unit <= kWide)) {      // as over the vocabulary: not finite, or wide
                             v[p] = 0.0f;
                             for (int c = 0; c < kC; ++c)
                                 v[p] = fmaf((float)board[c * kS + (move[p] & 255u)], (float)w[c * kF + (move[p] >> 8)], v[p]);

@@ -1106,3 +1106,26 @@ def test_kernel_gradient_of_more_boards_than_a_round(ctx, moves):
         m = int(per.astype(np.int64).sum())
         case["moves"] = np.tile(sq, again)[:m], np.tile(fl, again)[:m], per
     check_on_gpu(ctx, case)
+
+
+@gpu
+@pytest.mark.parametrize("value", [1e3, 1e6, 1e9, 1e20])
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_a_large_factor_of_zero(ctx, moves, value):
+    """An element of the kernel, or a feature, that only meets zeros has no part in any logit, however large."""
+    for what in ("kernel", "feature"):
+        case = make(12, torch.float32, seed=61, moves=moves, longest=50)
+        x, k = case["x"].view(12, 32, 64), case["k"]
+        if what == "kernel":
+            x[:, 11], k[11, 7:9] = 0, value
+        else:
+            k[11], x[:, 11, 20:24] = 0, value
+        if moves:
+            whole_lists(case, 4)
+            sq, fl, per = case["moves"]
+            first = np.cumsum(per.astype(int)) - per
+            sq[first], fl[first], sq[first + 1], fl[first + 1] = 21, 30, 40, 7
+            case["t"] = torch.from_numpy(np.arange(12) % 4)
+        else:
+            case["t"] = torch.from_numpy(np.arange(12) * 333 + 21)
+        check_all(ctx, case)
