@@ -120,6 +120,14 @@ __device__ __forceinline__ void scale_of(float largest, int least, float& scale,
     back = __uint_as_float((unsigned)(127 - 13 + e) << 23);
 }
 
+// From the lanes' largest magnitudes to the largest of all (infinity or NaN where one is not finite); whether one that is
+// not zero lies more than 2^16 below it.
+__device__ __forceinline__ bool range_of(float& largest) {
+    const float mine = largest;
+    largest = lanes_reduce<true>(mine);
+    return __ballot(mine > 0.0f && mine < largest * 0x1p-16f) != 0;
+}
+
 constexpr int kTiles = 5;                        // of 16 filters
 constexpr int kRow = 40;                         // 16-bit elements of a row of 32 in LDS: 16 rows start in 16 different bank groups
 constexpr int kTerm = kS * kRow;                 // elements of 64 rows
@@ -134,20 +142,22 @@ struct Features {
     typename Raw<T>::type raw[8];
     u32x4 column[4][kTerms];
     float back;
+    bool uneven;
 
     __device__ __forceinline__ void load(const T* board, int col, int q) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const typename Raw<T>::type*>(board + (8 * q + i) * kS + 4 * col);
     }
-    // One scale for the board; float32: not finite where a feature is not.
+    // One scale for the board.
     __device__ __forceinline__ void convert() {
         back = 1.0f;
+        uneven = false;
         float scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};
         if constexpr (kTerms == 2) {
             float largest = 0.0f;
 #pragma unroll
             for (int i = 0; i < 32; ++i) largest = larger(largest, fabsf(raw[i >> 2][i & 3]));
-            largest = lanes_reduce<true>(largest);
+            uneven = range_of(largest);
             scale_of(largest, -100, scale[0], back);
             scale[1] = scale[2] = scale[3] = scale[0];
         }
@@ -256,8 +266,9 @@ __device__ __forceinline__ void store_part(const f32x4 (&dw)[2][kTiles], unsigne
 // The kernel's scale, by its largest element.  Every wave looks at all of it (9 KB out of the cache, loads that are
 // in flight beside those of its operands), which spares a pass through LDS and a barrier.
 template <typename T>
-__device__ __forceinline__ void head_scale(const T* __restrict__ w, int lane, float& scale, float& back) {
+__device__ __forceinline__ bool head_scale(const T* __restrict__ w, int lane, float& scale, float& back) {
     scale = back = 1.0f;
+    bool uneven = false;
     if constexpr (Arith<T>::kTerms == 2) {
         constexpr int kPieces = kXW / 4, kLoads = (kPieces + 63) / 64;
         f32x4 v[kLoads];
@@ -266,8 +277,10 @@ __device__ __forceinline__ void head_scale(const T* __restrict__ w, int lane, fl
         float largest = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4 * kLoads; ++i) largest = larger(largest, fabsf(v[i >> 2][i & 3]));
-        scale_of(lanes_reduce<true>(largest), -100, scale, back);
+        uneven = range_of(largest);
+        scale_of(largest, -100, scale, back);
     }
+    return uneven;
 }
 
 // Eight values as an operand.
@@ -328,9 +341,11 @@ struct HeadLds {                                 // the kernel as operands, 16 b
 constexpr int kWaveLds = 2 * kTerm * 2;          // bytes a wave: the crossing
 static_assert(kWaveLds >= kPartBytes, "at the end it takes the wave's kernel gradient");
 
-// A float32 board whose largest feature and the kernel's largest element make 2^12 or more, or are not finite.  What two
-// float16 terms lose, 2^-38 of the largest, would begin to show in logits that the largest take no part in (a filter that a
-// column of -1e30 takes out of the softmax, say), so such a board goes by float32 MFMAs, which take a few times as long.
+// Two float16 terms lose 2^-38 of the largest factor.  That shows where the largest takes no part: in logits, where a filter
+// that a column of -1e30 takes out of the softmax makes the others' products small beside it, in gradients too where the
+// products are ordinary.  So a float32 board goes by float32 MFMAs, three times as long (65 536 in 1.16 ms), if its largest
+// feature and the kernel's largest element make 2^12 or more or are not finite, or if features or kernel are uneven:
+// some lane's 32 and more have a largest 2^16 below the largest of all.
 constexpr float kWide = 0x1p-16f;                // 2^(12 - 2) by the scales' reciprocals, 2^-13 each
 
 __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -457,6 +472,7 @@ __global__ __launch_bounds__(512, WANT ? 2 : 3) void k_policy_loss(const T* __re
     if (base < n) features.load(x + base * (kC * kS), col, q);
 
     float w_back;
+    bool w_uneven;
     {
         // an operand a wave at a time: five for the logits, six for the way back; all of a wave's are read at once
         constexpr int kOperands = kTiles + (WANT & kFeaturesGrad ? 6 : 0), kRounds = (kOperands + 3) / 4;
@@ -472,7 +488,7 @@ __global__ __launch_bounds__(512, WANT ? 2 : 3) void k_policy_loss(const T* __re
             }
         }
         float w_scale;
-        head_scale<T>(w, lane, w_scale, w_back);
+        w_uneven = head_scale<T>(w, lane, w_scale, w_back);
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
             const int i = wave + r * waves, j = i - kTiles;
@@ -579,7 +595,7 @@ __global__ __launch_bounds__(512, WANT ? 2 : 3) void k_policy_loss(const T* __re
                 rz = __builtin_amdgcn_rcpf(z);
                 d_target = at_target([&](float e) { return e - (lane == t_lane ? z : 0.0f); }) * rz;
             };
-            if (NT == 2 && __builtin_expect(!(w_back * x_back <= kWide), 0)) {
+            if (NT == 2 && __builtin_expect(!(w_back * x_back <= kWide) || w_uneven || features.uneven, 0)) {
                 const T* board = x + b * (kC * kS);
                 f32x16 v[kTiles];
                 wide_logits(board, w, col, q, v);

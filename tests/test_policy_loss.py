@@ -1129,3 +1129,45 @@ def test_a_large_factor_of_zero(ctx, moves, value):
         else:
             case["t"] = torch.from_numpy(np.arange(12) * 333 + 21)
         check_all(ctx, case)
+
+
+@gpu
+@pytest.mark.parametrize("what", ["filter", "square"])
+@pytest.mark.parametrize("moves", [False, True], ids=["vocabulary", "moves"])
+def test_large_values_beside_small_factors(ctx, moves, what):
+    """As test_logits_far_below_the_others with products of ordinary size: values of 1e8 and more, taken out of the softmax,
+    meet factors of 2^-20 and less.  The gradients of what is left have the ordinary values' precision."""
+    case = make(9, torch.float32, seed=24, moves=moves)
+    case["x"] += 0.25
+    x, k = case["x"].view(9, 32, 64), case["k"]
+    if what == "filter":
+        x *= 2.0 ** -20
+        k[:, 7], k[:, 64] = -1e8, -0.5e8         # 32 channels of 2^-22 and more: -380 and below
+        masked = lambda f, s: (f == 7) | (f == 64)
+    else:
+        k *= 2.0 ** -20
+        k[11] = -(k[11].abs() + 0.125 * 2.0 ** -20)
+        x[:, 11, 5], x[:, 11, 63] = 4e9, 2e9     # -230 and below
+        masked = lambda f, s: (s == 5) | (s == 63)
+    if moves:
+        sq, fl, per = whole_lists(case, 3)
+        first = np.cumsum(per.astype(int)) - per
+        sq[first], fl[first], sq[first + 1], fl[first + 1] = 5, 7, 9, 11
+        case["t"] = torch.ones(9, dtype=torch.int64)
+    else:
+        case["t"] = torch.arange(9) + 64 * 20 + 10
+    left = without(case, masked)
+    small = dict(left, x=case["x"].clone(), k=case["k"].clone())
+    if what == "filter":
+        small["k"][:, 7] = small["k"][:, 64] = 0
+    else:
+        small["x"].view(9, 32, 64)[:, 11, 5] = small["x"].view(9, 32, 64)[:, 11, 63] = 0
+    ref = reference(small)
+    tol = limits(ref, small)
+    d = on_gpu(case)
+    # what is taken out has probabilities of e^-230 at most, times values of 4e9 below every tolerance
+    close(forward(ctx, d), ref["loss"], tol[0], "loss")
+    got = call(ctx, d)
+    close(got[1], ref["d_features"], tol[1], "d_features")
+    close(got[2], ref["d_kernel"], tol[2], "d_kernel")
+    assert torch.equal(call(ctx, d, kernel_grad=False)[1], got[1]) and torch.equal(call(ctx, d, features_grad=False)[2], got[2])
