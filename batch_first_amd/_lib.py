@@ -15,7 +15,6 @@ TORCH_PATH = os.path.join(_HERE, "libbatchfirst_torch.so")
 BF_OK, BF_E_ARG, BF_E_HIP, BF_E_FORMAT, BF_E_NOGPU = 0, -1, -2, -3, -4
 BF_PRECISION_F32, BF_PRECISION_BF16, BF_PRECISION_F32_SPLIT, BF_PRECISION_F32_SPLIT3 = 0, 1, 2, 3
 BF_TYPE_F32, BF_TYPE_BF16, BF_TYPE_F16 = 0, 1, 2
-BF_POLICY_VOCABULARY = 4672
 BF_NOALLOC_MAX_BOARDS = 262144
 BF_SPLIT_BOARDS_DEFAULT = 512
 PRECISIONS = {"f32": BF_PRECISION_F32, "fp32": BF_PRECISION_F32, "float32": BF_PRECISION_F32,

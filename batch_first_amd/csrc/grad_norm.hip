@@ -7,8 +7,9 @@
 // many tensors it spans, with 16-byte accesses and four of them in flight a thread, and leaves one partial sum; every
 // workgroup of the scaling pass adds the partial sums up by itself, in the same fixed order, which spares a launch between the two.
 // The scaling pass walks its run backwards, so that it begins with what the first pass has left in the caches (100 M float32
-// elements clipped in 208 us; forwards 253).  The norm of 268 M float32 elements takes 182 us, 5.9 TB/s; clipping 307
-// bfloat16 tensors of 60 M elements 81 us, of which 78 on the GPU, 4.6 TB/s for reading twice and writing once.  A few chunks, as a head's own gradient, take one workgroup and one launch.
+// elements clipped in 208 us; forwards 253).  The norm of 268 M float32 elements takes 181 us, 5.9 TB/s; clipping 307
+// bfloat16 tensors of 60 M elements 83 us, of which 77 on the GPU, 4.7 TB/s for reading twice and writing once.  A few
+// chunks, as a head's own gradient, take one workgroup and one launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

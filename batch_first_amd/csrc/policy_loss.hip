@@ -30,9 +30,12 @@ constexpr int kC = 32, kS = 64, kF = 73, kVocab = kF * kS, kXW = kC * kF;
 //
 // float32 operands travel as two float16 terms (22 bits), scaled by a power of two so that the larger term stays normal
 // down to 2^-27 of the largest: over the vocabulary the kernel's by its largest element and the features' by the board's,
-// over moves by the filter's and by the square's; of the four products of terms the least is left out (2^-22).  bfloat16 and float16 operands are exact as they are.  The logits'
-// gradients d (before the weight) travel as two terms: bfloat16 ones for bfloat16 features, else float16 ones, scaled like
-// the features.  Their largest is the target's, which is the negative sum of all the others.
+// over moves by the filter's and by the square's; of the four products of terms the least is left out (2^-22).  (float32
+// MFMAs alone would take 384 us for the 65 536 boards below that take 276.)  Where the largest may take no part in a sum and
+// the bits below it count, the sum is float32 throughout: kWide below.  bfloat16 and float16 operands are exact as they are.
+// The logits' gradients d (before the weight) travel as two terms: float16 ones, scaled like the features, or for bfloat16
+// features bfloat16 ones (16 bits, 2^-17 of d beside the 2^-8 of their result's rounding).  Their largest is the target's,
+// which is the negative sum of all the others.
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -328,10 +331,10 @@ enum { kFeaturesGrad = 1, kKernelGrad = 2 };
 //            or filters at a time, as they lie in the lanes, and read transposed (32 filters at a time); the sums stay
 //            in registers over all the wave's boards.
 //
-// Loss and both gradients of 65 536 float32 boards: 267 to 280 us, 3.9 TB/s of features and gradients (a copy reaches
-// 4.75; float32 MFMAs alone would take 384); of 32 768 bfloat16 boards 95 us.  Bound by issue: of a board's 5 600 cycles a
-// SIMD the 765 (bfloat16; float32 880) vector instructions take 3 400 and the 108 (192) MFMAs 1 700 (3 100), with two
-// waves of 220 to 254 registers a SIMD to overlap them.  The loss alone reads 65 536 float32 boards in 119 us, 4.5 TB/s.
+// Loss and both gradients of 65 536 float32 boards: 274 to 283 us, 3.9 TB/s of features and gradients (a copy reaches
+// 4.75), 322 on average from a cold start; of 32 768 bfloat16 boards 97 us.  Bound by issue: of a board's 5 600 cycles a
+// SIMD the 765 (bfloat16; float32 895) vector instructions take 3 400 and the 108 (192) MFMAs 1 700 (3 100), with two
+// waves of 220 to 256 registers a SIMD to overlap them.  The loss alone reads 65 536 float32 boards in 119 us, 4.5 TB/s.
 
 template <typename T>
 struct HeadLds {                                 // the kernel as operands, 16 bytes a lane
@@ -731,8 +734,9 @@ __global__ __launch_bounds__(512, WANT ? 2 : 3) void k_policy_loss(const T* __re
 // 4.4 TB/s (a copy reaches 4.75), 8 191 bfloat16 boards in 30 us, the loss alone of 65 536 float32 boards in 109 us.  (One
 // float32 sum a move, with the gradients added up in LDS, took 342 us: its chains of reads and writes left the memory
 // idle; LDS's own float adds take 200 cycles each and 880 us.)  A wave's boards are neighbours: it finds where its
-// lists begin by adding up the counts of all boards before its own, a byte a board beside the 8 to 16 KB that each
-// board costs, and needs no pass over them beforehand.
+// lists begin by adding up the counts of all boards before its own, and needs no pass over them beforehand: a byte a
+// board for every workgroup after it, out of the caches, 128 (gradients) to 512 (16-bit losses) a board on average beside the
+// board's own 4 to 16 KB.  At 2^20 boards it does not show: 4.7 (gradients) and 4.9 TB/s (loss, bfloat16), 5.2 (float32).
 
 template <typename T>
 struct MoveHeadLds {

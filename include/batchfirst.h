@@ -297,9 +297,12 @@ int bf_multi_policy_finish_host(bf_multi* m, const uint8_t* h_from_square, const
  * l[filter][square] = sum over channels of kernel[channel][filter] * features[channel][square]; they are never written
  * out.  Logits, softmax sums and the sums of the gradients are float32 or wider; a gradient has its input's type.
  * All pointers but bf_global_norm's and bf_clip_grad_norm's tables are device pointers on the context's GPU.  Features,
- * kernels, their gradients and workspaces need 16-byte alignment, the rest that of their elements; outputs overlap nothing.  The calls allocate nothing, read nothing back, enqueue kernels only (so they
- * can be captured into a graph) and give the same bits for the same inputs.  A workspace belongs to one call at a time:
- * calls that may overlap, or graphs whose replays may, need one each. */
+ * kernels, their gradients and workspaces need 16-byte alignment, the rest that of their elements; outputs overlap nothing.
+ * The calls allocate nothing, read nothing back, enqueue kernels only (so they can be captured into a graph) and give the
+ * same bits for the same inputs.  A workspace belongs to one call at a time: calls that may overlap, or graphs whose replays
+ * may, need one each.
+ * float32 factors take part with 22 bits and more; what adds less than 2^-37 of a board's largest product to a gradient may
+ * be lost. */
 enum { BF_TYPE_F32 = 0, BF_TYPE_BF16 = 1, BF_TYPE_F16 = 2 };
 #define BF_POLICY_VOCABULARY 4672u /* 73 filters x 64 squares */
 
@@ -340,7 +343,7 @@ int bf_global_norm(bf_ctx* ctx, const void* const* h_tensors, const size_t* h_co
                    float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* The same, and then every element times min(1, max_norm / (norm + 1e-6)), in place: a norm of infinity makes the factor
- * 0, one of NaN makes it NaN.  Tensors that overlap are refused (an element would be scaled twice). */
+ * 0 (NaN if max_norm is infinite too), one of NaN makes it NaN.  Tensors that overlap are refused (an element would be scaled twice). */
 int bf_clip_grad_norm(bf_ctx* ctx, void* const* h_tensors, const size_t* h_counts, const int* h_types, size_t n_tensors,
                       float max_norm, float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream);
 

@@ -1171,3 +1171,20 @@ def test_large_values_beside_small_factors(ctx, moves, what):
     close(got[1], ref["d_features"], tol[1], "d_features")
     close(got[2], ref["d_kernel"], tol[2], "d_kernel")
     assert torch.equal(call(ctx, d, kernel_grad=False)[1], got[1]) and torch.equal(call(ctx, d, features_grad=False)[2], got[2])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_unlisted_filters_may_hold_anything(ctx, dtype):
+    """As unlisted squares: NaN and infinities in columns of the kernel that no listed move uses."""
+    case = make(6, dtype, seed=14, moves=True, longest=20)
+    sq, fl, per = whole_lists(case, 1)
+    fl[:] = fl % 60
+    case["t"] = torch.zeros(6, dtype=torch.int64)
+    case["k"][:, 60:] = 0
+    clean = check_all(ctx, case)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        case["k"][5:9, 62:70] = bad
+        d = on_gpu(case)
+        assert torch.equal(forward(ctx, d), clean[0]), bad
+        assert all(torch.equal(a, b) for a, b in zip(call(ctx, d), clean)), bad
